@@ -51,8 +51,9 @@ SIGNATURES["ns_probe_empty"] = [_I32, _I32, _VP]
 SIGNATURES["ns_probe_linear_loop"] = [_VP] * 7 + [_I32, _I32, _VP]
 RESTYPES = {"ns_decode_attention_workspace": _SZ, "ns_w4_gptq_workspace": _SZ,
             "ns_w4_linear_workspace": _SZ, "ns_prompt_attention_workspace": _SZ,
-            "ns_w4_linear_swiglu_rows_workspace": _SZ}
-# Entry points of this package's own callers (csrc/internal_ops.h), not part of the public ABI.
+            "ns_w4_linear_swiglu_rows_workspace": _SZ, "ns_paged_attention_workspace": _SZ}
+# Entry points of this package's own callers (csrc/internal_ops.h, csrc/batch_ops.h), not part of the
+# public ABI.
 INTERNAL_SIGNATURES = {
     "ns_prompt_qkv": [_VP] * 5 + [_I32] * 6 + [_VP],
     "ns_w4_linear_rows": [_VP] * 4 + [_I32] * 4 + [_VP],
@@ -62,6 +63,11 @@ INTERNAL_SIGNATURES = {
     "ns_prompt_attention_workspace": [_I32] * 4,
     "ns_prompt_attention": [_VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _SZ, _I32, _I32, _I32, _I32,
                             _VP],
+    "ns_paged_append": [_VP, _I64] + [_VP] * 5 + [_I64, _I32, _VP, _VP, _I64, _I64, _I32, _I32, _VP]
+                       + [_I32] * 5 + [_VP],
+    "ns_paged_attention_workspace": [_I32] * 8,
+    "ns_paged_attention": [_VP, _I64, _VP, _VP, _I64, _I64, _I32, _I32, _VP, _I64, _I32, _VP, _VP, _VP,
+                           _VP, _SZ] + [_I32] * 8 + [_F32, _VP],
 }
 
 
@@ -574,6 +580,134 @@ class Kernels:
             out.data_ptr(), None if work is None else work.data_ptr(),
             0 if work is None else work.numel(), T, n_heads, Hk, pos0, self._stream())
         self._check(rc, "ns_prompt_attention")
+        return out
+
+    # ------------------------------------------------------------------ a batch over a paged cache
+    @staticmethod
+    def _batch_args(T, pages, lens, k_pages, v_pages, q_start):
+        """Checks of a batch's metadata and pools; returns them as the C entry points take them."""
+        for t, n in ((pages, "pages"), (lens, "lens"), (q_start, "q_start")):
+            if t is not None:
+                _require_gpu_tensor(t, n, torch.int32)
+        for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            _require_gpu_tensor(t, n, torch.bfloat16)
+            if t.dim() != 4 or t.stride(3) != 1 or t.stride(2) != t.shape[3]:
+                raise ValueError(f"{n} must be [n_pages, Hk, page_size, D] with contiguous heads")
+        if k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+            raise ValueError("k_pages and v_pages must be alike")
+        B = lens.shape[0]
+        if lens.dim() != 1 or not lens.is_contiguous():
+            raise ValueError("lens must be a contiguous [B] tensor")
+        if pages.dim() != 2 or pages.shape[0] != B or pages.stride(1) != 1:
+            raise ValueError("pages must be [B, width] with contiguous rows")
+        if q_start is None:
+            if T != B:
+                raise ValueError("without q_start every sequence has one token row")
+        elif q_start.dim() != 1 or q_start.shape[0] != B + 1 or not q_start.is_contiguous():
+            raise ValueError("q_start must be a contiguous [B + 1] tensor")
+        n_pages, Hk, page_size, D = k_pages.shape
+        # (the stride of a dimension of size 1 says nothing)
+        strides = (k_pages.stride(0) if n_pages > 1 else 0, k_pages.stride(1) if Hk > 1 else 0)
+        width = pages.shape[1]
+        table = (pages.data_ptr(), pages.stride(0) if B > 1 else width, width)
+        return B, Hk, D, page_size, n_pages, strides, table
+
+    def paged_append(self, qkv, bias, inv_freq, pages, lens, k_pages, v_pages, n_heads, q_start=None,
+                     out=None):
+        """The new tokens of a batch of sequences: bias add and RoPE of the fused projection output
+        qkv [T, (Hq + 2Hk) * D] (rows may be strided), k and v heads into the paged cache; returns
+        the q heads [T, Hq * D].
+
+        k_pages, v_pages [n_pages, Hk, page_size, D] (page_size a multiple of 16, heads contiguous,
+        e.g. one layer of a larger pool), pages [B, width] int32: the pages of each sequence's
+        positions 0 .. page_size - 1, page_size .. and so on. Token rows q_start[b] .. q_start[b + 1] - 1
+        (int32 [B + 1], ascending; without it one row per sequence) are sequence b's, at its last
+        positions: lens [B] int32 counts them. All of it is read on the device, so a captured graph
+        replays at any lengths. Rows past the last sequence's are left alone, tokens whose page is
+        outside the pool are not stored. Angles are position * inv_freq in float64, and a value is
+        rounded once. The reference serves one sequence at a time (qwen.py:113-122)."""
+        _require_gpu_tensor(qkv, "qkv", torch.bfloat16)
+        _require_gpu_tensor(inv_freq, "inv_freq", torch.float32)
+        if qkv.dim() != 2 or qkv.stride(1) != 1:
+            raise ValueError("qkv must be [T, (Hq + 2Hk) * D] with contiguous rows")
+        T = qkv.shape[0]
+        B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
+                                                                        q_start)
+        if qkv.shape[1] != (n_heads + 2 * Hk) * D:
+            raise ValueError("qkv must hold n_heads + 2 Hk heads of D values per row")
+        if inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be contiguous with head_dim / 2 elements")
+        if bias is not None:
+            _require_gpu_tensor(bias, "bias", torch.bfloat16)
+            if bias.numel() != qkv.shape[1] or not bias.is_contiguous():
+                raise ValueError("bias must be contiguous with one value per column of qkv")
+        if out is None:
+            out = torch.empty((T, n_heads * D), dtype=torch.bfloat16, device=qkv.device)
+        else:
+            _require_gpu_tensor(out, "out", torch.bfloat16)
+            if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
+        if T == 0 or B == 0:
+            return out
+        rc = self.lib.ns_paged_append(
+            qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
+            None if bias is None else bias.data_ptr(), inv_freq.data_ptr(),
+            None if q_start is None else q_start.data_ptr(), lens.data_ptr(), *table, k_pages.data_ptr(),
+            v_pages.data_ptr(), *strides, n_pages, page_size, out.data_ptr(), T, B, n_heads, Hk, D,
+            self._stream())
+        self._check(rc, "ns_paged_append")
+        return out
+
+    def paged_attention_workspace(self, T, B, n_heads, n_kv_heads, head_dim, max_len, ragged=False,
+                                  shared=0, device=None):
+        """A uint8 device tensor of the workspace paged_attention uses for these sizes (max_len: table
+        width * page_size; ragged: with q_start), or None. Launches that may overlap in time need
+        workspaces of their own."""
+        n = int(self.lib.ns_paged_attention_workspace(T, B, n_heads, n_kv_heads, head_dim, max_len,
+                                                      int(ragged), shared))
+        return torch.empty(n, dtype=torch.uint8, device=device or "cuda") if n else None
+
+    def paged_attention(self, q, k_pages, v_pages, pages, lens, n_heads, q_start=None, shared=0,
+                        window=0, sinks=0, scale=None, work=None, out=None):
+        """Causal grouped-query attention of a batch's new tokens over its paged cache, their own keys
+        and values included (paged_append first; pages, lens and q_start as there): q [T, Hq * D]
+        (rows may be strided), head size 64 or 128; returns [T, Hq * D] bf16.
+
+        With ``window`` a token sees the last ``window`` positions (its own among them) and the first
+        ``sinks`` ones. ``shared``: the first ``shared`` positions have the same pages in every row of
+        ``pages`` (the caller's statement; they are read through row 0); their keys and values are then
+        read once for the whole batch. A token that sees nothing gets zeros; rows past the last
+        sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be positive. ``work``: from
+        paged_attention_workspace, allocated here when it is not given. The reference has SDPA over one
+        sequence's cache (qwen.py:124-133)."""
+        _require_gpu_tensor(q, "q", torch.bfloat16)
+        if q.dim() != 2 or q.stride(1) != 1:
+            raise ValueError("q must be [T, Hq * D] with contiguous rows")
+        T = q.shape[0]
+        B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
+                                                                        q_start)
+        if q.shape[1] != n_heads * D:
+            raise ValueError("q must hold n_heads heads of D values per row")
+        if out is None:
+            out = torch.empty((T, n_heads * D), dtype=torch.bfloat16, device=q.device)
+        else:
+            _require_gpu_tensor(out, "out", torch.bfloat16)
+            if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
+        if T == 0 or B == 0:
+            return out
+        if work is None:
+            work = self.paged_attention_workspace(T, B, n_heads, Hk, D, table[2] * page_size,
+                                                  q_start is not None, shared, device=q.device)
+        else:
+            _require_gpu_tensor(work, "work", torch.uint8)
+        rc = self.lib.ns_paged_attention(
+            q.data_ptr(), q.stride(0) if T > 1 else q.shape[1], k_pages.data_ptr(), v_pages.data_ptr(),
+            *strides, n_pages, page_size, *table, lens.data_ptr(),
+            None if q_start is None else q_start.data_ptr(), out.data_ptr(),
+            None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
+            Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, self._stream())
+        self._check(rc, "ns_paged_attention")
         return out
 
     # ------------------------------------------------------------------ packed tile format
