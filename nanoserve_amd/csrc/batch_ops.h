@@ -76,6 +76,35 @@ int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, co
                        int Hq, int Hk, int D, int shared, int window, int sinks, float scale,
                        void* stream);
 
+/*
+ * Bytes of workspace ns_sample uses for these sizes, 0 for none or for sizes it rejects. Launches that
+ * may overlap in time need workspaces of their own.
+ */
+size_t ns_sample_workspace(int B, int V, int fp32);
+
+/*
+ * One token per row of logits [B] rows row_stride apart of V values (bf16, or fp32 with fp32 != 0),
+ * from a given random number u [B] in [0, 1). Per row, with l the logits, T the temperature and
+ * z_i = (l_i - max l) / T, w_i = exp(z_i):
+ *   - order the tokens by falling logit, equal ones by rising index
+ *   - keep the first top_k (all for top_k <= 0)
+ *   - of those keep the shortest beginning whose weights reach top_p of their sum (all for
+ *     top_p >= 1, at least one)
+ *   - of those keep the ones with w_i >= min_p (min_p above 1 counts as 1)
+ *   - out = the first token, by index, at which the running sum of the kept weights exceeds u times
+ *     their whole sum
+ * T <= 0: the first token of that order. NaN logits count as -inf, +inf as the largest fp32; -inf is never
+ * drawn; out = -1 where nothing is left. u below 0 (or NaN) counts as 0, u from 1 on as the last kept token.
+ * Settings per row: temps, top_ks, top_ps, min_ps [B] device arrays, each NULL for the scalar beside it.
+ * Weights are held in units of 2^-42 of the largest in 64-bit integers and summed exactly, so the token
+ * does not depend on the order of any sum.
+ * -2 for B <= 0, V <= 0, V > 2^20, row_stride < V, NULL or misaligned pointers (logits 2 or 4 bytes).
+ */
+int ns_sample(const void* logits, int fp32, long long row_stride, const float* u, const float* temps,
+              float temp, const int* top_ks, int top_k, const float* top_ps, float top_p,
+              const float* min_ps, float min_p, int* out, void* work, size_t work_bytes, int B, int V,
+              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

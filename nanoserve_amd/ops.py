@@ -51,7 +51,8 @@ SIGNATURES["ns_probe_empty"] = [_I32, _I32, _VP]
 SIGNATURES["ns_probe_linear_loop"] = [_VP] * 7 + [_I32, _I32, _VP]
 RESTYPES = {"ns_decode_attention_workspace": _SZ, "ns_w4_gptq_workspace": _SZ,
             "ns_w4_linear_workspace": _SZ, "ns_prompt_attention_workspace": _SZ,
-            "ns_w4_linear_swiglu_rows_workspace": _SZ, "ns_paged_attention_workspace": _SZ}
+            "ns_w4_linear_swiglu_rows_workspace": _SZ, "ns_paged_attention_workspace": _SZ,
+            "ns_sample_workspace": _SZ}
 # Entry points of this package's own callers (csrc/internal_ops.h, csrc/batch_ops.h), not part of the
 # public ABI.
 INTERNAL_SIGNATURES = {
@@ -68,6 +69,9 @@ INTERNAL_SIGNATURES = {
     "ns_paged_attention_workspace": [_I32] * 8,
     "ns_paged_attention": [_VP, _I64, _VP, _VP, _I64, _I64, _I32, _I32, _VP, _I64, _I32, _VP, _VP, _VP,
                            _VP, _SZ] + [_I32] * 8 + [_F32, _VP],
+    "ns_sample_workspace": [_I32] * 3,
+    "ns_sample": [_VP, _I32, _I64, _VP, _VP, _F32, _VP, _I32, _VP, _F32, _VP, _F32, _VP, _VP, _SZ, _I32,
+                  _I32, _VP],
 }
 
 
@@ -708,6 +712,66 @@ class Kernels:
             None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
             Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, self._stream())
         self._check(rc, "ns_paged_attention")
+        return out
+
+    # ------------------------------------------------------------------ the next token
+    def sample_workspace(self, B, vocab, dtype=torch.bfloat16, device=None):
+        """A uint8 device tensor of the workspace sample uses for these sizes, or None. Launches that
+        may overlap in time need workspaces of their own."""
+        n = int(self.lib.ns_sample_workspace(B, vocab, int(dtype == torch.float32)))
+        return torch.empty(n, dtype=torch.uint8, device=device or "cuda") if n else None
+
+    def sample(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, work=None, out=None):
+        """One token id per row of logits [B, vocab] (bf16 or float32, rows may be strided, vocab at
+        most 2^20) from the given random numbers u [B] float32 in [0, 1): int32 [B].
+
+        Tokens ordered by falling logit (equal ones by index): the first ``top_k`` are kept (0: all), of
+        those the shortest beginning that holds ``top_p`` of their probability (at least one), of those
+        the ones of at least ``min_p`` times the largest probability; the token is the first, by index,
+        at which the running sum of the kept probabilities exceeds u times their sum. Temperature 0:
+        the largest logit. A setting is a number or a tensor [B] (float32, top_k int32) with one for
+        each row. NaN logits are never drawn, nor is -inf; a row without any other gives -1. The same
+        arguments give the same token, eager or replayed, whatever else is in the batch. ``work``: from
+        sample_workspace, allocated here when it is not given. The reference decodes greedily
+        (qwen.py:166-177)."""
+        if not isinstance(logits, torch.Tensor):
+            raise TypeError("logits must be a torch.Tensor")
+        fp32 = logits.dtype is torch.float32
+        _require_gpu_tensor(logits, "logits", torch.float32 if fp32 else torch.bfloat16)
+        _require_gpu_tensor(u, "u", torch.float32)
+        if logits.dim() != 2 or logits.stride(1) != 1:
+            raise ValueError("logits must be [B, vocab] with contiguous rows")
+        B, V = logits.shape
+        if tuple(u.shape) != (B,) or not u.is_contiguous():
+            raise ValueError(f"u must be a contiguous [{B}] tensor")
+        args = []
+        for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                               ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+            if isinstance(t, torch.Tensor):
+                _require_gpu_tensor(t, name, dtype)
+                if tuple(t.shape) != (B,) or not t.is_contiguous():
+                    raise ValueError(f"{name} must be a number or a contiguous [{B}] tensor")
+                args += [t.data_ptr(), 0]
+            else:
+                if not t >= 0 or (name in ("top_p", "min_p") and t > 1):
+                    raise ValueError(f"{name} is out of range: {t}")
+                args += [None, min(int(t), V) if dtype is torch.int32 else t]
+        if out is None:
+            out = torch.empty(B, dtype=torch.int32, device=logits.device)
+        else:
+            _require_gpu_tensor(out, "out", torch.int32)
+            if tuple(out.shape) != (B,) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{B}] tensor")
+        if B == 0:
+            return out
+        if work is None:
+            work = self.sample_workspace(B, V, logits.dtype, device=logits.device)
+        else:
+            _require_gpu_tensor(work, "work", torch.uint8)
+        rc = self.lib.ns_sample(logits.data_ptr(), int(fp32), logits.stride(0) if B > 1 else V, u.data_ptr(),
+                                *args, out.data_ptr(), None if work is None else work.data_ptr(),
+                                0 if work is None else work.numel(), B, V, self._stream())
+        self._check(rc, "ns_sample")
         return out
 
     # ------------------------------------------------------------------ packed tile format

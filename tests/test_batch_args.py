@@ -115,3 +115,40 @@ def test_wrapper_refusals(monkeypatch):
                     (dict(q_start=torch.zeros(5, **ints)), ValueError)):
         with pytest.raises(err):
             append(**kw)
+
+
+SAMPLE = dict(x=P, fp32=0, rs=100, u=P, T=None, k=None, p=None, m=None, out=P, work=P, bytes=1 << 30, B=2, V=100)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(x=None), dict(x=P + 1), dict(x=P + 2, fp32=1), dict(rs=99), dict(u=None), dict(u=P + 2), dict(T=P + 1),
+    dict(k=P + 2), dict(p=P + 3), dict(m=P + 1), dict(out=None), dict(out=P + 2), dict(B=0), dict(V=0),
+    dict(V=(1 << 20) + 1, rs=1 << 22)], ids=str)
+def test_sample_refuses(lib, bad):
+    a = {**SAMPLE, **bad}
+    assert lib.ns_sample(a["x"], a["fp32"], a["rs"], a["u"], a["T"], 1.0, a["k"], 0, a["p"], 1.0, a["m"], 0.0,
+                         a["out"], a["work"], a["bytes"], a["B"], a["V"], None) == -2
+
+
+def test_sample_wrapper_refusals(monkeypatch):
+    k = Kernels()
+    with pytest.raises(ValueError):
+        k.sample(torch.zeros(1, 8), torch.zeros(1))
+
+    def check(t, name, dtype):
+        if t.dtype != dtype:
+            raise TypeError(name)
+
+    monkeypatch.setattr(ops, "_require_gpu_tensor", check)
+    x, u = torch.zeros(2, 8), torch.zeros(2)
+    for args, kw, err in (((x.half(), u), {}, TypeError), ((x.t(), torch.zeros(8)), {}, ValueError),
+                          ((x[0], u), {}, ValueError), ((x, torch.zeros(3)), {}, ValueError),
+                          ((x, u.double()), {}, TypeError), ((x, u), dict(temperature=-1.0), ValueError),
+                          ((x, u), dict(temperature=float("nan")), ValueError), ((x, u), dict(top_k=-1), ValueError),
+                          ((x, u), dict(top_p=1.5), ValueError), ((x, u), dict(top_p=-0.5), ValueError),
+                          ((x, u), dict(min_p=2.0), ValueError), ((x, u), dict(top_k=torch.zeros(2)), TypeError),
+                          ((x, u), dict(top_p=torch.zeros(3)), ValueError),
+                          ((x, u), dict(out=torch.zeros(2, dtype=torch.int64)), TypeError),
+                          ((x, u), dict(out=torch.zeros(3, dtype=I32)), ValueError)):
+        with pytest.raises(err):
+            k.sample(*args, **kw)
