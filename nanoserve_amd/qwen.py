@@ -516,16 +516,31 @@ class Qwen2Runner:
         return F.linear(h, self.lm_head)
 
     @torch.no_grad()
-    def generate(self, prompt_ids, n_new: int, use_graph: bool = True):
-        """Greedy decoding (reference qwen.py:166-177): returns the ``n_new`` generated ids. The
-        decode steps replay one captured graph when ``use_graph``."""
+    def generate(self, prompt_ids, n_new: int, use_graph: bool = True, temperature: float = 0.0,
+                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, u=None):
+        """Returns the ``n_new`` generated ids. The decode steps replay one captured graph when
+        ``use_graph``. Greedy at temperature 0 (reference qwen.py:166-177); at others each token is
+        drawn by ``Kernels.sample`` with these settings from the random numbers u [n_new] float32 in
+        [0, 1) (default: torch.rand)."""
         T = prompt_ids.shape[0]
+        if temperature > 0:
+            if u is None:
+                u = torch.rand(n_new, device=self.dev)
+            elif tuple(u.shape) != (n_new,):
+                raise ValueError(f"u must hold {n_new} random numbers")
+            work = self.k.sample_workspace(1, self.shape.vocab, self.logits.dtype, device=self.dev)
+
+        def token(logits, n):
+            if temperature > 0:
+                return self.k.sample(logits, u[n:n + 1], temperature, top_k, top_p, min_p, work=work)[0]
+            return logits[-1].argmax()
+
         self.alloc_cache(T + n_new)
         if use_graph and n_new > 1:
             self.capture_decode()
         # generated ids stay on the device until the end: no host synchronisation per token
         ids = torch.empty(n_new, dtype=torch.int64, device=self.dev)
-        ids[0] = self.forward(prompt_ids, 0, use_cache=True, last_only=True)[-1].argmax()
+        ids[0] = token(self.forward(prompt_ids, 0, use_cache=True, last_only=True), 0)
         for n in range(1, n_new):
-            ids[n] = self.decode(ids[n - 1], T + n - 1)[-1].argmax()
+            ids[n] = token(self.decode(ids[n - 1], T + n - 1), n)
         return ids.tolist()
