@@ -39,9 +39,20 @@ struct PagedArgs {
   float *opart, *ml;     // own keys: [cap][Hq][D] and [cap][Hq][2] (maximum, sum)
   float *shpart, *shml;  // shared keys: [splits][T][Hq][D] and [..][2]
   long long cap;
-  int Hq, Hk, R, shared, window, sinks, sh_splits, unit;
+  int Hq, Hk, R, shared, window, sinks, sh_splits, sh_grid, unit;
   float per_target;  // kv heads / workgroups aimed at
   float c;           // scale * log2(e)
+};
+
+// LDS of a workgroup: 64 KiB (D = 128: two stages of 64 rows of K and of V; D = 64: four). Separate arrays,
+// not one: a read of a stage then provably does not alias the loads in flight into another, so the
+// compiler puts no wait for those before it.
+template <int D>
+constexpr int ring_stages() {
+  return D == 128 ? 2 : 4;
+}
+struct Ring {
+  uint16_t *k[4], *v[4];
 };
 
 // The key blocks that some query of a range sees: positions k0 .. k1 - 1, of them those below `first`
@@ -82,13 +93,14 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, int b) {
   return x;
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive, over the lanes
-  const int lane = __lane_id();
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int u = __shfl_up(v, o, kWave);
-    v += lane >= o ? u : 0;
-  }
+// Inclusive prefix sums over the wave by DPP (row shifts, then row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
 }
 
@@ -105,8 +117,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
     if (base + lane < B) x = span_of<BLK, ROWS>(a, base + lane);
     total += (float)x.tiles * (float)x.blocks;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, kWave);
+  total = wave_sum(total);
   const int share = __builtin_amdgcn_readfirstlane((int)ceilf(total * a.per_target));
   const int per = max(a.unit, (share + a.unit - 1) / a.unit * a.unit);
 
@@ -139,6 +150,12 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
   return false;
 }
 
+// attn_lds_load16 for rows that one workgroup reads, once.
+__device__ __forceinline__ void lds_stream16(__amdgpu_buffer_rsrc_t r, uint16_t* dst, uint32_t voff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, voff, 0, 0,
+                                           kStreamAux);
+}
+
 // A block's loads have landed when at most n newer ones of this wave are in flight (n a multiple of 4
 // below 16).
 __device__ __forceinline__ void wait_loads(int n) {
@@ -167,22 +184,17 @@ __device__ __forceinline__ void wait_loads(int n) {
 //  * Value rows that the token does not see are not read but zero: their probability is 0, and whatever
 //    the page holds there (it may be NaN) must not reach the sum.
 template <int D>
-__global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a) {
+__device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, const Ring& lds,
+                                         float (&red)[2][kOneWaves][16]) {
   constexpr int kBlk = kOneRows * D, kChunks = D / 8, kRowsPerLoad = 64 / kChunks,
-                kLoads = kOneRows / kRowsPerLoad, kStages = D == 128 ? 2 : 4;
-  // one array per stage, so that reads of a stage do not wait for the loads into the others
-  __shared__ __align__(16) uint16_t st0[kOneWaves][2 * kBlk], st1[kOneWaves][2 * kBlk];
-  __shared__ __align__(16) uint16_t st2[kStages > 2 ? kOneWaves : 1][kStages > 2 ? 2 * kBlk : 8],
-      st3[kStages > 2 ? kOneWaves : 1][kStages > 2 ? 2 * kBlk : 8];
-  __shared__ float red_m[kOneWaves][16], red_l[kOneWaves][16];
-
+                kLoads = kOneRows / kRowsPerLoad, kStages = ring_stages<D>();
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = blockIdx.x % a.Hk, R = a.R;
+  const int R = a.R;
   int b, split;
   long long slot;
   Span sp;
-  if (!find_item<kOneRows, 0>(a, blockIdx.x / a.Hk, b, sp, split, slot)) return;
+  if (!find_item<kOneRows, 0>(a, item, b, sp, split, slot)) return;
   const bool direct = sp.splits == 1 && a.sh_splits == 0;
   if (!direct && slot + sp.splits > a.cap) return;
 
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
   auto v_swz = [](int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); };
   auto seen_key = [&](int key) { return (key < n) & (key >= k0) & ((key >= lo) | (key < first)); };
   const uint32_t lr = lane / kChunks, ch = lane % kChunks;
-  auto issue = [&](uint16_t* st, int i) {
+  auto issue = [&](uint16_t* ks, uint16_t* vs, int i) {
     if ((i & 63) == 0) refill(i);
     const int page = __builtin_amdgcn_readlane(ids, i & 63), key0 = __builtin_amdgcn_readlane(keys, i & 63);
     const bool ok = (unsigned)page < (unsigned)a.p.n_pages;
@@ -231,13 +243,12 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) {
       const int row = kRowsPerLoad * p + lr;
-      attn_lds_load16(kres, st + 512 * p, row * 2 * D + 16u * (ch ^ k_swz(row)), 0);
+      lds_stream16(kres, ks + 512 * p, row * 2 * D + 16u * (ch ^ k_swz(row)));
     }
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) {
       const int row = kRowsPerLoad * p + lr;
-      attn_lds_load16(vres, st + kBlk + 512 * p,
-                      seen_key(key0 + row) ? row * 2 * D + 16u * (ch ^ v_swz(row)) : kOut, 0);
+      lds_stream16(vres, vs + 512 * p, seen_key(key0 + row) ? row * 2 * D + 16u * (ch ^ v_swz(row)) : kOut);
     }
   };
 
@@ -246,12 +257,12 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
   for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;  // of head r16
   const int vrow = 4 * grp + (r16 >> 2);
-  auto compute = [&](const uint16_t* st, int page, int key0) {
+  auto compute = [&](const uint16_t* ks, const uint16_t* vs, int page, int key0) {
     const bool ok = (unsigned)page < (unsigned)a.p.n_pages;
     f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) {
-      const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(st + r16 * D + 8 * ((4 * s + grp) ^ k_swz(r16)));
+      const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(ks + r16 * D + 8 * ((4 * s + grp) ^ k_swz(r16)));
       sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kf),
                                                    __builtin_bit_cast(bf16x8_t, qf[s]), sc, 0, 0, 0);
     }
@@ -293,7 +304,7 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
     for (int d = 0; d < D / 16; ++d) {
       const int chunk = (2 * d + ((lane & 3) >> 1)) ^ v_swz(vrow);
       const s16x4_t vb = __builtin_bit_cast(
-          s16x4_t, lds_read_tr16(st + kBlk + vrow * D + 8 * chunk + 4 * (lane & 1)));
+          s16x4_t, lds_read_tr16(vs + vrow * D + 8 * chunk + 4 * (lane & 1)));
       o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pah, vb, o[d], 0, 0, 0);
       o[d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(pal, vb, o[d], 0, 0, 0);
     }
@@ -303,45 +314,49 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
   };
 
   int pg[kStages], k1st[kStages];  // page and first position of the blocks in flight
-  auto start = [&](auto stage, uint16_t* st, int i) {
+  auto start = [&](auto stage, int i) {
     constexpr int S = decltype(stage)::value;
-    issue(st, i);
+    issue(lds.k[S] + wv * kBlk, lds.v[S] + wv * kBlk, i);
     pg[S] = __builtin_amdgcn_readlane(ids, i & 63);
     k1st[S] = __builtin_amdgcn_readlane(keys, i & 63);
+  };
+  auto step = [&](auto stage, int i) {
+    constexpr int S = decltype(stage)::value;
+    wait_loads(2 * kLoads * min(cnt - 1 - i, kStages - 1));
+    compute(lds.k[S] + wv * kBlk, lds.v[S] + wv * kBlk, pg[S], k1st[S]);
+    if (i + kStages < cnt) start(stage, i + kStages);
   };
   using S0 = std::integral_constant<int, 0>;
   using S1 = std::integral_constant<int, 1>;
   using S2 = std::integral_constant<int, (kStages > 2 ? 2 : 0)>;
   using S3 = std::integral_constant<int, (kStages > 2 ? 3 : 0)>;
-  if (cnt > 0) start(S0{}, st0[wv], 0);
-  if (cnt > 1) start(S1{}, st1[wv], 1);
+  if (cnt > 0) start(S0{}, 0);
+  if (cnt > 1) start(S1{}, 1);
   if constexpr (kStages > 2) {
-    if (cnt > 2) start(S2{}, st2[wv], 2);
-    if (cnt > 3) start(S3{}, st3[wv], 3);
+    if (cnt > 2) start(S2{}, 2);
+    if (cnt > 3) start(S3{}, 3);
   }
-  auto step = [&](auto stage, uint16_t* st, int i) {
-    constexpr int S = decltype(stage)::value;
-    wait_loads(2 * kLoads * min(cnt - 1 - i, kStages - 1));
-    compute(st, pg[S], k1st[S]);
-    if (i + kStages < cnt) start(stage, st, i + kStages);
-  };
   for (int i = 0; i < cnt; i += kStages) {
-    step(S0{}, st0[wv], i);
-    if (i + 1 < cnt) step(S1{}, st1[wv], i + 1);
+    step(S0{}, i);
+    if (i + 1 < cnt) step(S1{}, i + 1);
     if constexpr (kStages > 2) {
-      if (i + 2 < cnt) step(S2{}, st2[wv], i + 2);
-      if (i + 3 < cnt) step(S3{}, st3[wv], i + 3);
+      if (i + 2 < cnt) step(S2{}, i + 2);
+      if (i + 3 < cnt) step(S3{}, i + 3);
     }
   }
   l += lane_xor16(l);
   l += lane_xor32(l);
 
-  // ---- merge of the waves through their (then free) first stages: [16][D] fp32 per wave
-  float* ored = reinterpret_cast<float*>(st0[wv]);
+  // ---- merge of the waves through their (then free) first stages: fp32, heads 0 .. 7 in the K half and
+  // 8 .. 15 in the V half
+  auto (&red_m) = red[0];
+  auto (&red_l) = red[1];
+  float *ok = reinterpret_cast<float*>(lds.k[0]), *ov_ = reinterpret_cast<float*>(lds.v[0]);
+  float* half = (grp < 2 ? ok : ov_) + wv * kBlk / 2 + (4 * grp & 7) * D;
 #pragma unroll
   for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) ored[(4 * grp + r) * D + 16 * d + r16] = o[d][r];
+    for (int r = 0; r < 4; ++r) half[r * D + 16 * d + r16] = o[d][r];
   if (grp == 0) {
     red_m[wv][r16] = m;
     red_l[wv][r16] = l;
@@ -357,7 +372,7 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
 #pragma unroll
     for (int k = 0; k < kOneWaves; ++k) {
       const float f = exp2f(red_m[k][hh] - mz);  // 0 for a wave without keys
-      ov = fmaf(f, reinterpret_cast<const float*>(st0[k])[i], ov);
+      ov = fmaf(f, (hh < 8 ? ok : ov_)[k * kBlk / 2 + (hh & 7) * D + d], ov);
       lt = fmaf(f, red_l[k][hh], lt);
     }
     const int h = g * R + hh;
@@ -389,14 +404,12 @@ __global__ void __launch_bounds__(kOneWaves* kWave) paged_one_kernel(PagedArgs a
 //  * A row sees positions below `hi` and from `lo` on or below `sinks`; blocks that no row of the tile
 //    sees are left out of its list, blocks that all rows see whole skip the comparisons.
 template <int D, bool kShared>
-__global__ void __launch_bounds__(256, 2) paged_tile_kernel(PagedArgs a) {
-  constexpr int kTile = kTileKeys * D, kChunks = D / 8, kRowsPerLoad = 64 / kChunks,
-                kLoads = 16 / kRowsPerLoad, kDT = D / 32;
-  __shared__ __align__(16) uint16_t ks0[kTile], ks1[kTile], vs0[kTile], vs1[kTile];
-  __shared__ int lim[4][2];
+__device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, int (&lim)[4][2]) {
+  constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad, kDT = D / 32,
+                kStages = ring_stages<D>();
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = blockIdx.x % a.Hk, R = a.R;
+  const int R = a.R;
   const int jq = lane & 31, kh = lane >> 5;
 
   int split, splits, r0, rows, k0, k1;
@@ -404,7 +417,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(PagedArgs a) {
   Span sp{};
   int b = 0;
   if constexpr (kShared) {
-    const int tiles = (a.s.T * R + kTileRows - 1) / kTileRows, item = blockIdx.x / a.Hk;
+    const int tiles = (a.s.T * R + kTileRows - 1) / kTileRows;
     split = item / tiles;
     splits = a.sh_splits;
     r0 = item % tiles * kTileRows;
@@ -413,7 +426,7 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(PagedArgs a) {
     k1 = min(a.shared, a.s.width * a.s.page_size);
   } else {
     int within;
-    if (!find_item<kTileKeys, kTileRows>(a, blockIdx.x / a.Hk, b, sp, within, slot)) return;
+    if (!find_item<kTileKeys, kTileRows>(a, item, b, sp, within, slot)) return;
     splits = sp.splits;
     split = within % splits;
     r0 = (sp.tiles - 1 - within / splits) * kTileRows;  // longest tiles first
@@ -445,26 +458,39 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(PagedArgs a) {
   const bool real = wrow + jq < rows && pos >= 0;
   const int hi = real ? min(pos + 1, k1) : 0, lo = low_limit(a, pos);
   const int first = a.window > 0 ? a.sinks : 0;
-  // limits over the wave's rows and over the tile's
-  int hi_min = real ? hi : INT_MAX, hi_max = hi, lo_min = real ? lo : INT_MAX, lo_max = real ? lo : 0;
+  // limits over the wave's rows and over the tile's: a sequence's positions rise with its rows, the rows of
+  // the whole batch need a look at each
+  int hi_min, hi_max, lo_min, lo_max, top, low;
+  if constexpr (kShared) {
+    hi_min = real ? hi : INT_MAX, hi_max = hi, lo_min = real ? lo : INT_MAX, lo_max = real ? lo : 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    hi_min = min(hi_min, __shfl_xor(hi_min, o, kWave));
-    hi_max = max(hi_max, __shfl_xor(hi_max, o, kWave));
-    lo_min = min(lo_min, __shfl_xor(lo_min, o, kWave));
-    lo_max = max(lo_max, __shfl_xor(lo_max, o, kWave));
+    for (int o = 16; o > 0; o >>= 1) {
+      hi_min = min(hi_min, __shfl_xor(hi_min, o, kWave));
+      hi_max = max(hi_max, __shfl_xor(hi_max, o, kWave));
+      lo_min = min(lo_min, __shfl_xor(lo_min, o, kWave));
+      lo_max = max(lo_max, __shfl_xor(lo_max, o, kWave));
+    }
+    hi_min = __builtin_amdgcn_readfirstlane(hi_min);
+    hi_max = __builtin_amdgcn_readfirstlane(hi_max);
+    lo_min = __builtin_amdgcn_readfirstlane(lo_min);
+    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    if (lane == 0) {
+      lim[wv][0] = hi_max;
+      lim[wv][1] = lo_min;
+    }
+    lds_sync();
+    top = __builtin_amdgcn_readfirstlane(max(max(lim[0][0], lim[1][0]), max(lim[2][0], lim[3][0])));
+    low = __builtin_amdgcn_readfirstlane(min(min(lim[0][1], lim[1][1]), min(lim[2][1], lim[3][1])));
+  } else {
+    const int p0 = sp.n - sp.nn;  // of the sequence's first new token; below 0 with more of them than positions
+    const int wfirst = p0 + min(wrow, rows - 1) / R, wlast = p0 + min(wrow + 31, rows - 1) / R;
+    hi_min = wrow + 31 < rows && wfirst >= 0 ? wfirst + 1 : 0;  // (0: some lane's row sees nothing)
+    hi_max = wrow < rows ? max(wlast + 1, 0) : 0;
+    lo_min = low_limit(a, wfirst);
+    lo_max = low_limit(a, wlast);
+    top = max(p0 + min(r0 + kTileRows - 1, rows - 1) / R + 1, 0);
+    low = low_limit(a, p0 + r0 / R);
   }
-  hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-  hi_max = __builtin_amdgcn_readfirstlane(hi_max);
-  lo_min = __builtin_amdgcn_readfirstlane(lo_min);
-  lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-  if (lane == 0) {
-    lim[wv][0] = hi_max;
-    lim[wv][1] = lo_min;
-  }
-  lds_sync();
-  const int top = __builtin_amdgcn_readfirstlane(max(max(lim[0][0], lim[1][0]), max(lim[2][0], lim[3][0])));
-  const int low = __builtin_amdgcn_readfirstlane(min(min(lim[0][1], lim[1][1]), min(lim[2][1], lim[3][1])));
   const KeyBlocks<kTileKeys> kb(k0, top, low, first);
   const int j0 = (int)((long long)kb.count() * split / splits);
   const int j1 = (int)((long long)kb.count() * (split + 1) / splits);
@@ -613,24 +639,41 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(PagedArgs a) {
       }
   };
 
-  // Block j is ready once every wave's loads of it have landed, and past the barrier nobody reads block
-  // j - 1, whose stage takes block j + 1: each wave waits for its loads of j and its reads of j - 1.
-  auto ready = [] {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+  // Block j is ready once every wave's loads of it have landed (those of up to kStages - 2 newer blocks stay
+  // in flight), and past the barrier nobody reads block j - 1, whose stage is loaded next: each wave waits for
+  // its loads of j and its reads of j - 1.
+  uint32_t gr[kStages];
+  auto fill = [&](auto stage, int j) {
+    constexpr int S = decltype(stage)::value;
+    if (j < j1) issue(lds.k[S], lds.v[S], j, gr[S]);
   };
-  uint32_t g0 = 0, g1 = 0;
-  if (j0 < j1) issue(ks0, vs0, j0, g0);
-  for (int j = j0; j < j1; j += 2) {
-    ready();
-    if (j + 1 < j1) issue(ks1, vs1, j + 1, g1);
-    compute(ks0, vs0, j, g0);
-    if (j + 1 == j1) break;
-    ready();
-    if (j + 2 < j1) issue(ks0, vs0, j + 2, g0);
-    compute(ks1, vs1, j + 1, g1);
+  auto step = [&](auto stage, auto last, int j) {
+    constexpr int S = decltype(stage)::value;
+    asm volatile("" ::: "memory");
+    wait_loads(2 * kLoads * min(j1 - 1 - j, kStages - 2));
+    lds_sync();
+    fill(last, j + kStages - 1);
+    compute(lds.k[S], lds.v[S], j, gr[S]);
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, (kStages > 2 ? 2 : 0)>;
+  using S3 = std::integral_constant<int, (kStages > 2 ? 3 : 0)>;
+  fill(S0{}, j0);
+  if constexpr (kStages > 2) {
+    fill(S1{}, j0 + 1);
+    fill(S2{}, j0 + 2);
+  }
+  for (int j = j0; j < j1; j += kStages) {
+    if constexpr (kStages == 2) {
+      step(S0{}, S1{}, j);
+      if (j + 1 < j1) step(S1{}, S0{}, j + 1);
+    } else {
+      step(S0{}, S3{}, j);
+      if (j + 1 < j1) step(S1{}, S0{}, j + 1);
+      if (j + 2 < j1) step(S2{}, S1{}, j + 2);
+      if (j + 3 < j1) step(S3{}, S2{}, j + 3);
+    }
   }
 
   l += lane_xor32(l);
@@ -662,15 +705,41 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(PagedArgs a) {
     a.rows[t] = make_int4((int)(slot + tok), sp.nn, splits, 0);
 }
 
+// The launch: workgroups of the shared keys first (kWithShared), then those of the sequences' own keys. Both in
+// one launch, since either alone leaves CUs idle.
+template <int D, bool kOne, bool kWithShared>
+__global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedArgs a) {
+  constexpr int kArr = kTileKeys * D, kFour = ring_stages<D>() > 2 ? kArr : 8;
+  __shared__ __align__(16) uint16_t k0[kArr], v0[kArr], k1[kArr], v1[kArr], k2[kFour], v2[kFour], k3[kFour], v3[kFour];
+  __shared__ float red[2][kOneWaves][16];
+  __shared__ int lim[4][2];
+  const Ring lds{{k0, k1, k2, k3}, {v0, v1, v2, v3}};
+  int id = blockIdx.x;
+  if constexpr (kWithShared) {
+    if (id < a.sh_grid) {
+      tile_body<D, true>(a, id / a.Hk, id % a.Hk, lds, lim);
+      return;
+    }
+    id -= a.sh_grid;
+  }
+  if constexpr (kOne)
+    one_body<D>(a, id / a.Hk, id % a.Hk, lds, red);
+  else
+    tile_body<D, false>(a, id / a.Hk, id % a.Hk, lds, lim);
+}
+
 // ------------------------------------------------------------------ merge of the partials
-// kWavesPer waves per (token, head); lane = D / 64 dimensions. A partial without keys has maximum -inf.
+// kWavesPer waves per (token, head), or one wave per `per` heads of a token; lane = D / 64 dimensions. A partial
+// without keys has maximum -inf.
 template <int D, int kWavesPer>
-__global__ void __launch_bounds__(256) paged_merge_kernel(PagedArgs a) {
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedArgs a, int per) {
   constexpr int V = D / 64, kBatch = 8;
   __shared__ float red_m[4], red_l[4], red_o[4][D];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = a.Hq / per;
   const long long id = (long long)blockIdx.x * (4 / kWavesPer) + wv / kWavesPer;
-  const int t = __builtin_amdgcn_readfirstlane((int)(id / a.Hq)), h = __builtin_amdgcn_readfirstlane((int)(id % a.Hq));
+  const int t = __builtin_amdgcn_readfirstlane((int)(id / groups));
+  const int h0 = __builtin_amdgcn_readfirstlane((int)(id % groups)) * per;
   const int w = wv % kWavesPer;
   bool live = t < a.s.T && (!a.s.q_start || (t >= a.s.q_start[0] && t < a.s.q_start[a.s.B]));
   int4 info = make_int4(0, 0, 0, 0);
@@ -679,6 +748,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedArgs a) {
   live = live && info.x >= 0 && info.y > 0 && info.z > 0 &&
          info.x + (long long)info.y * (info.z - 1) < a.cap && (info.z > 1 || a.sh_splits > 0);
   const int parts = live ? a.sh_splits + info.z : 0;
+  if (kWavesPer == 1 && !live) return;
+  for (int h = h0; h < h0 + per; ++h) {
   float m = -INFINITY, l = 0.f, acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
@@ -748,6 +819,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedArgs a) {
     *reinterpret_cast<uint32_t*>(op) = pack_bf16x2_rne(acc[0] * inv, acc[1] * inv);
   else
     *op = static_cast<uint16_t>(f32_to_bf16_rne(acc[0] * inv));
+  }
 }
 
 // ------------------------------------------------------------------ launch plan
@@ -773,7 +845,7 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   const int R = Hq / Hk;
   shared = std::min(shared, max_len);
   p.one = !ragged && R <= 16;
-  p.unit = p.one ? 8 : 4;  // 128 and 256 keys
+  p.unit = 4;  // 64 keys (a block per wave) and 256
   p.target = p.one ? 2 * cus : 3 * cus / 2;
   const int blk = p.one ? kOneRows : kTileKeys;
   const long long most = ((max_len + blk - 1) / blk + p.unit - 1) / p.unit;  // ranges of one sequence
@@ -784,7 +856,7 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   if (shared > 0) {
     const long long st = ((long long)T * R + kTileRows - 1) / kTileRows;
     const int blocks = (shared + kTileKeys - 1) / kTileKeys;
-    const long long want = (3 * cus / 2 + st * Hk - 1) / (st * Hk);
+    const long long want = 2 * cus / (st * Hk);
     p.sh_splits = (int)std::max(1ll, std::min<long long>(want, blocks / 4));
     p.sh_items = st * p.sh_splits;
   }
@@ -797,22 +869,23 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-template <int D>
+template <int D, bool kOne>
 void launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
-  if (p.sh_splits > 0)
-    hipLaunchKernelGGL((paged_tile_kernel<D, true>), dim3((unsigned)(p.sh_items * a.Hk)), dim3(256), 0, st, a);
-  const dim3 grid((unsigned)(p.items * a.Hk));
-  if (p.one)
-    hipLaunchKernelGGL(paged_one_kernel<D>, grid, dim3(kOneWaves * kWave), 0, st, a);
+  const dim3 grid((unsigned)(p.items * a.Hk + a.sh_grid));
+  if (a.sh_grid > 0)
+    hipLaunchKernelGGL((paged_attn_kernel<D, kOne, true>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((paged_tile_kernel<D, false>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_attn_kernel<D, kOne, false>), grid, dim3(256), 0, st, a);
   if (p.bytes == 0) return;
+  // few rows and many partials (about, if the batch's sequences are alike) take a workgroup per row; many
+  // rows, which seldom have more than one partial, a wave per token
   const long long rows = (long long)a.s.T * a.Hq;
-  const long long most = p.sh_splits + p.target / a.Hk + 1;  // partials of a row at most, about
-  if (most > 8 && rows <= 8192)
-    hipLaunchKernelGGL((paged_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a);
+  const long long most = p.sh_splits + p.target / ((long long)a.Hk * a.s.B) + 1;
+  const int per = rows > 32768 ? a.Hq : 1;
+  if (most > 16 && rows <= 8192)
+    hipLaunchKernelGGL((paged_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, 1);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, 1>), dim3((unsigned)((rows / per + 3) / 4)), dim3(256), 0, st, a, per);
 }
 
 }  // namespace
@@ -843,7 +916,7 @@ int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, co
   if (!q || !out || !ns::aligned(q, 16) || !ns::aligned(out, 16)) return -2;
   if (q_stride % 8 || q_stride < (long long)Hq * D) return -2;
   const ns::Plan p = ns::make_plan(T, B, Hq, Hk, D, max_len, q_start != nullptr, shared);
-  if (p.items * Hk >= (1ll << 31) || p.sh_items * Hk >= (1ll << 31) || p.cap >= (1ll << 31)) return -2;
+  if ((p.items + p.sh_items) * Hk >= (1ll << 31) || p.cap >= (1ll << 31)) return -2;
   if (p.bytes > 0) {
     if (!work || !ns::aligned(work, 16) || work_bytes < p.bytes) return -2;
     a.rows = static_cast<int4*>(work);
@@ -863,14 +936,15 @@ int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, co
   a.window = window;
   a.sinks = sinks;
   a.sh_splits = p.sh_splits;
+  a.sh_grid = (int)(p.sh_items * Hk);
   a.unit = p.unit;
   a.per_target = (float)Hk / (float)p.target;
   a.c = scale * 1.4426950408889634f;
   const auto st = static_cast<hipStream_t>(stream);
   if (D == 64)
-    ns::launch_paged<64>(a, p, st);
+    p.one ? ns::launch_paged<64, true>(a, p, st) : ns::launch_paged<64, false>(a, p, st);
   else
-    ns::launch_paged<128>(a, p, st);
+    p.one ? ns::launch_paged<128, true>(a, p, st) : ns::launch_paged<128, false>(a, p, st);
   return static_cast<int>(hipGetLastError());
 }
 
