@@ -216,39 +216,53 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
     }
   }
 
-  // lane i: page and first position of the wave's block 64 (i / 64) + i
+  // lane i: offset in the pools and first position of the wave's block 64 (.. / 64) + i; no page: position -1
   const int* table = a.s.table + (size_t)b * a.s.table_stride;
-  int ids = -1, keys = 0;
+  uint64_t offs = 0;
+  int keys = -1;
   auto refill = [&](int i) {
     const int v = i + lane;
-    keys = 0;
-    ids = -1;
     if (v < cnt) {
       keys = kOneRows * kb.block(j0 + wv + kOneWaves * v);
-      ids = table[keys / a.s.page_size];
+      const int id = table[keys / a.s.page_size];
+      offs = 2 * ((uint64_t)(uint32_t)id * a.p.page_stride + (uint64_t)g * a.p.head_stride +
+                  (uint64_t)(keys % a.s.page_size) * D);
+      if ((unsigned)id >= (unsigned)a.p.n_pages) keys = -1;
     }
   };
   auto k_swz = [](int row) { return D == 128 ? row & 15 : (row >> 1) & 7; };
   auto v_swz = [](int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); };
   auto seen_key = [&](int key) { return (key < n) & (key >= k0) & ((key >= lo) | (key < first)); };
-  const uint32_t lr = lane / kChunks, ch = lane % kChunks;
+  auto whole = [&](int key0) { return key0 >= k0 && key0 >= lo && key0 + kOneRows <= n; };
+  uint32_t k_off[kLoads], v_off[kLoads];  // of this lane's 16 bytes in a block
+  const int lr = lane / kChunks;
+#pragma unroll
+  for (int p = 0; p < kLoads; ++p) {
+    const int row = kRowsPerLoad * p + lr;
+    const uint32_t ch = lane % kChunks;
+    k_off[p] = row * 2 * D + 16u * (ch ^ k_swz(row));
+    v_off[p] = row * 2 * D + 16u * (ch ^ v_swz(row));
+  }
   auto issue = [&](uint16_t* ks, uint16_t* vs, int i) {
     if ((i & 63) == 0) refill(i);
-    const int page = __builtin_amdgcn_readlane(ids, i & 63), key0 = __builtin_amdgcn_readlane(keys, i & 63);
-    const bool ok = (unsigned)page < (unsigned)a.p.n_pages;
-    const size_t off = (size_t)(ok ? page : 0) * a.p.page_stride + (size_t)g * a.p.head_stride +
-                       (size_t)(key0 % a.s.page_size) * D;
-    const auto kres = __builtin_amdgcn_make_buffer_rsrc(a.p.k + off, (short)0, ok ? kBlk * 2 : 0, 0x00020000);
-    const auto vres = __builtin_amdgcn_make_buffer_rsrc(a.p.v + off, (short)0, ok ? kBlk * 2 : 0, 0x00020000);
+    const int key0 = __builtin_amdgcn_readlane(keys, i & 63);
+    const bool ok = key0 >= 0;
+    const uint64_t off = ok ? (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(offs >> 32), i & 63) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readlane((uint32_t)offs, i & 63)
+                            : 0;
+    const auto kres = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(a.p.k) + off, (short)0,
+                                                        ok ? kBlk * 2 : 0, 0x00020000);
+    const auto vres = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(a.p.v) + off, (short)0,
+                                                        ok ? kBlk * 2 : 0, 0x00020000);
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) {
-      const int row = kRowsPerLoad * p + lr;
-      lds_stream16(kres, ks + 512 * p, row * 2 * D + 16u * (ch ^ k_swz(row)));
-    }
+    for (int p = 0; p < kLoads; ++p) lds_stream16(kres, ks + 512 * p, k_off[p]);
+    if (whole(key0)) {
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) {
-      const int row = kRowsPerLoad * p + lr;
-      lds_stream16(vres, vs + 512 * p, seen_key(key0 + row) ? row * 2 * D + 16u * (ch ^ v_swz(row)) : kOut);
+      for (int p = 0; p < kLoads; ++p) lds_stream16(vres, vs + 512 * p, v_off[p]);
+    } else {
+#pragma unroll
+      for (int p = 0; p < kLoads; ++p)
+        lds_stream16(vres, vs + 512 * p, seen_key(key0 + kRowsPerLoad * p + lr) ? v_off[p] : kOut);
     }
   };
 
@@ -257,8 +271,7 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
   for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;  // of head r16
   const int vrow = 4 * grp + (r16 >> 2);
-  auto compute = [&](const uint16_t* ks, const uint16_t* vs, int page, int key0) {
-    const bool ok = (unsigned)page < (unsigned)a.p.n_pages;
+  auto compute = [&](const uint16_t* ks, const uint16_t* vs, int key0) {
     f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < D / 32; ++s) {
@@ -268,10 +281,13 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
     }
     float sr[4], bm = -INFINITY;  // head r16, keys 4 grp + r (base-2 logits)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      sr[r] = ok & seen_key(key0 + 4 * grp + r) ? sc[r] * a.c : -INFINITY;
-      bm = fmaxf(bm, sr[r]);
+    for (int r = 0; r < 4; ++r) sr[r] = sc[r] * a.c;
+    if (!whole(key0)) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sr[r] = (key0 >= 0) & seen_key(key0 + 4 * grp + r) ? sr[r] : -INFINITY;
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bm = fmaxf(bm, sr[r]);
     bm = fmaxf(bm, lane_xor16(bm));
     bm = fmaxf(bm, lane_xor32(bm));
     const float mn = fmaxf(m, bm);
@@ -313,17 +329,16 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
     asm volatile("" ::: "memory");
   };
 
-  int pg[kStages], k1st[kStages];  // page and first position of the blocks in flight
+  int at[kStages];  // first positions of the blocks in flight
   auto start = [&](auto stage, int i) {
     constexpr int S = decltype(stage)::value;
     issue(lds.k[S] + wv * kBlk, lds.v[S] + wv * kBlk, i);
-    pg[S] = __builtin_amdgcn_readlane(ids, i & 63);
-    k1st[S] = __builtin_amdgcn_readlane(keys, i & 63);
+    at[S] = __builtin_amdgcn_readlane(keys, i & 63);
   };
   auto step = [&](auto stage, int i) {
     constexpr int S = decltype(stage)::value;
     wait_loads(2 * kLoads * min(cnt - 1 - i, kStages - 1));
-    compute(lds.k[S] + wv * kBlk, lds.v[S] + wv * kBlk, pg[S], k1st[S]);
+    compute(lds.k[S] + wv * kBlk, lds.v[S] + wv * kBlk, at[S]);
     if (i + kStages < cnt) start(stage, i + kStages);
   };
   using S0 = std::integral_constant<int, 0>;
@@ -503,49 +518,57 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(qp + 16 * s);
   }
 
-  // lane i: page and row in it of 16-row group i % 4 of block j0 + 16 (.. / 16) + i / 4 of the list
+  // lane i: offset in the pools of 16-row group i % 4 of block j0 + 16 (.. / 16) + i / 4 of the list
   const int* table = a.s.table + (kShared ? 0 : (size_t)b * a.s.table_stride);
-  int ids = -1, inpage = 0;
-  uint64_t valid = 0;
+  uint64_t offs = 0, valid = 0;
   auto refill = [&](int j) {
     const int v = j + (lane >> 2);
-    ids = -1;
-    inpage = 0;
+    int id = -1;
     if (v < j1) {
       const int key = kTileKeys * kb.block(v) + 16 * (lane & 3);
-      if (key < top) {
-        ids = table[key / a.s.page_size];
-        inpage = key % a.s.page_size;
-      }
+      if (key < top) id = table[key / a.s.page_size];
+      offs = 2 * ((uint64_t)(uint32_t)id * a.p.page_stride + (uint64_t)g * a.p.head_stride +
+                  (uint64_t)(key % a.s.page_size) * D);
     }
-    if ((unsigned)ids >= (unsigned)a.p.n_pages) ids = -1;
-    valid = __ballot(ids >= 0);
+    valid = __ballot((unsigned)id < (unsigned)a.p.n_pages);
   };
   auto k_swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
   auto v_swz = [](int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; };
-  const uint32_t lr = lane / kChunks, ch = lane % kChunks;
+  uint32_t k_off[kLoads], v_off[kLoads];  // of this lane's 16 bytes in a group
+  const int lr = lane / kChunks;
+#pragma unroll
+  for (int p = 0; p < kLoads; ++p) {
+    const int r = kRowsPerLoad * p + lr;
+    const uint32_t ch = lane % kChunks;
+    k_off[p] = r * 2 * D + 16u * (ch ^ k_swz(16 * wv + r));
+    v_off[p] = r * 2 * D + 16u * (ch ^ v_swz(r));
+  }
   auto issue = [&](uint16_t* ks, uint16_t* vs, int j, uint32_t& groups) {
     const int jj = j - j0;
     if ((jj & 15) == 0) refill(j);
     const int e = 4 * (jj & 15);
     groups = (uint32_t)(valid >> e) & 15u;
-    const int page = __builtin_amdgcn_readlane(ids, e + wv), in = __builtin_amdgcn_readlane(inpage, e + wv);
+    const bool ok = (groups >> wv) & 1;
+    const uint64_t off = ok ? (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(offs >> 32), e + wv) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readlane((uint32_t)offs, e + wv)
+                            : 0;
+    const auto kres = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(a.p.k) + off, (short)0,
+                                                        ok ? 32 * D : 0, 0x00020000);
+    const auto vres = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(a.p.v) + off, (short)0,
+                                                        ok ? 32 * D : 0, 0x00020000);
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p) attn_lds_load16(kres, &ks[16 * wv * D + 512 * p], k_off[p], 0);
     const int key0 = kTileKeys * kb.block(j) + 16 * wv;
-    const size_t off = (size_t)max(page, 0) * a.p.page_stride + (size_t)g * a.p.head_stride + (size_t)in * D;
-    const int bytes = page >= 0 ? 16 * D * 2 : 0;
-    const auto kres = __builtin_amdgcn_make_buffer_rsrc(a.p.k + off, (short)0, bytes, 0x00020000);
-    const auto vres = __builtin_amdgcn_make_buffer_rsrc(a.p.v + off, (short)0, bytes, 0x00020000);
+    if (key0 >= k0 && key0 >= low && key0 + 16 <= top) {
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) {
-      const int r = 16 * wv + kRowsPerLoad * p + lr;
-      attn_lds_load16(kres, &ks[16 * wv * D + 512 * p], (r - 16 * wv) * 2 * D + 16u * (ch ^ k_swz(r)), 0);
-    }
-    // value rows that no row of the tile sees are zero, whatever the page holds
+      for (int p = 0; p < kLoads; ++p) attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], v_off[p], 0);
+    } else {  // value rows that no row of the tile sees are zero, whatever the page holds
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) {
-      const int r = kRowsPerLoad * p + lr, key = key0 + r;
-      const bool see = (key >= k0) & (key < top) & ((key >= low) | (key < first));
-      attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], see ? r * 2 * D + 16u * (ch ^ v_swz(r)) : kOut, 0);
+      for (int p = 0; p < kLoads; ++p) {
+        const int key = key0 + kRowsPerLoad * p + lr;
+        const bool see = (key >= k0) & (key < top) & ((key >= low) | (key < first));
+        attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], see ? v_off[p] : kOut, 0);
+      }
     }
   };
 
@@ -582,17 +605,27 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
                                                        __builtin_bit_cast(bf16x8_t, qf[d]), s[u], 0, 0, 0);
       }
     }
-    if (key0 + kTileKeys > hi_min || (key0 < lo_max && key0 + kTileKeys > first) || key0 < k0 || groups != 15u) {
+    // (flags from bitwise operators and one comparison: with && this compiler builds a branch per value, and
+    // some of those lost their store)
+    if (groups != 15u || (key0 < first && lo_max > 0)) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          // (one flag from bitwise operators: with && this compiler builds a branch per value, and
-          // some of those lost their store)
           const int key = key0 + 32 * u + 8 * (r >> 2) + 4 * kh + (r & 3);
           const bool see = (key < hi) & (key >= k0) & ((key >= lo) | (key < first)) &
                            (((groups >> (2 * u + (r >> 3))) & 1) != 0);
           s[u][r] = see ? s[u][r] : -INFINITY;
+        }
+    } else if (key0 + kTileKeys > hi_min || key0 < lo_max || key0 < k0) {  // positions from, .. to - 1
+      const int from = max(lo, k0);
+      const uint32_t span = (uint32_t)max(hi - from, 0);
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t at = (uint32_t)(key0 + 4 * kh - from + 32 * u + 8 * (r >> 2) + (r & 3));
+          s[u][r] = at < span ? s[u][r] : -INFINITY;
         }
     }
     float bm = s[0][0];
