@@ -111,15 +111,35 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
                                           long long& slot) {
   const int lane = __lane_id(), B = a.s.B;
   Span x{};
-  float total = 0.f;  // (every wave of every launch adds the same values in the same order)
+  float total = 0.f, tiles = 0.f;  // (every wave of the launch adds the same values in the same order)
   for (int base = 0; base < B; base += kWave) {
     x = Span{};
     if (base + lane < B) x = span_of<BLK, ROWS>(a, base + lane);
     total += (float)x.tiles * (float)x.blocks;
+    tiles += (float)x.tiles;
   }
   total = wave_sum(total);
   const int share = __builtin_amdgcn_readfirstlane((int)ceilf(total * a.per_target));
-  const int per = max(a.unit, (share + a.unit - 1) / a.unit * a.unit);
+  int per = max(a.unit, (share + a.unit - 1) / a.unit * a.unit);
+  // Sequences end inside a share: where that makes more items than workgroups aimed at, the last ones would
+  // start when the others end. Larger shares then, a few times at most, if the items can be that few at all
+  // (us without and with: 64 sequences of 1000 to 8000 positions 118.7, 110.0; 20 of 1000 to 4000 with 8 kv
+  // heads 41.9, 38.5; 200 of up to 1000, whose 800 items are more anyway, 51.6, 59.0).
+  const bool fits = B <= 4 * kWave && wave_sum(tiles) * a.per_target < 0.9f;
+#pragma unroll 1
+  for (int step = 0; step < 3 && fits; ++step) {
+    int items = 0;
+    for (int base = 0; base < B; base += kWave) {
+      if (B > kWave) {
+        x = Span{};
+        if (base + lane < B) x = span_of<BLK, ROWS>(a, base + lane);
+      }
+      items += x.nn > 0 ? x.tiles * max(1, (x.blocks + per - 1) / per) : 0;
+    }
+    const float over = (float)__builtin_amdgcn_readlane(wave_scan(items), kWave - 1) * a.per_target;
+    if (over <= 1.f) break;
+    per = ((int)((float)per * fminf(over, 2.f)) / a.unit + 1) * a.unit;
+  }
 
   int seen = 0;
   slot = 0;
@@ -889,7 +909,9 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   if (shared > 0) {
     const long long st = ((long long)T * R + kTileRows - 1) / kTileRows;
     const int blocks = (shared + kTileKeys - 1) / kTileKeys;
-    const long long want = 2 * cus / (st * Hk);
+    // One workgroup per CU, which leaves the other half of its LDS to the sequences' own keys. us for one, one and
+    // a half, two and three: 96 sequences (194 tokens) behind 16384 99.6, 108.8, 116.5, 126.8.
+    const long long want = cus / (st * Hk);
     p.sh_splits = (int)std::max(1ll, std::min<long long>(want, blocks / 4));
     p.sh_items = st * p.sh_splits;
   }
