@@ -126,6 +126,21 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return pa < pb + b.nbytes and pb < pa + a.nbytes
 
 
+def _one_device(**tensors) -> None:
+    """Raises unless the tensors (None: absent) are all on the current device, whose stream is launched on."""
+    here = _current_device()
+    for n, t in tensors.items():
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"{n} is on device {t.get_device()}, the current one is {here}")
+
+
+def _apart(out: torch.Tensor, t: torch.Tensor, name: str) -> None:
+    """Raises if the contiguous out shares memory with t, whose last dimension is contiguous."""
+    a, b = out.data_ptr(), t.data_ptr()
+    if out.numel() and t.numel() and a < b + 2 * ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) and b < a + out.nbytes:
+        raise ValueError(f"out must not overlap {name}")
+
+
 class Kernels:
     """W4A16 kernels through the C ABI. ``path`` defaults to the in-tree library."""
 
@@ -645,12 +660,15 @@ class Kernels:
             _require_gpu_tensor(bias, "bias", torch.bfloat16)
             if bias.numel() != qkv.shape[1] or not bias.is_contiguous():
                 raise ValueError("bias must be contiguous with one value per column of qkv")
+        _one_device(qkv=qkv, bias=bias, inv_freq=inv_freq, pages=pages, lens=lens, k_pages=k_pages,
+                    v_pages=v_pages, q_start=q_start, out=out)
         if out is None:
             out = torch.empty((T, n_heads * D), dtype=torch.bfloat16, device=qkv.device)
         else:
             _require_gpu_tensor(out, "out", torch.bfloat16)
             if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
+            _apart(out, qkv, "qkv")
         if T == 0 or B == 0:
             return out
         rc = self.lib.ns_paged_append(
@@ -692,12 +710,15 @@ class Kernels:
                                                                         q_start)
         if q.shape[1] != n_heads * D:
             raise ValueError("q must hold n_heads heads of D values per row")
+        _one_device(q=q, k_pages=k_pages, v_pages=v_pages, pages=pages, lens=lens, q_start=q_start, work=work,
+                    out=out)
         if out is None:
             out = torch.empty((T, n_heads * D), dtype=torch.bfloat16, device=q.device)
         else:
             _require_gpu_tensor(out, "out", torch.bfloat16)
             if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
+            _apart(out, q, "q")
         if T == 0 or B == 0:
             return out
         if work is None:
@@ -723,7 +744,7 @@ class Kernels:
 
     def sample(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, work=None, out=None):
         """One token id per row of logits [B, vocab] (bf16 or float32, rows may be strided, vocab at
-        most 2^20) from the given random numbers u [B] float32 in [0, 1): int32 [B].
+        most 2^20, at most 65535 rows) from the given random numbers u [B] float32 in [0, 1): int32 [B].
 
         Tokens ordered by falling logit (equal ones by index): the first ``top_k`` are kept (0: all), of
         those the shortest beginning that holds ``top_p`` of their probability (at least one), of those
@@ -744,18 +765,20 @@ class Kernels:
         B, V = logits.shape
         if tuple(u.shape) != (B,) or not u.is_contiguous():
             raise ValueError(f"u must be a contiguous [{B}] tensor")
-        args = []
+        args, tensors = [], {}
         for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                                ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
             if isinstance(t, torch.Tensor):
                 _require_gpu_tensor(t, name, dtype)
                 if tuple(t.shape) != (B,) or not t.is_contiguous():
                     raise ValueError(f"{name} must be a number or a contiguous [{B}] tensor")
+                tensors[name] = t
                 args += [t.data_ptr(), 0]
             else:
                 if not t >= 0 or (name in ("top_p", "min_p") and t > 1):
                     raise ValueError(f"{name} is out of range: {t}")
                 args += [None, min(int(t), V) if dtype is torch.int32 else t]
+        _one_device(logits=logits, u=u, work=work, out=out, **tensors)
         if out is None:
             out = torch.empty(B, dtype=torch.int32, device=logits.device)
         else:

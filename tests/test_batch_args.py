@@ -56,9 +56,9 @@ def test_paged_attention_workspace_sizes(lib):
     def size(T=4, B=4, Hq=28, Hk=4, D=128, max_len=4096, ragged=0, shared=0):
         return lib.ns_paged_attention_workspace(T, B, Hq, Hk, D, max_len, ragged, shared)
 
-    # nothing to merge: no key range of 128 rows (single tokens) or 256 (prompts) is ever split
-    assert size(max_len=128) == 0 and size(max_len=256, ragged=1) == 0
-    assert size() > 0 and size(shared=1) > 0 and size(max_len=128, shared=1) > 0
+    # nothing to merge: no key range of 64 rows (single tokens) or 256 (prompts) is ever split
+    assert size(max_len=64) == 0 and size(max_len=256, ragged=1) == 0
+    assert size() > 0 and size(shared=1) > 0 and size(max_len=64, shared=1) > 0
     # a table far wider than the batch's lengths does not grow it: the GPU's workgroups bound the parts
     assert size(max_len=1 << 29) == size(max_len=1 << 20) < 64 << 20
     assert size(D=96) == size(Hq=6) == size(T=0) == size(max_len=0) == size(shared=-1) == 0
@@ -81,11 +81,14 @@ def test_wrapper_refusals(monkeypatch):
             raise TypeError(name)
 
     monkeypatch.setattr(ops, "_require_gpu_tensor", check)
+    monkeypatch.setattr(ops, "_current_device", lambda: -1)  # what CPU tensors say
+    monkeypatch.setattr(Kernels, "_stream", staticmethod(lambda: 0))
 
     def attend(q=torch.zeros(3, 512, dtype=BF16), kp=_pool(), vp=_pool(), pages=torch.zeros(3, 4, **ints),
                lens=torch.zeros(3, **ints), heads=4, **kw):
         return k.paged_attention(q, kp, vp, pages, lens, heads, **kw)
 
+    buf = torch.zeros(4, 4096, dtype=BF16)
     for kw, err in ((dict(q=torch.zeros(3, 512)), TypeError), (dict(q=torch.zeros(512, 3, dtype=BF16).t()), ValueError),
                     (dict(heads=3), ValueError), (dict(q=torch.zeros(4, 512, dtype=BF16)), ValueError),
                     (dict(kp=_pool(dtype=torch.float16)), TypeError), (dict(vp=_pool(shape=(8, 2, 32, 128))), ValueError),
@@ -97,10 +100,11 @@ def test_wrapper_refusals(monkeypatch):
                     (dict(lens=torch.zeros(6, **ints)[::2]), ValueError),
                     (dict(q_start=torch.zeros(3, **ints)), ValueError),
                     (dict(out=torch.zeros(3, 256, dtype=BF16)), ValueError),
+                    (dict(q=buf[0, :1536].view(3, 512), out=buf[0, 512:2048].view(3, 512)), ValueError),
+                    (dict(q=buf[:3, :512], out=buf[2, 500:2036].view(3, 512)), ValueError),
                     (dict(work=torch.zeros(9)), TypeError), (dict(window=-2), RuntimeError),
                     (dict(scale=0.0), RuntimeError)):
         if err is RuntimeError:
-            monkeypatch.setattr(Kernels, "_stream", staticmethod(lambda: 0))
             kw["work"] = torch.zeros(1 << 20, dtype=torch.uint8)
         with pytest.raises(err):
             attend(**kw)
@@ -112,9 +116,17 @@ def test_wrapper_refusals(monkeypatch):
     for kw, err in ((dict(qkv=torch.zeros(3, 1024)), TypeError), (dict(qkv=torch.zeros(3, 512, dtype=BF16)), ValueError),
                     (dict(bias=torch.zeros(512, dtype=BF16)), ValueError), (dict(inv=torch.zeros(32)), ValueError),
                     (dict(inv=torch.zeros(64).half()), TypeError), (dict(out=torch.zeros(3, 1024, dtype=BF16)), ValueError),
+                    (dict(qkv=buf[:3, :1024], out=buf[2, 1000:2536].view(3, 512)), ValueError),
                     (dict(q_start=torch.zeros(5, **ints)), ValueError)):
         with pytest.raises(err):
             append(**kw)
+    # tensors of another device than the current one, whose stream the launch would go to
+    monkeypatch.setattr(ops, "_current_device", lambda: 0)
+    for call in (attend, append):
+        with pytest.raises(ValueError, match="current"):
+            call()
+    with pytest.raises(ValueError, match="current"):
+        k.sample(torch.zeros(2, 8), torch.zeros(2))
 
 
 SAMPLE = dict(x=P, fp32=0, rs=100, u=P, T=None, k=None, p=None, m=None, out=P, work=P, bytes=1 << 30, B=2, V=100)
@@ -140,6 +152,7 @@ def test_sample_wrapper_refusals(monkeypatch):
             raise TypeError(name)
 
     monkeypatch.setattr(ops, "_require_gpu_tensor", check)
+    monkeypatch.setattr(ops, "_current_device", lambda: -1)
     x, u = torch.zeros(2, 8), torch.zeros(2)
     for args, kw, err in (((x.half(), u), {}, TypeError), ((x.t(), torch.zeros(8)), {}, ValueError),
                           ((x[0], u), {}, ValueError), ((x, torch.zeros(3)), {}, ValueError),
