@@ -6,12 +6,13 @@
 // never sorted. It is read up to three times, by several workgroups per row, in launches of their own:
 //   max   the largest logit, and that of every tile of 512
 //   hist  a histogram, linear in the logit, of counts for top-k and of weights for top-p: 2048 bins over
-//         the logits whose weight is not zero. The cut lies in one bin.
-//   scan  all tokens down to that bin into a list, if they fit; else the weights of the bins above it, per
-//         tile, and the tokens of that bin into the list
+//         the logits whose weight is not zero. The cut lies in one bin. Not for a top-k of at most as many
+//         tokens as there are tiles: its tokens are not below the k-th largest tile maximum.
+//   scan  all tokens down to that bin or maximum into a list, if they fit; else the weights of the bins
+//         above it, per tile, and the tokens of that bin into the list
 //   end   (one workgroup per row) the list sorted in LDS and cut exactly; the draw, from the list or from
 //         the tiles' sums and then within one tile
-// hist is left out where nothing cuts by count or sum. top-p of a top-k longer than the list takes scan and
+// hist is left out where no row needs it. top-p of a top-k longer than the list takes scan and
 // end twice. hist and scan skip tiles whose maximum does not matter to them. A bin with more tokens than
 // the list holds (flat rows, rows of few values) is cut by `end` alone, digit by digit of the key.
 //  * Launches, each with little code, and not one kernel with a counter that finds a row's last workgroup:
@@ -52,11 +53,16 @@ enum Todo { kFirst, kDone, kSum, kToList, kTopK, kTopP, kSlow };
 struct RowState {
   int todo;
   uint32_t cut;
+  float from;      // kToList: the least logit of the list
   uint32_t above;  // kTopK: tokens in higher bins
-  uint32_t pad;
   uint64_t total;  // kToList: the weights that top-p refers to (0: those of the list's first top_k)
   uint64_t need;   // kTopP: what the weights of the bin's first tokens have to reach
 };
+
+// Whether the tiles' maxima bound this top-k (each thread ranks up to two of them).
+__host__ __device__ inline bool tiles_bound(int top_k, int tiles) {
+  return top_k <= tiles && tiles <= 2 * kThreads && top_k <= kList;
+}
 
 struct SampleArgs {
   const void* logits;
@@ -266,7 +272,7 @@ __device__ __forceinline__ void each_tile(const Row<E>& row, const float* tile_m
 struct Settings {
   float T, top_p, min_p, u;
   int top_k;
-  bool k_on, p_on, m_on, greedy, weighted;
+  bool k_on, p_on, m_on, greedy, weighted, by_tiles;
   float top, bins_per, low;  // logits below `low` weigh nothing
   uint32_t min_key;
   Weight weight;
@@ -282,6 +288,7 @@ struct Settings {
     m_on = min_p > 0.f;
     greedy = !(T > 0.f) || top_k == 1 || top_p <= 0.f;
     weighted = p_on && (!k_on || top_k > kList);  // else the list has all weights that top-p needs
+    by_tiles = k_on && tiles_bound(top_k, a.tiles);
     const int lane = threadIdx.x & 63;
     top = wave_max(lane < a.parts ? a.part_max[r * kMaxParts + lane] : -INFINITY);
     if (top == -INFINITY) greedy = true;
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_hist_kernel(SampleArgs a) 
   __shared__ uint32_t counts[kBins];
   const int r = blockIdx.y, tid = threadIdx.x;
   const Settings c(a, r);
-  if (c.greedy || !(c.k_on || c.p_on)) return;
+  if (c.greedy || c.by_tiles || !(c.k_on || c.p_on)) return;
   const Row<E> row{static_cast<const E*>(a.logits) + (size_t)r * a.row_stride, a.V};
   int t0, t1;
   part_tiles(a, blockIdx.x, t0, t1);
@@ -463,6 +470,7 @@ __device__ __forceinline__ void cut_by_weight(const Settings& c, const uint64_t*
   for (int i = threadIdx.x; i <= (int)st.cut; i += kThreads) some += counts[i];
   block_exclusive<uint32_t>(some, n, s.red32);
   st.total = total;
+  st.from = c.low;
   st.need = need - done;
   st.todo = n <= kShort ? kToList : counts[st.cut] <= kList ? kTopP : kSlow;
 }
@@ -474,6 +482,46 @@ __device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Set
   RowState st{};
   if (c.greedy || !(c.k_on || c.p_on)) {
     st.todo = c.greedy ? kDone : kSum;
+    return st;
+  }
+  st.from = c.low;
+  if (c.by_tiles) {  // the top_k-th largest maximum: the least of those with fewer than top_k above them
+    float* maxima = reinterpret_cast<float*>(counts);
+    const float* tile_max = a.tile_max + (size_t)r * a.tiles;
+    const int quads = (a.tiles + 3) / 4;
+    for (int i = tid; i < 4 * quads; i += kThreads) maxima[i] = i < a.tiles ? tile_max[i] : -INFINITY;
+    __syncthreads();
+    const float v0 = maxima[min(tid, a.tiles - 1)], v1 = maxima[min(tid + kThreads, a.tiles - 1)];
+    int above0 = 0, above1 = 0;
+    if (a.tiles <= kThreads) {
+#pragma unroll 8
+      for (int q = 0; q < quads; ++q) {
+        const f32x4_t m = reinterpret_cast<const f32x4_t*>(maxima)[q];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) above0 += m[e] > v0;
+      }
+      above1 = c.top_k;
+    } else {
+#pragma unroll 4
+      for (int q = 0; q < quads; ++q) {
+        const f32x4_t m = reinterpret_cast<const f32x4_t*>(maxima)[q];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          above0 += m[e] > v0;
+          above1 += m[e] > v1;
+        }
+      }
+    }
+    float least = fminf(above0 < c.top_k ? v0 : INFINITY, above1 < c.top_k ? v1 : INFINITY);
+    least = -wave_max(-least);
+    if ((tid & 63) == 0) s.red32[tid >> 6] = __float_as_uint(least);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRowWaves; ++k) least = fminf(least, __uint_as_float(s.red32[k]));
+    __syncthreads();
+    st.todo = kToList;
+    st.cut = kBins - 1;
+    st.from = fmaxf(least, c.low);
     return st;
   }
   uint32_t some = 0, n;
@@ -500,7 +548,7 @@ __device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Set
 template <typename E>
 __global__ void __launch_bounds__(kThreads, 4) sample_scan_kernel(SampleArgs a) {
   __shared__ uint64_t weights[kBins];  // then the list
-  __shared__ uint32_t counts[kBins];
+  __shared__ __align__(16) uint32_t counts[kBins];
   __shared__ Scratch s;
   __shared__ uint32_t n, base;
   static_assert(kList <= kBins, "the list takes the histogram's place");
@@ -530,11 +578,12 @@ __global__ void __launch_bounds__(kThreads, 4) sample_scan_kernel(SampleArgs a) 
     if (at < kList) list[at] = (uint64_t)~key_of(x) << 32 | (uint32_t)index;
   };
   if (st.todo == kToList) {
-    each_tile<4>(row, tile_max, t0, t1, [&](float m) { return m >= low && c.bin(m) <= cut; },
+    const float from = st.from;
+    each_tile<4>(row, tile_max, t0, t1, [&](float m) { return m >= from && c.bin(m) <= cut; },
                  [&](int, int i, const float (&x)[8]) {
 #pragma unroll
                    for (int e = 0; e < 8; ++e)
-                     if (x[e] >= low && c.bin(x[e]) <= cut) put(x[e], i + e);
+                     if (x[e] >= from && c.bin(x[e]) <= cut) put(x[e], i + e);
                  }, [](int) {});
   } else {
     c.set_min_key();
@@ -569,7 +618,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_scan_kernel(SampleArgs a) 
                  }, none);
   }
   __syncthreads();
-  const uint32_t mine = min(n, (uint32_t)kList);
+  // (a list by tiles may overflow, where many tokens are level: its count says so)
+  const uint32_t mine = n;
   if (mine == 0) return;
   if (tid == 0) base = atomicAdd(&a.list_n[2 * r + a.round], mine);
   __syncthreads();
@@ -832,11 +882,11 @@ __global__ void __launch_bounds__(kThreads) sample_end_kernel(SampleArgs a) {
     c.set_min_key();
     uint32_t n = 0;
     if (st.todo != kSum && st.todo != kSlow) {
-      n = min(a.list_n[2 * r + a.round], (uint32_t)kList);
-      for (uint32_t i = tid; i < n; i += kThreads) s.list[i] = a.list[((size_t)r * 2 + a.round) * kList + i];
+      n = a.list_n[2 * r + a.round];
+      for (uint32_t i = tid; i < n && n <= kList; i += kThreads) s.list[i] = a.list[((size_t)r * 2 + a.round) * kList + i];
       __syncthreads();
     }
-    if (st.todo == kSlow) {
+    if (st.todo == kSlow || n > kList) {
       slow_row(row, tile_max, a.tiles, c, s, out);
     } else {
       // the exact cut in the list: its tokens in order, as many as top-k has left or top-p needs
@@ -889,7 +939,24 @@ __global__ void __launch_bounds__(kThreads) sample_end_kernel(SampleArgs a) {
         tau = entry_key(s.list[keep - 1]);
         end = (uint32_t)s.list[keep - 1] + 1;
       }
-      if (more.todo == kDone) {
+      if (st.todo == kToList && keep <= 2 * kWave) {
+        // few tokens: each adds up those up to its index
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (kPer * tid + e < keep) s.weights[kPer * tid + e] = entry_key(s.list[kPer * tid + e]) >= c.min_key ? w[e] : 0;
+        __syncthreads();
+        if (tid < (int)keep) {
+          const uint32_t index = (uint32_t)s.list[tid];
+          uint64_t upto = 0, whole = 0;
+          for (uint32_t j = 0; j < keep; ++j) {
+            const uint64_t v = s.weights[j];
+            whole += v;
+            upto += (uint32_t)s.list[j] <= index ? v : 0;
+          }
+          const uint64_t v = s.weights[tid];
+          if (pick_here(upto - v, v, c.draw(whole))) *out = (int)index;
+        }
+      } else if (more.todo == kDone) {
         for (int t = tid; t < a.tiles; t += kThreads)
           s.weights[t] = st.todo == kToList ? 0 : a.tile_w[(size_t)r * a.tiles + t];
         __syncthreads();
@@ -936,7 +1003,8 @@ void launch_sample(SampleArgs a, int B, hipStream_t st) {
   const bool greedy = !a.temps && !(a.temp > 0.f);
   const dim3 grid(a.parts, B), block(kThreads);
   hipLaunchKernelGGL(sample_max_kernel<E>, grid, block, 0, st, a);
-  if ((k || p) && !greedy) hipLaunchKernelGGL(sample_hist_kernel<E>, grid, block, 0, st, a);
+  const bool by_tiles = k && !a.top_ks && tiles_bound(a.top_k, a.tiles);
+  if ((k || p) && !greedy && !by_tiles) hipLaunchKernelGGL(sample_hist_kernel<E>, grid, block, 0, st, a);
   const int rounds = k && p && (a.top_ks || a.top_k > kList) ? 2 : 1;
   for (a.round = 0; a.round < rounds; ++a.round) {
     if (!greedy) hipLaunchKernelGGL(sample_scan_kernel<E>, grid, block, 0, st, a);

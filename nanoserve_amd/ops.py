@@ -126,12 +126,21 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return pa < pb + b.nbytes and pb < pa + a.nbytes
 
 
-def _one_device(**tensors) -> None:
-    """Raises unless the tensors (None: absent) are all on the current device, whose stream is launched on."""
+def _require_here(t: torch.Tensor, name: str, dtype: torch.dtype, here: int) -> None:
+    """_require_gpu_tensor, and that t is on the current device ``here``, whose stream is launched on."""
+    if type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == here:
+        return
+    _require_gpu_tensor(t, name, dtype)
+    if t.get_device() != here:
+        raise ValueError(f"{name} is on device {t.get_device()}, the current one is {here}")
+
+
+def _device_of(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    """_require_gpu_tensor of a call's first tensor; returns the current device, which it must be on."""
+    _require_gpu_tensor(t, name, dtype)
     here = _current_device()
-    for n, t in tensors.items():
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"{n} is on device {t.get_device()}, the current one is {here}")
+    _require_here(t, name, dtype, here)
+    return here
 
 
 def _apart(out: torch.Tensor, t: torch.Tensor, name: str) -> None:
@@ -603,33 +612,35 @@ class Kernels:
 
     # ------------------------------------------------------------------ a batch over a paged cache
     @staticmethod
-    def _batch_args(T, pages, lens, k_pages, v_pages, q_start):
+    def _batch_args(T, pages, lens, k_pages, v_pages, q_start, here):
         """Checks of a batch's metadata and pools; returns them as the C entry points take them."""
-        for t, n in ((pages, "pages"), (lens, "lens"), (q_start, "q_start")):
-            if t is not None:
-                _require_gpu_tensor(t, n, torch.int32)
-        for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-            _require_gpu_tensor(t, n, torch.bfloat16)
-            if t.dim() != 4 or t.stride(3) != 1 or t.stride(2) != t.shape[3]:
-                raise ValueError(f"{n} must be [n_pages, Hk, page_size, D] with contiguous heads")
-        if k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        _require_here(pages, "pages", torch.int32, here)
+        _require_here(lens, "lens", torch.int32, here)
+        _require_here(k_pages, "k_pages", torch.bfloat16, here)
+        _require_here(v_pages, "v_pages", torch.bfloat16, here)
+        shape, strides = k_pages.shape, k_pages.stride()
+        if len(shape) != 4 or strides[3] != 1 or strides[2] != shape[3]:
+            raise ValueError("k_pages must be [n_pages, Hk, page_size, D] with contiguous heads")
+        if v_pages.shape != shape or v_pages.stride() != strides:
             raise ValueError("k_pages and v_pages must be alike")
-        B = lens.shape[0]
         if lens.dim() != 1 or not lens.is_contiguous():
             raise ValueError("lens must be a contiguous [B] tensor")
+        B = lens.shape[0]
         if pages.dim() != 2 or pages.shape[0] != B or pages.stride(1) != 1:
             raise ValueError("pages must be [B, width] with contiguous rows")
         if q_start is None:
             if T != B:
                 raise ValueError("without q_start every sequence has one token row")
-        elif q_start.dim() != 1 or q_start.shape[0] != B + 1 or not q_start.is_contiguous():
-            raise ValueError("q_start must be a contiguous [B + 1] tensor")
-        n_pages, Hk, page_size, D = k_pages.shape
-        # (the stride of a dimension of size 1 says nothing)
-        strides = (k_pages.stride(0) if n_pages > 1 else 0, k_pages.stride(1) if Hk > 1 else 0)
+        else:
+            _require_here(q_start, "q_start", torch.int32, here)
+            if q_start.dim() != 1 or q_start.shape[0] != B + 1 or not q_start.is_contiguous():
+                raise ValueError("q_start must be a contiguous [B + 1] tensor")
+        n_pages, Hk, page_size, D = shape
         width = pages.shape[1]
-        table = (pages.data_ptr(), pages.stride(0) if B > 1 else width, width)
-        return B, Hk, D, page_size, n_pages, strides, table
+        # (the stride of a dimension of size 1 says nothing)
+        return (B, Hk, D, page_size, n_pages,
+                (strides[0] if n_pages > 1 else 0, strides[1] if Hk > 1 else 0),
+                (pages.data_ptr(), pages.stride(0) if B > 1 else width, width))
 
     def paged_append(self, qkv, bias, inv_freq, pages, lens, k_pages, v_pages, n_heads, q_start=None,
                      out=None):
@@ -645,38 +656,36 @@ class Kernels:
         replays at any lengths. Rows past the last sequence's are left alone, tokens whose page is
         outside the pool are not stored. Angles are position * inv_freq in float64, and a value is
         rounded once. The reference serves one sequence at a time (qwen.py:113-122)."""
-        _require_gpu_tensor(qkv, "qkv", torch.bfloat16)
-        _require_gpu_tensor(inv_freq, "inv_freq", torch.float32)
+        here = _device_of(qkv, "qkv", torch.bfloat16)
+        _require_here(inv_freq, "inv_freq", torch.float32, here)
         if qkv.dim() != 2 or qkv.stride(1) != 1:
             raise ValueError("qkv must be [T, (Hq + 2Hk) * D] with contiguous rows")
-        T = qkv.shape[0]
+        T, columns = qkv.shape
         B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
-                                                                        q_start)
-        if qkv.shape[1] != (n_heads + 2 * Hk) * D:
+                                                                        q_start, here)
+        if columns != (n_heads + 2 * Hk) * D:
             raise ValueError("qkv must hold n_heads + 2 Hk heads of D values per row")
         if inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
             raise ValueError("inv_freq must be contiguous with head_dim / 2 elements")
         if bias is not None:
-            _require_gpu_tensor(bias, "bias", torch.bfloat16)
-            if bias.numel() != qkv.shape[1] or not bias.is_contiguous():
+            _require_here(bias, "bias", torch.bfloat16, here)
+            if bias.numel() != columns or not bias.is_contiguous():
                 raise ValueError("bias must be contiguous with one value per column of qkv")
-        _one_device(qkv=qkv, bias=bias, inv_freq=inv_freq, pages=pages, lens=lens, k_pages=k_pages,
-                    v_pages=v_pages, q_start=q_start, out=out)
         if out is None:
-            out = torch.empty((T, n_heads * D), dtype=torch.bfloat16, device=qkv.device)
+            out = qkv.new_empty((T, n_heads * D))
         else:
-            _require_gpu_tensor(out, "out", torch.bfloat16)
+            _require_here(out, "out", torch.bfloat16, here)
             if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
             _apart(out, qkv, "qkv")
         if T == 0 or B == 0:
             return out
         rc = self.lib.ns_paged_append(
-            qkv.data_ptr(), qkv.stride(0) if T > 1 else qkv.shape[1],
+            qkv.data_ptr(), qkv.stride(0) if T > 1 else columns,
             None if bias is None else bias.data_ptr(), inv_freq.data_ptr(),
             None if q_start is None else q_start.data_ptr(), lens.data_ptr(), *table, k_pages.data_ptr(),
             v_pages.data_ptr(), *strides, n_pages, page_size, out.data_ptr(), T, B, n_heads, Hk, D,
-            self._stream())
+            _raw_stream(here))
         self._check(rc, "ns_paged_append")
         return out
 
@@ -702,22 +711,20 @@ class Kernels:
         sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be positive. ``work``: from
         paged_attention_workspace, allocated here when it is not given. The reference has SDPA over one
         sequence's cache (qwen.py:124-133)."""
-        _require_gpu_tensor(q, "q", torch.bfloat16)
+        here = _device_of(q, "q", torch.bfloat16)
         if q.dim() != 2 or q.stride(1) != 1:
             raise ValueError("q must be [T, Hq * D] with contiguous rows")
-        T = q.shape[0]
+        T, columns = q.shape
         B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
-                                                                        q_start)
-        if q.shape[1] != n_heads * D:
+                                                                        q_start, here)
+        if columns != n_heads * D:
             raise ValueError("q must hold n_heads heads of D values per row")
-        _one_device(q=q, k_pages=k_pages, v_pages=v_pages, pages=pages, lens=lens, q_start=q_start, work=work,
-                    out=out)
         if out is None:
-            out = torch.empty((T, n_heads * D), dtype=torch.bfloat16, device=q.device)
+            out = q.new_empty((T, columns))
         else:
-            _require_gpu_tensor(out, "out", torch.bfloat16)
-            if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
-                raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
+            _require_here(out, "out", torch.bfloat16, here)
+            if tuple(out.shape) != (T, columns) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{T}, {columns}] tensor")
             _apart(out, q, "q")
         if T == 0 or B == 0:
             return out
@@ -725,13 +732,13 @@ class Kernels:
             work = self.paged_attention_workspace(T, B, n_heads, Hk, D, table[2] * page_size,
                                                   q_start is not None, shared, device=q.device)
         else:
-            _require_gpu_tensor(work, "work", torch.uint8)
+            _require_here(work, "work", torch.uint8, here)
         rc = self.lib.ns_paged_attention(
-            q.data_ptr(), q.stride(0) if T > 1 else q.shape[1], k_pages.data_ptr(), v_pages.data_ptr(),
+            q.data_ptr(), q.stride(0) if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
             *strides, n_pages, page_size, *table, lens.data_ptr(),
             None if q_start is None else q_start.data_ptr(), out.data_ptr(),
             None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
-            Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, self._stream())
+            Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
         self._check(rc, "ns_paged_attention")
         return out
 
@@ -758,31 +765,29 @@ class Kernels:
         if not isinstance(logits, torch.Tensor):
             raise TypeError("logits must be a torch.Tensor")
         fp32 = logits.dtype is torch.float32
-        _require_gpu_tensor(logits, "logits", torch.float32 if fp32 else torch.bfloat16)
-        _require_gpu_tensor(u, "u", torch.float32)
+        here = _device_of(logits, "logits", torch.float32 if fp32 else torch.bfloat16)
+        _require_here(u, "u", torch.float32, here)
         if logits.dim() != 2 or logits.stride(1) != 1:
             raise ValueError("logits must be [B, vocab] with contiguous rows")
         B, V = logits.shape
         if tuple(u.shape) != (B,) or not u.is_contiguous():
             raise ValueError(f"u must be a contiguous [{B}] tensor")
-        args, tensors = [], {}
+        args = []
         for name, t, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
                                ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
             if isinstance(t, torch.Tensor):
-                _require_gpu_tensor(t, name, dtype)
+                _require_here(t, name, dtype, here)
                 if tuple(t.shape) != (B,) or not t.is_contiguous():
                     raise ValueError(f"{name} must be a number or a contiguous [{B}] tensor")
-                tensors[name] = t
                 args += [t.data_ptr(), 0]
             else:
                 if not t >= 0 or (name in ("top_p", "min_p") and t > 1):
                     raise ValueError(f"{name} is out of range: {t}")
                 args += [None, min(int(t), V) if dtype is torch.int32 else t]
-        _one_device(logits=logits, u=u, work=work, out=out, **tensors)
         if out is None:
-            out = torch.empty(B, dtype=torch.int32, device=logits.device)
+            out = logits.new_empty(B, dtype=torch.int32)
         else:
-            _require_gpu_tensor(out, "out", torch.int32)
+            _require_here(out, "out", torch.int32, here)
             if tuple(out.shape) != (B,) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{B}] tensor")
         if B == 0:
@@ -790,10 +795,10 @@ class Kernels:
         if work is None:
             work = self.sample_workspace(B, V, logits.dtype, device=logits.device)
         else:
-            _require_gpu_tensor(work, "work", torch.uint8)
+            _require_here(work, "work", torch.uint8, here)
         rc = self.lib.ns_sample(logits.data_ptr(), int(fp32), logits.stride(0) if B > 1 else V, u.data_ptr(),
                                 *args, out.data_ptr(), None if work is None else work.data_ptr(),
-                                0 if work is None else work.numel(), B, V, self._stream())
+                                0 if work is None else work.numel(), B, V, _raw_stream(here))
         self._check(rc, "ns_sample")
         return out
 

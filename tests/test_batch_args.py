@@ -82,7 +82,7 @@ def test_wrapper_refusals(monkeypatch):
 
     monkeypatch.setattr(ops, "_require_gpu_tensor", check)
     monkeypatch.setattr(ops, "_current_device", lambda: -1)  # what CPU tensors say
-    monkeypatch.setattr(Kernels, "_stream", staticmethod(lambda: 0))
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
 
     def attend(q=torch.zeros(3, 512, dtype=BF16), kp=_pool(), vp=_pool(), pages=torch.zeros(3, 4, **ints),
                lens=torch.zeros(3, **ints), heads=4, **kw):

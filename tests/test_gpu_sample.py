@@ -123,6 +123,28 @@ def test_draw_follows_the_weights(kernels):
     assert kernels.sample(x.cuda(), u.cuda(), temperature=0.0).tolist() == [2] * 7
 
 
+# top-k around the rules: as many as tiles (297 of 152064, one thread each; 800 of 409600, two), the list
+# (2048), and top-p behind a top-k that no list holds; rows whose candidates crowd one bin or overflow it
+@pytest.mark.parametrize("V,ks", [(152064, (296, 297, 298, 2047, 2048, 2049, 20000)), (409600, (799, 800, 801, 2048)),
+                                  (1 << 20, (50, 2048, 5000))])
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_top_k_rules(kernels, V, ks, dtype):
+    g = torch.Generator().manual_seed(V)
+    for kind in ("spread", "crowded", "few tiles"):
+        x = torch.randn(2, V, generator=g) * 2
+        if kind == "crowded":
+            x = (x * 3).round() / 3
+        if kind == "few tiles":
+            x[:, 3000:] -= 1e4
+        x = x.to(dtype).cuda()
+        u = torch.rand(2, generator=g)
+        for k in ks:
+            for p, m in ((1.0, 0.0), (0.9, 0.0), (0.7, 0.02)):
+                got = kernels.sample(x, u.cuda(), 1.5, k, p, m)
+                T, p_, m_ = (torch.full((2,), v, dtype=torch.float32) for v in (1.5, p, m))
+                _compare(got.cpu(), x.cpu(), u, T, torch.full((2,), k), p_, m_)
+
+
 @pytest.mark.parametrize("B", [1, 3, 64])
 @pytest.mark.parametrize("dtype", [BF16, torch.float32])
 def test_graph_replays(kernels, B, dtype):
