@@ -785,12 +785,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedArgs a) {
 // kWavesPer waves per (token, head), or one wave per `per` heads of a token; lane = D / 64 dimensions. A partial
 // without keys has maximum -inf.
 template <int D, int kWavesPer>
-__global__ void __launch_bounds__(256) paged_merge_kernel(PagedArgs a, int per) {
-  constexpr int V = D / 64, kBatch = 8;
-  __shared__ float red_m[4], red_l[4], red_o[4][D];
+__global__ void __launch_bounds__(kWavesPer > 1 ? 64 * kWavesPer : 256) paged_merge_kernel(PagedArgs a, int per) {
+  constexpr int V = D / 64, kBatch = 8, kRowsPer = kWavesPer > 1 ? 1 : 4;
+  __shared__ float red_m[kWavesPer], red_l[kWavesPer], red_o[kWavesPer][D];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int groups = a.Hq / per;
-  const long long id = (long long)blockIdx.x * (4 / kWavesPer) + wv / kWavesPer;
+  const long long id = (long long)blockIdx.x * kRowsPer + wv / kWavesPer;
   const int t = __builtin_amdgcn_readfirstlane((int)(id / groups));
   const int h0 = __builtin_amdgcn_readfirstlane((int)(id % groups)) * per;
   const int w = wv % kWavesPer;
@@ -880,7 +880,8 @@ struct Plan {
   bool one;           // the one-token kernel
   int unit, target;   // least blocks per workgroup, workgroups aimed at
   long long items;    // workgroups per kv head of the own-keys launch
-  long long cap;      // token slots of its partials
+  long long ranges;   // of one sequence at most
+  long long cap;      // token slots of the partials
   int sh_splits;
   long long sh_items;
   size_t bytes;       // workspace
@@ -901,7 +902,7 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   p.unit = 4;  // 64 keys (a block per wave) and 256
   p.target = p.one ? 2 * cus : 3 * cus / 2;
   const int blk = p.one ? kOneRows : kTileKeys;
-  const long long most = ((max_len + blk - 1) / blk + p.unit - 1) / p.unit;  // ranges of one sequence
+  const long long most = p.ranges = ((max_len + blk - 1) / blk + p.unit - 1) / p.unit;
   const long long tiles = p.one ? B : std::min<long long>((long long)T * R / kTileRows + B, (long long)T * R);
   const long long per_head = p.target / Hk + 2;
   p.items = std::min(tiles * most, per_head + tiles);
@@ -932,15 +933,20 @@ void launch_paged(const PagedArgs& a, const Plan& p, hipStream_t st) {
   else
     hipLaunchKernelGGL((paged_attn_kernel<D, kOne, false>), grid, dim3(256), 0, st, a);
   if (p.bytes == 0) return;
-  // few rows and many partials (about, if the batch's sequences are alike) take a workgroup per row; many
-  // rows, which seldom have more than one partial, a wave per token
+  // Few rows with many partials (about that many, if the batch's sequences are alike) take a workgroup each: of
+  // four waves, or of eight (us of the whole call with 1, 4, 8 and 16 waves: one sequence of 700, 11 partials,
+  // 10.1, 9.4, 9.9, 10.5; 32 behind 4096 shared positions, 21 partials, 25.2, 22.8, 25.2, 30.5; one of 32000,
+  // 129 partials, -, 23.3, 21.7, 21.7). Many rows, which seldom have more than one partial, take a wave per token.
   const long long rows = (long long)a.s.T * a.Hq;
-  const long long most = p.sh_splits + p.target / ((long long)a.Hk * a.s.B) + 1;
-  const int per = rows > 32768 ? a.Hq : 1;
-  if (most > 16 && rows <= 8192)
+  const long long most = p.sh_splits + std::min<long long>(p.target / ((long long)a.Hk * a.s.B) + 1, p.ranges);
+  if (most > 64 && rows <= 8192) {
+    hipLaunchKernelGGL((paged_merge_kernel<D, 8>), dim3((unsigned)rows), dim3(512), 0, st, a, 1);
+  } else if (most > 8 && rows <= 8192) {
     hipLaunchKernelGGL((paged_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, 1);
-  else
+  } else {
+    const int per = rows > 32768 ? a.Hq : 1;
     hipLaunchKernelGGL((paged_merge_kernel<D, 1>), dim3((unsigned)((rows / per + 3) / 4)), dim3(256), 0, st, a, per);
+  }
 }
 
 }  // namespace
