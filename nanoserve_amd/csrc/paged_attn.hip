@@ -901,21 +901,26 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   p.one = !ragged && R <= 16;
   p.unit = 4;  // 64 keys (a block per wave) and 256
   p.target = p.one ? 2 * cus : 3 * cus / 2;
-  const int blk = p.one ? kOneRows : kTileKeys;
-  const long long most = p.ranges = ((max_len + blk - 1) / blk + p.unit - 1) / p.unit;
-  const long long tiles = p.one ? B : std::min<long long>((long long)T * R / kTileRows + B, (long long)T * R);
-  const long long per_head = p.target / Hk + 2;
-  p.items = std::min(tiles * most, per_head + tiles);
-  p.cap = std::min((long long)T * most, T + (p.one ? 1 : kTileRows / R + 1) * per_head);
   if (shared > 0) {
     const long long st = ((long long)T * R + kTileRows - 1) / kTileRows;
     const int blocks = (shared + kTileKeys - 1) / kTileKeys;
     // One workgroup per CU, which leaves the other half of its LDS to the sequences' own keys. us for one, one and
     // a half, two and three: 96 sequences (194 tokens) behind 16384 99.6, 108.8, 116.5, 126.8.
     const long long want = cus / (st * Hk);
-    p.sh_splits = (int)std::max(1ll, std::min<long long>(want, blocks / 4));
+    // at least four blocks each, two where that leaves fewer than eight splits (8 sequences behind 1024: 14.4 ->
+    // 11.8 us; always two: 32 behind 4096 23.3 -> 26.5)
+    const int most = std::max(blocks / 4, std::min(blocks / 2, 8));
+    p.sh_splits = (int)std::max(1ll, std::min<long long>(want, most));
     p.sh_items = st * p.sh_splits;
   }
+  if (p.one && p.sh_items > 0)  // the rest of one round of workgroups
+    p.target = (int)std::max<long long>(cus, 2ll * cus - p.sh_items * Hk);
+  const int blk = p.one ? kOneRows : kTileKeys;
+  const long long most = p.ranges = ((max_len + blk - 1) / blk + p.unit - 1) / p.unit;
+  const long long tiles = p.one ? B : std::min<long long>((long long)T * R / kTileRows + B, (long long)T * R);
+  const long long per_head = p.target / Hk + 2;
+  p.items = std::min(tiles * most, per_head + tiles);
+  p.cap = std::min((long long)T * most, T + (p.one ? 1 : kTileRows / R + 1) * per_head);
   if (p.cap > T || p.sh_splits > 0) {
     const size_t parts = ((size_t)p.cap + (size_t)p.sh_splits * T) * Hq;
     p.bytes = (size_t)T * sizeof(int4) + parts * (D + 2) * sizeof(float);
