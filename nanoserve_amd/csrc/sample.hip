@@ -331,7 +331,7 @@ struct Settings {
 
 struct Scratch {  // of the workgroup-wide sums and searches
   uint64_t red64[kRowWaves], hit64;
-  uint32_t red32[kRowWaves], hit;
+  uint32_t red32[kRowWaves], hit, above, in;
 };
 
 // The bin, from the first on (last: from the last down), at which the running sum of h reaches `target`
@@ -458,26 +458,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_hist_kernel(SampleArgs a) 
 }
 
 // ------------------------------------------------------------------ scan
-// top-p's bin by the histogram's weights
-__device__ __forceinline__ void cut_by_weight(const Settings& c, const uint64_t* weights, const uint32_t* counts,
-                                              Scratch& s, RowState& st) {
-  uint64_t sum = 0, total, done;
-  for (int i = threadIdx.x; i < kBins; i += kThreads) sum += weights[i];
-  block_exclusive<uint64_t>(sum, total, s.red64);
-  const uint64_t need = c.reach(total);
-  st.cut = crossing<false, uint64_t>(weights, need, done, s.red64, s);
-  uint32_t some = 0, n;
-  for (int i = threadIdx.x; i <= (int)st.cut; i += kThreads) some += counts[i];
-  block_exclusive<uint32_t>(some, n, s.red32);
-  st.total = total;
-  st.from = c.low;
-  st.need = need - done;
-  st.todo = n <= kShort ? kToList : counts[st.cut] <= kList ? kTopP : kSlow;
-}
-
 // What the row's histogram says.
-__device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Settings& c, uint64_t* weights,
-                                           uint32_t* counts, Scratch& s) {
+__device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Settings& c, float* maxima, Scratch& s) {
   const int tid = threadIdx.x;
   RowState st{};
   if (c.greedy || !(c.k_on || c.p_on)) {
@@ -486,7 +468,6 @@ __device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Set
   }
   st.from = c.low;
   if (c.by_tiles) {  // the top_k-th largest maximum: the least of those with fewer than top_k above them
-    float* maxima = reinterpret_cast<float*>(counts);
     const float* tile_max = a.tile_max + (size_t)r * a.tiles;
     const int quads = (a.tiles + 3) / 4;
     for (int i = tid; i < 4 * quads; i += kThreads) maxima[i] = i < a.tiles ? tile_max[i] : -INFINITY;
@@ -524,41 +505,69 @@ __device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Set
     st.from = fmaxf(least, c.low);
     return st;
   }
-  uint32_t some = 0, n;
-  for (int i = tid; i < kBins; i += kThreads) {
-    some += counts[i] = a.counts[(size_t)r * kBins + i];
-    if (c.weighted) weights[i] = a.weights[(size_t)r * kBins + i];
+  // this thread's bins, and the counts and weights of those before them
+  uint32_t in[kBinsPer], some = 0, n;
+  uint64_t w[kBinsPer], sum = 0, total = 0;
+#pragma unroll
+  for (int e = 0; e < kBinsPer; ++e) {
+    in[e] = a.counts[(size_t)r * kBins + kBinsPer * tid + e];
+    w[e] = c.weighted ? a.weights[(size_t)r * kBins + kBinsPer * tid + e] : 0;
+    some += in[e];
+    sum += w[e];
   }
-  block_exclusive<uint32_t>(some, n, s.red32);
-  if (c.k_on && (uint32_t)c.top_k < n) {
-    st.cut = crossing<false, uint32_t>(counts, (uint32_t)c.top_k, st.above, s.red32, s);
-    const uint32_t in = counts[st.cut];
-    st.todo = st.above + in <= kList ? kToList : c.top_k > kList && in <= kList ? kTopK : kSlow;
-  } else if (n <= kShort || (c.p_on && !c.weighted)) {  // (then n <= top_k <= kList)
+  uint32_t before = block_exclusive<uint32_t>(some, n, s.red32);
+  const bool by_count = c.k_on && (uint32_t)c.top_k < n;
+  if (!by_count && (n <= kShort || (c.p_on && !c.weighted))) {  // (without weights n <= top_k <= kList)
     st.cut = kBins - 1;
     st.todo = kToList;
-  } else if (c.p_on) {
-    cut_by_weight(c, weights, counts, s, st);
-  } else {
+    return st;
+  }
+  if (!by_count && !c.p_on) {
     st.todo = kSum;
+    return st;
+  }
+  uint64_t done = c.weighted ? block_exclusive<uint64_t>(sum, total, s.red64) : 0;
+  const uint64_t need = c.reach(total);
+#pragma unroll
+  for (int e = 0; e < kBinsPer; ++e) {
+    const bool here = by_count ? before < (uint32_t)c.top_k && before + in[e] >= (uint32_t)c.top_k
+                               : done < need && done + w[e] >= need;
+    if (here) {
+      s.hit = kBinsPer * tid + e;
+      s.above = before;
+      s.in = in[e];
+      s.hit64 = done;
+    }
+    before += in[e];
+    done += w[e];
+  }
+  __syncthreads();
+  st.cut = s.hit;
+  const uint32_t above = s.above, level = s.in;
+  if (by_count) {
+    st.above = above;
+    st.todo = above + level <= kList ? kToList : c.top_k > kList && level <= kList ? kTopK : kSlow;
+  } else {
+    st.total = total;
+    st.need = need - s.hit64;
+    st.todo = above + level <= kShort ? kToList : level <= kList ? kTopP : kSlow;
   }
   return st;
 }
 
 template <typename E>
 __global__ void __launch_bounds__(kThreads, 4) sample_scan_kernel(SampleArgs a) {
-  __shared__ uint64_t weights[kBins];  // then the list
-  __shared__ __align__(16) uint32_t counts[kBins];
+  __shared__ __align__(16) float maxima[2 * kThreads];
+  __shared__ uint64_t list[kList];
   __shared__ Scratch s;
   __shared__ uint32_t n, base;
-  static_assert(kList <= kBins, "the list takes the histogram's place");
   const int r = blockIdx.y, tid = threadIdx.x;
   RowState* state = a.state + 2 * r + a.round;
   if (a.round && state->todo == kDone) return;
   Settings c(a, r);
   RowState st;
   if (a.round == 0) {
-    st = decide(a, r, c, weights, counts, s);
+    st = decide(a, r, c, maxima, s);
     if (blockIdx.x == 0 && tid == 0) *state = st;
   } else {
     st = *state;
@@ -572,7 +581,6 @@ __global__ void __launch_bounds__(kThreads, 4) sample_scan_kernel(SampleArgs a) 
   part_tiles(a, blockIdx.x, t0, t1);
   const float low = c.low;
   const uint32_t cut = st.cut;
-  uint64_t* list = weights;
   auto put = [&](float x, int index) {
     const uint32_t at = atomicAdd(&n, 1u);
     if (at < kList) list[at] = (uint64_t)~key_of(x) << 32 | (uint32_t)index;
@@ -636,6 +644,23 @@ struct EndShared {
   int first;
   uint32_t last;
 };
+
+// top-p's bin by the histogram's weights
+__device__ __forceinline__ void cut_by_weight(const Settings& c, const uint64_t* weights, const uint32_t* counts,
+                                              Scratch& s, RowState& st) {
+  uint64_t sum = 0, total, done;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) sum += weights[i];
+  block_exclusive<uint64_t>(sum, total, s.red64);
+  const uint64_t need = c.reach(total);
+  st.cut = crossing<false, uint64_t>(weights, need, done, s.red64, s);
+  uint32_t some = 0, n;
+  for (int i = threadIdx.x; i <= (int)st.cut; i += kThreads) some += counts[i];
+  block_exclusive<uint32_t>(some, n, s.red32);
+  st.total = total;
+  st.from = c.low;
+  st.need = need - done;
+  st.todo = n <= kShort ? kToList : counts[st.cut] <= kList ? kTopP : kSlow;
+}
 
 // Ascending, n2 a power of two. Thread t exchanges pair t: with distances up to 64 a wave's pairs stay
 // within its own 128 values, in order by themselves, and only the other steps need the workgroup's barrier
