@@ -62,8 +62,8 @@ size_t ns_paged_attention_workspace(int T, int B, int Hq, int Hk, int D, int max
  * sees, zeros where that is nothing; token rows of no sequence are left alone. q: rows q_stride apart,
  * heads contiguous. Products of bf16 operands, softmax and all sums in fp32; probabilities enter the
  * second product as two bf16 terms (16 significant bits).
- * shared > 0: the caller states that positions 0 .. shared - 1 lie in the same pages for every
- * sequence that is that long; they are read through the table's first row, once for the whole batch.
+ * shared > 0: the caller states that positions 0 .. shared - 1, as far as a sequence has them, lie in the
+ * same pages for every sequence; they are read through the row of the longest one, once for the batch.
  * Values (NaN and infinities among them) in positions that no token of a sequence sees have no
  * effect; a NaN value that some token of a launch tile sees may reach the tile's other tokens of the same kv head.
  * -2 for D other than 64 and 128, Hq % Hk, negative window, sinks or shared, scale not positive and finite,

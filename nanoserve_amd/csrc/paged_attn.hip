@@ -71,6 +71,27 @@ struct KeyBlocks {
   __device__ int block(int j) const { return j < na ? a0 + j : m0 + j - na; }
 };
 
+// One of the longest sequences: its table row has every shared position that any sequence has.
+__device__ __forceinline__ int longest(const PagedArgs& a) {
+  const int lane = __lane_id();
+  int most = -1, at = 0;
+  for (int b = lane; b < a.s.B; b += kWave) {
+    const int n = a.s.positions(b);
+    if (n > most) {
+      most = n;
+      at = b;
+    }
+  }
+  int m = max(most, 0);  // (lanes shifted in from outside count as 0)
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x111, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x112, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x114, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x118, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x142, 0xa, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(at, __builtin_ctzll(__ballot(most == __builtin_amdgcn_readlane(m, 63))));
+}
+
 __device__ __forceinline__ int low_limit(const PagedArgs& a, int pos) {
   return a.window > 0 ? max(pos + 1 - a.window, 0) : 0;
 }
@@ -459,6 +480,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     rows = a.s.T * R;
     k0 = 0;
     k1 = min(a.shared, a.s.width * a.s.page_size);
+    b = longest(a);
   } else {
     int within;
     if (!find_item<kTileKeys, kTileRows>(a, item, b, sp, within, slot)) return;
@@ -477,10 +499,12 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   const int row = min(wrow + jq, rows - 1);
   const int tok = row / R, hq = g * R + row % R;
   int t, pos;
+  bool counts = wrow + jq < rows;  // a row with a result, which is zero if it sees nothing
   if constexpr (kShared) {
     t = tok;
     const int sb = a.s.sequence(t);
     pos = -1;
+    counts &= sb >= 0;
     if (sb >= 0) {
       int row0, nn;
       a.s.tokens(sb, row0, nn);
@@ -490,14 +514,14 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     t = sp.row0 + tok;
     pos = sp.n - sp.nn + tok;
   }
-  const bool real = wrow + jq < rows && pos >= 0;
+  const bool real = counts && pos >= 0;
   const int hi = real ? min(pos + 1, k1) : 0, lo = low_limit(a, pos);
   const int first = a.window > 0 ? a.sinks : 0;
   // limits over the wave's rows and over the tile's: a sequence's positions rise with its rows, the rows of
   // the whole batch need a look at each
   int hi_min, hi_max, lo_min, lo_max, top, low;
   if constexpr (kShared) {
-    hi_min = real ? hi : INT_MAX, hi_max = hi, lo_min = real ? lo : INT_MAX, lo_max = real ? lo : 0;
+    hi_min = counts ? hi : INT_MAX, hi_max = hi, lo_min = real ? lo : INT_MAX, lo_max = real ? lo : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       hi_min = min(hi_min, __shfl_xor(hi_min, o, kWave));
@@ -539,7 +563,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   }
 
   // lane i: offset in the pools of 16-row group i % 4 of block j0 + 16 (.. / 16) + i / 4 of the list
-  const int* table = a.s.table + (kShared ? 0 : (size_t)b * a.s.table_stride);
+  const int* table = a.s.table + (size_t)b * a.s.table_stride;
   uint64_t offs = 0, valid = 0;
   auto refill = [&](int j) {
     const int v = j + (lane >> 2);
@@ -680,16 +704,20 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
                                                                 p1 - __uint_as_float(term & 0xffff0000u));
       }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      bf16x8_t vf[kDT];
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
         const u32x2_t v0 = lds_read_tr16(&vb[vt[d] + 16 * u * D]);
         const u32x2_t v1 = lds_read_tr16(&vb[vt[d] + (16 * u + 8) * D]);
-        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, (u32x4_t){v0[0], v0[1], v1[0], v1[1]});
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, __builtin_bit_cast(bf16x8_t, pt[i][u]), o[d], 0, 0, 0);
+        vf[d] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v0[0], v0[1], v1[0], v1[1]});
       }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 0; d < kDT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d], __builtin_bit_cast(bf16x8_t, pt[i][u]), o[d], 0, 0, 0);
+    }
   };
 
   // Block j is ready once every wave's loads of it have landed (those of up to kStages - 2 newer blocks stay

@@ -645,8 +645,8 @@ class Kernels:
     def paged_append(self, qkv, bias, inv_freq, pages, lens, k_pages, v_pages, n_heads, q_start=None,
                      out=None):
         """The new tokens of a batch of sequences: bias add and RoPE of the fused projection output
-        qkv [T, (Hq + 2Hk) * D] (rows may be strided), k and v heads into the paged cache; returns
-        the q heads [T, Hq * D].
+        qkv [T, (Hq + 2Hk) * D] (rows any multiple of 8 elements apart), k and v heads into the paged
+        cache; returns the q heads [T, Hq * D].
 
         k_pages, v_pages [n_pages, Hk, page_size, D] (page_size a multiple of 16, heads contiguous,
         e.g. one layer of a larger pool), pages [B, width] int32: the pages of each sequence's
@@ -702,12 +702,12 @@ class Kernels:
                         window=0, sinks=0, scale=None, work=None, out=None):
         """Causal grouped-query attention of a batch's new tokens over its paged cache, their own keys
         and values included (paged_append first; pages, lens and q_start as there): q [T, Hq * D]
-        (rows may be strided), head size 64 or 128; returns [T, Hq * D] bf16.
+        (rows any multiple of 8 elements apart), head size 64 or 128; returns [T, Hq * D] bf16.
 
         With ``window`` a token sees the last ``window`` positions (its own among them) and the first
-        ``sinks`` ones. ``shared``: the first ``shared`` positions have the same pages in every row of
-        ``pages`` (the caller's statement; they are read through row 0); their keys and values are then
-        read once for the whole batch. A token that sees nothing gets zeros; rows past the last
+        ``sinks`` ones. ``shared``: the first ``shared`` positions, as far as a sequence has them, lie in
+        the same pages for every sequence (the caller's statement); their keys and values are then read
+        once for the whole batch. A token that sees nothing gets zeros; rows past the last
         sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be positive. ``work``: from
         paged_attention_workspace, allocated here when it is not given. The reference has SDPA over one
         sequence's cache (qwen.py:124-133)."""

@@ -252,3 +252,105 @@ def test_append(kernels, Hq, Hk, D, page, bias, lens, new):
                 keep[i, pg, :, 1, p % page] = want[t, Hq + i * Hk:Hq + (i + 1) * Hk]
                 tol[i, pg, :, 1, p % page] = bound[t, Hq + i * Hk:Hq + (i + 1) * Hk]
     assert bool(((pools.double() - keep).abs() <= tol).all())
+
+
+def test_shared_prefix_behind_an_empty_slot(kernels):
+    """A padded batch: the first slot has no positions and no pages, another is shorter than the prefix."""
+    Hq, Hk, D = 28, 4, 128
+    batch = R.PagedBatch([0, 300, 90, 260], None, Hk, D, 16, shared=256, seed=4)
+    batch.table[0] = -1
+    batch.table[2, 6:] = 1 << 30
+    q = _queries(batch.T, Hq, D, 6)
+    got = _attend(kernels, batch, q, Hq, shared=256)
+    _check(got, R.attention(batch, q, Hq), batch)
+    assert bool((got[0] == 0).all())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_offsets_past_32_bits(kernels, D):
+    """Pages whose offsets pass 2^32 bytes and 2^32 elements, for both operators; nothing is written
+    elsewhere."""
+    Hq, Hk, page = 4, 1, 16
+    n_pages = (1 << 32) // (page * D) + 70
+    k, v = (torch.empty(n_pages, Hk, page, D, dtype=BF16, device="cuda") for _ in range(2))
+    ids = [n_pages - 1, 3, (1 << 31) // (page * D) + 1, n_pages - 40]  # the low words of some collide
+    low = [i % ((1 << 32) // (page * D)) for i in ids if i >= (1 << 32) // (page * D)]
+    for pool in (k, v):
+        for i in low:
+            pool[i] = 9.0
+    n = page * len(ids) - 5
+    table = torch.tensor([ids], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(D)
+    qkv = torch.randn(n, (Hq + 2 * Hk) * D, generator=g, device="cuda").to(BF16)
+    inv = (1.0 / 1e6 ** (torch.arange(0, D, 2).float() / D)).cuda()
+    q = kernels.paged_append(qkv, None, inv, table, lens, k, v, Hq, q_start=start)
+    got = kernels.paged_attention(q, k, v, table, lens, Hq, q_start=start)
+    one = kernels.paged_attention(q[-1:], k, v, table, lens, Hq)
+    torch.cuda.synchronize()
+    assert all(bool((pool[i] == 9).all()) for pool in (k, v) for i in low)
+    kk, vv = (pool[torch.tensor(ids, device="cuda")][:, 0].reshape(-1, D)[:n].double() for pool in (k, v))
+    assert torch.equal(vv, qkv[:, (Hq + Hk) * D:].double())
+    s = (q.double().view(n, Hq, D).transpose(0, 1).reshape(-1, D) @ kk.t()).view(Hq, n, n) / D ** 0.5
+    s = s.masked_fill(~torch.ones(n, n, dtype=torch.bool, device="cuda").tril(), float("-inf"))
+    want = (torch.softmax(s, -1).view(-1, n) @ vv).view(Hq, n, D).transpose(0, 1)
+    bound = want.abs() * 2.0 ** -8 + 2.0 ** -13 * vv.abs().amax()
+    assert bool(((got.double().view(n, Hq, D) - want).abs() <= bound).all())
+    assert bool(((one.double().view(Hq, D) - want[-1]).abs() <= bound[-1]).all())
+
+
+@pytest.mark.parametrize("n,ragged", [(700001, False), (300007, True)])
+def test_long_cache(kernels, n, ragged):
+    """Far positions: keys planted at the start, the middle and the end decide the result."""
+    Hq, Hk, D, page = 7, 1, 128, 64
+    g = torch.Generator(device="cuda").manual_seed(n)
+    count = -(-n // page)
+    k, v = (torch.randn(count, Hk, page, D, generator=g, device="cuda").to(BF16) for _ in range(2))
+    k *= 0.05
+    table = torch.randperm(count, generator=g, device="cuda").to(torch.int32)[None]
+    T = 5 if ragged else 1
+    q = torch.randn(T, Hq * D, generator=g, device="cuda").to(BF16)
+    q[:, ::D] = 16.0
+    for j in (5, n // 2, n - T - 1, n - 2):
+        k[int(table[0, j // page]), 0, j % page, 0] = 18.0
+    start = torch.tensor([0, T], dtype=torch.int32, device="cuda") if ragged else None
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    got = kernels.paged_attention(q, k, v, table, lens, Hq, q_start=start).double().view(T, Hq, D)
+    kk, vv = (pool[table[0].long(), 0].reshape(-1, D)[:n].double() for pool in (k, v))
+    for t in range(T):
+        s = q[t].double().view(Hq, D) @ kk[:n - T + t + 1].t() / D ** 0.5
+        want = torch.softmax(s, -1) @ vv[:n - T + t + 1]
+        err = (got[t] - want).abs()
+        assert bool((err <= want.abs() * 2.0 ** -8 + 2.0 ** -13 * vv.abs().amax()).all())
+
+
+def test_many_sequences(kernels):
+    """A batch of a thousand: its items are found over many steps, single tokens and drafts."""
+    Hq, Hk, D = 4, 2, 64
+    lens = [(37 * i) % 90 for i in range(1000)]
+    for new in (None, [min(i % 5, n) for i, n in enumerate(lens)]):
+        batch = R.PagedBatch(lens, new, Hk, D, 16, seed=8)
+        q = _queries(batch.T, Hq, D, 8)
+        _check(_attend(kernels, batch, q, Hq), R.attention(batch, q, Hq), batch)
+
+
+def test_two_streams(kernels):
+    """Calls with workspaces of their own at once on two streams, tensors made on a third."""
+    Hq, Hk, D = 28, 4, 128
+    batch = R.PagedBatch([3000, 17, 900], None, Hk, D, 16, seed=3)
+    q = _queries(batch.T, Hq, D, 1)
+    want = _attend(kernels, batch, q, Hq)
+    x = torch.randn(3, 50000, generator=torch.Generator().manual_seed(1)).cuda()
+    u = torch.rand(3, generator=torch.Generator().manual_seed(2)).cuda()
+    tok = kernels.sample(x, u, 0.9, 0, 0.9)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append((kernels.paged_attention(q, batch.k, batch.v, batch.table, batch.lens, Hq),
+                         kernels.sample(x, u, 0.9, 0, 0.9)))
+    torch.cuda.synchronize()
+    for a, t in outs:
+        assert torch.equal(a, want) and torch.equal(t, tok)

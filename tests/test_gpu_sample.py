@@ -145,6 +145,25 @@ def test_top_k_rules(kernels, V, ks, dtype):
                 _compare(got.cpu(), x.cpu(), u, T, torch.full((2,), k), p_, m_)
 
 
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_extreme_temperatures_and_logits(kernels, dtype):
+    """Temperatures from the least normal number to infinity; logits of the type's lowest and highest."""
+    V, B = 3001, 24
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn(B, V, generator=g)
+    top = torch.finfo(dtype).max
+    x[1::4] *= 1e30
+    x[2::4] = torch.where(x[2::4] > 1, top, -top)
+    x[3::4] = torch.where(x[3::4] > 0, x[3::4], torch.tensor(torch.finfo(dtype).min))
+    x = x.to(dtype)
+    u = torch.rand(B, generator=g)
+    for T in (1.2e-38, 1e-30, 1e-3, 1e3, 1e30, math.inf):
+        for k, p, m in ((0, 1.0, 0.0), (7, 1.0, 0.0), (0, 0.6, 0.0), (0, 1.0, 0.3), (2500, 0.5, 0.1)):
+            got = kernels.sample(x.cuda(), u.cuda(), T, k, p, m)
+            T_, p_, m_ = (torch.full((B,), v, dtype=torch.float32) for v in (T, p, m))
+            _compare(got.cpu(), x, u, T_, torch.full((B,), k), p_, m_)
+
+
 @pytest.mark.parametrize("B", [1, 3, 64])
 @pytest.mark.parametrize("dtype", [BF16, torch.float32])
 def test_graph_replays(kernels, B, dtype):
