@@ -521,8 +521,11 @@ class Qwen2Runner:
         """Returns the ``n_new`` generated ids. The decode steps replay one captured graph when
         ``use_graph``. Greedy at temperature 0 (reference qwen.py:166-177); at others each token is
         drawn by ``Kernels.sample`` with these settings from the random numbers u [n_new] float32 in
-        [0, 1) (default: torch.rand)."""
+        [0, 1) (default: torch.rand); -1 stands where a step's logits left nothing to draw, and the
+        next step then starts from a zero embedding."""
         T = prompt_ids.shape[0]
+        if not temperature >= 0:
+            raise ValueError(f"temperature is out of range: {temperature}")
         if temperature > 0:
             if u is None:
                 u = torch.rand(n_new, device=self.dev)

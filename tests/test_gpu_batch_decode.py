@@ -1,5 +1,7 @@
 """The batch operators together, as a server uses them: a ragged prompt step, then decode steps of the
 whole batch, through a small W4A16 model's layers; every sequence against the one-sequence runner."""
+import math
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -96,3 +98,17 @@ def test_generate_samples(kernels):
     assert len(r.generate(ids, n, temperature=1.0)) == n
     with pytest.raises(ValueError):
         r.generate(ids, n, temperature=1.0, u=u[:3])
+
+
+def test_generate_without_a_token(kernels):
+    """Logits that are all NaN leave nothing to draw: -1, which the next step takes as a zero embedding, eager or
+    replayed. A temperature below zero or NaN is refused."""
+    shape = Qwen2Shape(layers=1, hidden=512, heads=4, kv_heads=2, intermediate=1024, vocab=2000)
+    r = Qwen2Runner.random(shape, seed=4, kernels=kernels)
+    ids = torch.arange(20).cuda()
+    for t in (-0.5, math.nan):
+        with pytest.raises(ValueError):
+            r.generate(ids, 3, temperature=t)
+    r.final_norm.fill_(math.nan)
+    for graph in (True, False):
+        assert r.generate(ids, 4, use_graph=graph, temperature=0.8, top_k=50, top_p=0.9) == [-1] * 4
