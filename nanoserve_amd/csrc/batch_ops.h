@@ -98,7 +98,8 @@ size_t ns_sample_workspace(int B, int V, int fp32);
  * Settings per row: temps, top_ks, top_ps, min_ps [B] device arrays, each NULL for the scalar beside it.
  * Weights are held in units of 2^-42 of the largest in 64-bit integers and summed exactly, so the token
  * does not depend on the order of any sum.
- * -2 for B <= 0, V <= 0, V > 2^20, row_stride < V, NULL or misaligned pointers (logits 2 or 4 bytes).
+ * -2 for B <= 0, B > 65535, V <= 0, V > 2^20, row_stride < V, NULL or misaligned pointers (logits 2 or 4
+ * bytes, int and float 4, work 16), work_bytes too small.
  */
 int ns_sample(const void* logits, int fp32, long long row_stride, const float* u, const float* temps,
               float temp, const int* top_ks, int top_k, const float* top_ps, float top_p,

@@ -2,8 +2,8 @@
 // tokens, prompts, a window with first tokens, and a prefix that all sequences share. The reference
 // has PyTorch SDPA over one contiguous cache (python/nanoserve/qwen.py:124-133).
 //
-// Three launches at most: the keys of the shared prefix (tile kernel over all tokens' rows), each
-// sequence's own keys (one-token kernel or tile kernel), and a merge of the fp32 partials.
+// Two launches at most: the keys of the shared prefix (tiles over all tokens' rows) together with each
+// sequence's own keys (streamed for single tokens, else tiles), and a merge of the fp32 partials.
 //
 // Work is dealt out on the device, because lengths are device values (a captured graph replays at any
 // lengths): every workgroup adds up the key blocks of the whole batch, takes the share per workgroup
@@ -224,6 +224,9 @@ __device__ __forceinline__ void wait_loads(int n) {
 //    read hit distinct banks), V rows so that the 4 x 16 blocks of a transposed read do.
 //  * Value rows that the token does not see are not read but zero: their probability is 0, and whatever
 //    the page holds there (it may be NaN) must not reach the sum.
+// Measured (28 / 4 heads of 128): 4 sequences of 98 000 127 us, 6.2 TB/s of reads (a read probe reaches 6.84); 32
+// of 3000 to 30000 with a window of 4096 52.6 us, 5.1 TB/s; 16 of 33 to 8191 30 us, of them 4 in the merge; one of
+// 700 with 12 / 2 heads 9.4 us, the latency of two launches.
 template <int D>
 __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, const Ring& lds,
                                          float (&red)[2][kOneWaves][16]) {
@@ -237,7 +240,7 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
   Span sp;
   if (!find_item<kOneRows, 0>(a, item, b, sp, split, slot)) return;
   const bool direct = sp.splits == 1 && a.sh_splits == 0;
-  if (!direct && slot + sp.splits > a.cap) return;
+  if (!direct && (slot < 0 || slot + sp.splits > a.cap)) return;
 
   const int n = sp.n, lo = low_limit(a, n - 1), first = a.window > 0 ? a.sinks : 0, k0 = a.shared;
   const KeyBlocks<kOneRows> kb(k0, n, lo, first);
@@ -456,9 +459,15 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
 //  * Scores are computed transposed, S^T = K Q^T on v_mfma_f32_32x32x16_bf16: a lane owns one query and
 //    16 of each 32 keys, so the softmax needs one lane swap per reduction and the score registers are,
 //    as they stand, the B operand of O^T = V^T P^T; ds_read_b64_tr_b16 delivers V^T's fragments.
-//  * Probabilities enter as two bf16 terms (16 significant bits).
+//  * Probabilities enter as two bf16 terms (16 significant bits): the error is then the output's own rounding, for
+//    1.5 times the products of one term.
 //  * A row sees positions below `hi` and from `lo` on or below `sinks`; blocks that no row of the tile
 //    sees are left out of its list, blocks that all rows see whole skip the comparisons.
+// Measured (28 / 4 heads of 128): prompts of 5 sequences of 2000 to 8000 654 us, 677 TFLOP/s, with the second term
+// 1015 (a large library product: 1265); matrix cores busy in half of the cycles and vector units in 58 %, at 1.8 GHz.
+// Issuing one half block's softmax between the products of its neighbours did not help (659 -> 681 to 730 us): the
+// other wave of the SIMD fills those slots already. 4095 tokens with a window of 1000 and 14 / 2 heads of 64 43 us;
+// 96 drafts of 1 to 3 tokens behind 16384 shared positions 108 us.
 template <int D, bool kShared>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, int (&lim)[4][2]) {
   constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad, kDT = D / 32,
@@ -492,7 +501,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     k1 = sp.n;
   }
   const bool direct = !kShared && splits == 1 && a.sh_splits == 0;
-  if (!kShared && !direct && slot + (long long)sp.nn * splits > a.cap) return;
+  if (!kShared && !direct && (slot < 0 || slot + (long long)sp.nn * splits > a.cap)) return;
 
   // this lane's query: rows past the end repeat the last and see nothing
   const int wrow = r0 + 32 * wv;
@@ -811,7 +820,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedArgs a) {
 
 // ------------------------------------------------------------------ merge of the partials
 // kWavesPer waves per (token, head), or one wave per `per` heads of a token; lane = D / 64 dimensions. A partial
-// without keys has maximum -inf.
+// without keys has maximum -inf. Bound by latency: 3.3 to 4.8 us for 12 to 1500 workgroups.
 template <int D, int kWavesPer>
 __global__ void __launch_bounds__(kWavesPer > 1 ? 64 * kWavesPer : 256) paged_merge_kernel(PagedArgs a, int per) {
   constexpr int V = D / 64, kBatch = 8, kRowsPer = kWavesPer > 1 ? 1 : 4;
@@ -927,7 +936,11 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   const int R = Hq / Hk;
   shared = std::min(shared, max_len);
   p.one = !ragged && R <= 16;
-  p.unit = 4;  // 64 keys (a block per wave) and 256
+  // Least range 64 keys (a block per wave) and 256. us with half, this and twice it: one token at 4000 13.2, 11.8,
+  // 11.4; at 700 9.4, 9.5, 9.9; 20 tokens after 4000 19.4, 19.8, 23.8.
+  p.unit = 4;
+  // As many workgroups as run at once; tiles: one and a half per CU, since a range of few blocks costs a partial of
+  // 128 rows (us with one, one and a half, two: 1000 tokens 42.3, 42.9, 49.5; 512 after 3000 68.1, 67.1, 59.8).
   p.target = p.one ? 2 * cus : 3 * cus / 2;
   if (shared > 0) {
     const long long st = ((long long)T * R + kTileRows - 1) / kTileRows;
