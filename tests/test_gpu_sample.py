@@ -145,6 +145,20 @@ def test_top_k_rules(kernels, V, ks, dtype):
                 _compare(got.cpu(), x.cpu(), u, T, torch.full((2,), k), p_, m_)
 
 
+# lists around the longest one that is ordered by rank (512), from one token on, with level tokens at the cut
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_list_lengths(kernels, dtype):
+    g = torch.Generator().manual_seed(7)
+    for V in (5000, 152064):
+        x = (torch.randn(2, V, generator=g) * 2).to(dtype)
+        u = torch.rand(2, generator=g)
+        for k in (2, 3, 4, 5, 63, 64, 65, 255, 256, 257, 510, 511, 512, 513, 514, 1025):
+            for p in (1.0, 0.6):
+                got = kernels.sample(x.cuda(), u.cuda(), 1.2, k, p)
+                T, p_, m_ = (torch.full((2,), v, dtype=torch.float32) for v in (1.2, p, 0.0))
+                _compare(got.cpu(), x, u, T, torch.full((2,), k), p_, m_)
+
+
 @pytest.mark.parametrize("dtype", [BF16, torch.float32])
 def test_extreme_temperatures_and_logits(kernels, dtype):
     """Temperatures from the least normal number to infinity; logits of the type's lowest and highest."""
