@@ -62,9 +62,10 @@ struct RowState {
   uint64_t need;   // kTopP: what the weights of the bin's first tokens have to reach
 };
 
-// Whether the tiles' maxima bound this top-k (each thread ranks up to two of them).
+// Whether the tiles' maxima bound this top-k.
+constexpr int kMostTiles = 1024;
 __host__ __device__ inline bool tiles_bound(int top_k, int tiles) {
-  return top_k <= tiles && tiles <= 2 * kThreads && top_k <= kList;
+  return top_k <= tiles && tiles <= kMostTiles && top_k <= kList;
 }
 
 struct SampleArgs {
@@ -461,8 +462,52 @@ __global__ void __launch_bounds__(kThreads, 4) sample_hist_kernel(SampleArgs a) 
 }
 
 // ------------------------------------------------------------------ scan
+// The k-th largest tile maximum, down to its key's upper bits (for bf16 exactly): the largest value of so many bits that at
+// least k maxima reach, bit by bit. Each wave by itself, the maxima in registers.
+struct Maxima {
+  static constexpr int kPer = kMostTiles / kWave;
+  uint32_t key[kPer];
+  __device__ Maxima(const float* tile_max, int tiles) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4)
+      if (kWave * i < tiles) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = lane + kWave * (i + e);
+          key[i + e] = __float_as_uint(tile_max[min(at, tiles - 1)]);
+        }
+      }
+  }
+};
+__device__ __forceinline__ float kth_maximum(Maxima& m, int tiles, int k, int bits) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < Maxima::kPer; ++i)
+    if (kWave * (i & ~3) < tiles) m.key[i] = lane + kWave * i < tiles ? key_of(__uint_as_float(m.key[i])) : 0;
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int bit = 30; bit >= 32 - bits; bit -= 2) {  // two bits at a time
+    const uint32_t n1 = t | 1u << bit, n2 = t | 2u << bit, n3 = t | 3u << bit;
+    int c1 = 0, c2 = 0, c3 = 0;
+#pragma unroll
+    for (int i = 0; i < Maxima::kPer; i += 4)
+      if (kWave * i < tiles) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          c1 += __builtin_popcountll(__ballot(m.key[i + e] >= n1));
+          c2 += __builtin_popcountll(__ballot(m.key[i + e] >= n2));
+          c3 += __builtin_popcountll(__ballot(m.key[i + e] >= n3));
+        }
+      }
+    t = c3 >= k ? n3 : c2 >= k ? n2 : c1 >= k ? n1 : t;
+  }
+  return value_of(t);  // (NaN where fewer than k are above -inf)
+}
+
 // What the row's histogram says.
-__device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Settings& c, float* maxima, Scratch& s) {
+__device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Settings& c, Maxima& maxima, int key_bits,
+                                          Scratch& s) {
   const int tid = threadIdx.x;
   RowState st{};
   if (c.greedy || !(c.k_on || c.p_on)) {
@@ -470,39 +515,8 @@ __device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Set
     return st;
   }
   st.from = c.low;
-  if (c.by_tiles) {  // the top_k-th largest maximum: the least of those with fewer than top_k above them
-    const float* tile_max = a.tile_max + (size_t)r * a.tiles;
-    const int quads = (a.tiles + 3) / 4;
-    for (int i = tid; i < 4 * quads; i += kThreads) maxima[i] = i < a.tiles ? tile_max[i] : -INFINITY;
-    __syncthreads();
-    const float v0 = maxima[min(tid, a.tiles - 1)], v1 = maxima[min(tid + kThreads, a.tiles - 1)];
-    int above0 = 0, above1 = 0;
-    if (a.tiles <= kThreads) {
-#pragma unroll 8
-      for (int q = 0; q < quads; ++q) {
-        const f32x4_t m = reinterpret_cast<const f32x4_t*>(maxima)[q];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) above0 += m[e] > v0;
-      }
-      above1 = c.top_k;
-    } else {
-#pragma unroll 4
-      for (int q = 0; q < quads; ++q) {
-        const f32x4_t m = reinterpret_cast<const f32x4_t*>(maxima)[q];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          above0 += m[e] > v0;
-          above1 += m[e] > v1;
-        }
-      }
-    }
-    float least = fminf(above0 < c.top_k ? v0 : INFINITY, above1 < c.top_k ? v1 : INFINITY);
-    least = -wave_max(-least);
-    if ((tid & 63) == 0) s.red32[tid >> 6] = __float_as_uint(least);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kRowWaves; ++k) least = fminf(least, __uint_as_float(s.red32[k]));
-    __syncthreads();
+  if (c.by_tiles) {
+    const float least = kth_maximum(maxima, a.tiles, c.top_k, key_bits);
     st.todo = kToList;
     st.cut = kBins - 1;
     st.from = fmaxf(least, c.low);
@@ -560,17 +574,17 @@ __device__ __forceinline__ RowState decide(const SampleArgs& a, int r, const Set
 
 template <typename E>
 __global__ void __launch_bounds__(kThreads, 4) sample_scan_kernel(SampleArgs a) {
-  __shared__ __align__(16) float maxima[2 * kThreads];
   __shared__ uint64_t list[kList];
   __shared__ Scratch s;
   __shared__ uint32_t n, base;
   const int r = blockIdx.y, tid = threadIdx.x;
   RowState* state = a.state + 2 * r + a.round;
   if (a.round && state->todo == kDone) return;
+  Maxima maxima(a.tile_max + (size_t)r * a.tiles, a.tiles <= kMostTiles ? a.tiles : 0);  // (in flight with the settings)
   Settings c(a, r);
   RowState st;
   if (a.round == 0) {
-    st = decide(a, r, c, maxima, s);
+    st = decide(a, r, c, maxima, sizeof(E) == 2 ? 16 : 20, s);
     if (blockIdx.x == 0 && tid == 0) *state = st;
   } else {
     st = *state;
