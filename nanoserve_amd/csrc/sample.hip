@@ -15,7 +15,7 @@
 // hist is left out where no row needs it. top-p of a top-k longer than the list takes scan and
 // end twice. hist and scan skip tiles whose maximum does not matter to them. A bin with more tokens than
 // the list holds (flat rows, rows of few values) is cut by `end` alone, digit by digit of the key.
-// Measured: one row of 152064 bf16 with top-k 20 and top-p 0.8 17 us (max 3.4, scan 7.7, end 5: latency); 256 rows of
+// Measured: one row of 152064 bf16 with top-k 20 and top-p 0.8 16 us (max 3.4, scan 8, end 5: latency); 256 rows of
 // 151936 fp32 with settings of their own 158 to 167 us (max 25, at 6.3 TB/s, hist 33, scan 40, end 21, second scan 23, end 20).
 //  * Launches, each with little code, and not one kernel with a counter that finds a row's last workgroup:
 //    the fences that its data needs between the XCDs' L2 caches cost more (256 rows without a cut 407 us).
@@ -462,8 +462,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_hist_kernel(SampleArgs a) 
 }
 
 // ------------------------------------------------------------------ scan
-// The k-th largest tile maximum, down to its key's upper bits (for bf16 exactly): the largest value of so many bits that at
-// least k maxima reach, bit by bit. Each wave by itself, the maxima in registers.
+// A row's tile maxima, dealt to the lanes of each wave.
 struct Maxima {
   static constexpr int kPer = kMostTiles / kWave;
   uint32_t key[kPer];
@@ -480,6 +479,9 @@ struct Maxima {
       }
   }
 };
+// The k-th largest tile maximum, down to its key's upper bits (for bf16 exactly): the largest value of so many bits that at
+// least k maxima reach, two bits at a time. Each wave by itself, the maxima in registers (us, against ranking every
+// maximum among all of them in LDS: one row of 152064 with top-k 20 16.7 -> 16.2, of 409600 with top-k 600 49 -> 40).
 __device__ __forceinline__ float kth_maximum(Maxima& m, int tiles, int k, int bits) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -487,7 +489,7 @@ __device__ __forceinline__ float kth_maximum(Maxima& m, int tiles, int k, int bi
     if (kWave * (i & ~3) < tiles) m.key[i] = lane + kWave * i < tiles ? key_of(__uint_as_float(m.key[i])) : 0;
   uint32_t t = 0;
 #pragma unroll 1
-  for (int bit = 30; bit >= 32 - bits; bit -= 2) {  // two bits at a time
+  for (int bit = 30; bit >= 32 - bits; bit -= 2) {
     const uint32_t n1 = t | 1u << bit, n2 = t | 2u << bit, n3 = t | 3u << bit;
     int c1 = 0, c2 = 0, c3 = 0;
 #pragma unroll
@@ -918,6 +920,10 @@ __global__ void __launch_bounds__(kThreads) sample_end_kernel(SampleArgs a) {
   const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const RowState st = a.state[2 * r + a.round];
   if (a.round && st.todo == kDone) return;
+  // the list's beginning, in flight with the settings; meaningless where there is no list or past its length
+  const uint64_t* listed = a.list + ((size_t)r * 2 + a.round) * kList;
+  const uint32_t length = a.list_n[2 * r + a.round];
+  const uint64_t entry = listed[tid];
   Settings c(a, r);
   const Row<E> row{static_cast<const E*>(a.logits) + (size_t)r * a.row_stride, a.V};
   const float* tile_max = a.tile_max + (size_t)r * a.tiles;
@@ -947,8 +953,9 @@ __global__ void __launch_bounds__(kThreads) sample_end_kernel(SampleArgs a) {
     c.set_min_key();
     uint32_t n = 0;
     if (st.todo != kSum && st.todo != kSlow) {
-      n = a.list_n[2 * r + a.round];
-      for (uint32_t i = tid; i < n && n <= kList; i += kThreads) s.list[i] = a.list[((size_t)r * 2 + a.round) * kList + i];
+      n = length;
+      s.list[tid] = entry;
+      for (uint32_t i = tid + kThreads; i < n && n <= kList; i += kThreads) s.list[i] = listed[i];
       __syncthreads();
     }
     if (st.todo == kSlow || n > kList) {
