@@ -16,7 +16,7 @@
 // end twice. hist and scan skip tiles whose maximum does not matter to them. A bin with more tokens than
 // the list holds (flat rows, rows of few values) is cut by `end` alone, digit by digit of the key.
 // Measured: one row of 152064 bf16 with top-k 20 and top-p 0.8 16 us (max 3.4, scan 8, end 5: latency); 256 rows of
-// 151936 fp32 with settings of their own 158 to 167 us (max 25, at 6.3 TB/s, hist 33, scan 40, end 21, second scan 23, end 20).
+// 151936 fp32 with settings of their own 158 to 167 us (max 25, at 6.3 TB/s, hist 33, scan 39, end 21, second scan 22, end 20).
 //  * Launches, each with little code, and not one kernel with a counter that finds a row's last workgroup:
 //    the fences that its data needs between the XCDs' L2 caches cost more (256 rows without a cut 407 us).
 //  * Weights exp((l - max) / T) are rounded to multiples of 2^-42 and summed as integers: sums do not
