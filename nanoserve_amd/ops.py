@@ -143,6 +143,16 @@ def _device_of(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
     return here
 
 
+def _work_args(work) -> tuple:
+    """Address and size of a uint8 workspace as the library takes them, (None, 0) for None. One whose
+    elements are strided or repeated (an expanded byte) spans another range than its size says."""
+    if work is None:
+        return None, 0
+    if not work.is_contiguous():
+        raise ValueError("work must be contiguous")
+    return work.data_ptr(), work.numel()
+
+
 def _apart(out: torch.Tensor, t: torch.Tensor, name: str) -> None:
     """Raises if the contiguous out shares memory with t, whose last dimension is contiguous."""
     a, b = out.data_ptr(), t.data_ptr()
@@ -294,7 +304,7 @@ class Kernels:
             self._check(rc, "ns_w4_linear")
         else:
             rc = self.lib.ns_w4_linear_ws(x.data_ptr(), Wq.data_ptr(), S.data_ptr(), y.data_ptr(),
-                                          max(M, 1), N, K, group, work.data_ptr(), work.numel(),
+                                          max(M, 1), N, K, group, *_work_args(work),
                                           self._stream())
             self._check(rc, "ns_w4_linear_ws")
         return y if M else y[:0]
@@ -389,8 +399,8 @@ class Kernels:
         if out is None:
             out = torch.empty((1, n_heads * head_dim), dtype=torch.bfloat16, device=q.device)
         rc = self.lib.ns_decode_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                          pos.data_ptr(), out.data_ptr(), work.data_ptr(),
-                                          work.numel(), n_heads, n_kv_heads, head_dim,
+                                          pos.data_ptr(), out.data_ptr(), *_work_args(work),
+                                          n_heads, n_kv_heads, head_dim,
                                           k_cache.shape[-2], self._stream())
         self._check(rc, "ns_decode_attention")
         return out
@@ -435,7 +445,7 @@ class Kernels:
         rc = self.lib.ns_decode_qkv_attention(
             qkv.data_ptr(), None if bias is None else bias.data_ptr(), inv_freq.data_ptr(),
             pos.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-            work.data_ptr(), work.numel(), n_heads, n_kv_heads, head_dim, k_cache.shape[-2],
+            *_work_args(work), n_heads, n_kv_heads, head_dim, k_cache.shape[-2],
             1 if merge else 0, None if rot is None else _rot_ptr(rot, head_dim), self._stream())
         self._check(rc, "ns_decode_qkv_attention")
         return out
@@ -476,7 +486,7 @@ class Kernels:
         N, K = Wq.shape[0], Wq.shape[1] * 8
         if out is None:
             out = torch.empty((1, N), dtype=torch.bfloat16, device=Wq.device)
-        rc = self.lib.ns_w4_gemv_decode_attn(attn_out.data_ptr(), work.data_ptr(),
+        rc = self.lib.ns_w4_gemv_decode_attn(attn_out.data_ptr(), _work_args(work)[0],
                                              pos.data_ptr(), max_len, n_heads, Wq.data_ptr(),
                                              S.data_ptr(), out.data_ptr(), N, K, group,
                                              self._stream())
@@ -605,8 +615,7 @@ class Kernels:
                 raise ValueError(f"out must be a contiguous [{T}, {n_heads * 128}] tensor")
         rc = self.lib.ns_prompt_attention(
             q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0),
-            out.data_ptr(), None if work is None else work.data_ptr(),
-            0 if work is None else work.numel(), T, n_heads, Hk, pos0, self._stream())
+            out.data_ptr(), *_work_args(work), T, n_heads, Hk, pos0, self._stream())
         self._check(rc, "ns_prompt_attention")
         return out
 
@@ -737,8 +746,8 @@ class Kernels:
             q.data_ptr(), q.stride(0) if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
             *strides, n_pages, page_size, *table, lens.data_ptr(),
             None if q_start is None else q_start.data_ptr(), out.data_ptr(),
-            None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
-            Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
+            *_work_args(work), T, B, n_heads, Hk, D, shared, window, sinks,
+            D ** -0.5 if scale is None else scale, _raw_stream(here))
         self._check(rc, "ns_paged_attention")
         return out
 
@@ -797,8 +806,7 @@ class Kernels:
         else:
             _require_here(work, "work", torch.uint8, here)
         rc = self.lib.ns_sample(logits.data_ptr(), int(fp32), logits.stride(0) if B > 1 else V, u.data_ptr(),
-                                *args, out.data_ptr(), None if work is None else work.data_ptr(),
-                                0 if work is None else work.numel(), B, V, _raw_stream(here))
+                                *args, out.data_ptr(), *_work_args(work), B, V, _raw_stream(here))
         self._check(rc, "ns_sample")
         return out
 
