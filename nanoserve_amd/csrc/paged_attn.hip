@@ -9,6 +9,7 @@
 // lengths): every workgroup adds up the key blocks of the whole batch, takes the share per workgroup
 // that spreads them over `target` workgroups, and finds its own sequence, row tile and range of blocks
 // by a wave-wide prefix sum over the sequences. One long and fifteen short sequences then end together.
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 #include <stdint.h>
@@ -211,6 +212,12 @@ __device__ __forceinline__ void wait_loads(int n) {
   asm volatile("" ::: "memory");
 }
 
+// The maximum that stands for a range of keys from here on: -inf if and only if the row sees none of them. Scores
+// that are all -inf, or all NaN (which fmaxf passes over), leave -inf too; the lowest finite value in its place
+// keeps their sums (0 and NaN) in the merge, where they weigh nothing beside finite scores (0 * NaN is NaN) and
+// divide 0 by 0 alone.
+__device__ __forceinline__ float seen_max(float m, bool seen) { return seen ? fmaxf(m, -FLT_MAX) : -INFINITY; }
+
 // ------------------------------------------------------------------ one token per sequence
 // Up to 16 query heads per kv head, bound by HBM. A workgroup takes a range of 16-row blocks of one
 // sequence and kv head; each of its four waves streams every fourth block through its own LDS ring
@@ -314,6 +321,7 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
 #pragma unroll
   for (int d = 0; d < D / 16; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;  // of head r16
+  bool seen = false;             // a block of the wave had a page, and so a key that the token sees
   const int vrow = 4 * grp + (r16 >> 2);
   auto compute = [&](const uint16_t* ks, const uint16_t* vs, int key0) {
     f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
@@ -382,6 +390,7 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
   auto step = [&](auto stage, int i) {
     constexpr int S = decltype(stage)::value;
     wait_loads(2 * kLoads * min(cnt - 1 - i, kStages - 1));
+    seen |= at[S] >= 0;
     compute(lds.k[S] + wv * kBlk, lds.v[S] + wv * kBlk, at[S]);
     if (i + kStages < cnt) start(stage, i + kStages);
   };
@@ -405,6 +414,7 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
   }
   l += lane_xor16(l);
   l += lane_xor32(l);
+  m = seen_max(m, seen);
 
   // ---- merge of the waves through their (then free) first stages: fp32, heads 0 .. 7 in the K half and
   // 8 .. 15 in the V half
@@ -631,6 +641,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = -INFINITY, l = 0.f;
+  bool seen = false;  // the lane's row saw one of the lane's keys
   const float c = a.c;
 
   // transpose-read offsets (elements) of the 32-dim tiles at key row 4 kh + (lane % 16) / 4
@@ -669,6 +680,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
           const bool see = (key < hi) & (key >= k0) & ((key >= lo) | (key < first)) &
                            (((groups >> (2 * u + (r >> 3))) & 1) != 0);
           s[u][r] = see ? s[u][r] : -INFINITY;
+          seen |= see;
         }
     } else if (key0 + kTileKeys > hi_min || key0 < lo_max || key0 < k0) {  // positions from, .. to - 1
       const int from = max(lo, k0);
@@ -680,6 +692,9 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
           const uint32_t at = (uint32_t)(key0 + 4 * kh - from + 32 * u + 8 * (r >> 2) + (r & 3));
           s[u][r] = at < span ? s[u][r] : -INFINITY;
         }
+      seen |= max(from, key0) < min(hi, key0 + kTileKeys);
+    } else {
+      seen = true;
     }
     float bm = s[0][0];
 #pragma unroll
@@ -767,9 +782,11 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   }
 
   l += lane_xor32(l);
+  const uint64_t see_lanes = __ballot(seen);  // a row's keys are spread over lanes jq and 32 + jq
+  seen = ((see_lanes >> jq | see_lanes >> (32 + jq)) & 1) != 0;
   if (wrow + jq >= rows) return;
   if (direct) {
-    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    const float inv = seen ? 1.f / l : 0.f;
     uint16_t* op = a.out + ((size_t)t * a.Hq + hq) * D + 4 * kh;
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
@@ -788,7 +805,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
         *reinterpret_cast<f32x4_t*>(op + 32 * d + 2 * r) =
             f32x4_t{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
     if (kh == 0)
-      *reinterpret_cast<float2*>((kShared ? a.shml : a.ml) + 2 * pr) = make_float2(m * c, l);
+      *reinterpret_cast<float2*>((kShared ? a.shml : a.ml) + 2 * pr) = make_float2(seen_max(m * c, seen), l);
   }
   // (also where the result is final, so that the merge does not read an older launch's entry)
   if (!kShared && a.rows && split == 0 && hq == 0 && kh == 0)
@@ -869,7 +886,7 @@ __global__ void __launch_bounds__(kWavesPer > 1 ? 64 * kWavesPer : 256) paged_me
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const float f = exp2f(mv[u] - mz);
-      if (f > 0.f) {  // (a partial that counts nothing may repeat another's values)
+      if (mv[u] > -INFINITY) {  // (a partial that counts nothing may repeat another's values)
         l = fmaf(f, lv[u], l);
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = fmaf(f, ov[u][e], acc[e]);

@@ -716,8 +716,8 @@ class Kernels:
         With ``window`` a token sees the last ``window`` positions (its own among them) and the first
         ``sinks`` ones. ``shared``: the first ``shared`` positions, as far as a sequence has them, lie in
         the same pages for every sequence (the caller's statement); their keys and values are then read
-        once for the whole batch. A token that sees nothing gets zeros; rows past the last
-        sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be positive. ``work``: from
+        once for the whole batch. A token that sees nothing gets zeros, one whose query or seen keys hold
+        NaN gets NaN; rows past the last sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be positive. ``work``: from
         paged_attention_workspace, allocated here when it is not given. The reference has SDPA over one
         sequence's cache (qwen.py:124-133)."""
         here = _device_of(q, "q", torch.bfloat16)
