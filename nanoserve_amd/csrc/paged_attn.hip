@@ -10,7 +10,6 @@
 // that spreads them over `target` workgroups, and finds its own sequence, row tile and range of blocks
 // by a wave-wide prefix sum over the sequences. One long and fifteen short sequences then end together.
 #include <float.h>
-#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -55,6 +54,12 @@ constexpr int ring_stages() {
 struct Ring {
   uint16_t *k[4], *v[4];
 };
+// Of a tile over the shared prefix: each row's positions (from, up to; the first tokens besides), and the least
+// and highest of each wave's.
+struct SharedRows {
+  int2 limits[kTileRows];
+  int lim[4][2];
+};
 
 // The key blocks that some query of a range sees: positions k0 .. k1 - 1, of them those below `first`
 // or from `lo` on.
@@ -72,6 +77,17 @@ struct KeyBlocks {
   __device__ int block(int j) const { return j < na ? a0 + j : m0 + j - na; }
 };
 
+// The largest of the lanes' values, none below 0 (lanes shifted in from outside count as 0).
+__device__ __forceinline__ int wave_most(int m) {
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x111, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x112, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x114, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x118, 0xf, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x142, 0xa, 0xf, false));
+  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(m, 63);
+}
+
 // One of the longest sequences: its table row has every shared position that any sequence has.
 __device__ __forceinline__ int longest(const PagedArgs& a) {
   const int lane = __lane_id();
@@ -83,14 +99,7 @@ __device__ __forceinline__ int longest(const PagedArgs& a) {
       at = b;
     }
   }
-  int m = max(most, 0);  // (lanes shifted in from outside count as 0)
-  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x111, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x112, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x114, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x118, 0xf, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x142, 0xa, 0xf, false));
-  m = max(m, __builtin_amdgcn_update_dpp(0, m, 0x143, 0xc, 0xf, false));
-  return __builtin_amdgcn_readlane(at, __builtin_ctzll(__ballot(most == __builtin_amdgcn_readlane(m, 63))));
+  return __builtin_amdgcn_readlane(at, __builtin_ctzll(__ballot(most == wave_most(max(most, 0)))));
 }
 
 __device__ __forceinline__ int low_limit(const PagedArgs& a, int pos) {
@@ -190,6 +199,17 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
     slot += __builtin_amdgcn_readlane(wave_scan(slots), kWave - 1);
   }
   return false;
+}
+
+// The lanes' bits together.
+__device__ __forceinline__ uint32_t wave_or(uint32_t v) {
+  v |= __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v |= __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v |= __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v |= __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v |= __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v |= __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return __builtin_amdgcn_readlane(v, 63);
 }
 
 // attn_lds_load16 for rows that one workgroup reads, once.
@@ -472,14 +492,16 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
 //  * Probabilities enter as two bf16 terms (16 significant bits): the error is then the output's own rounding, for
 //    1.5 times the products of one term.
 //  * A row sees positions below `hi` and from `lo` on or below `sinks`; blocks that no row of the tile
-//    sees are left out of its list, blocks that all rows see whole skip the comparisons.
+//    sees are left out of its list, blocks that all rows see whole skip the comparisons. Windows of different
+//    sequences over the shared prefix may lie apart: the positions between them stay in the list, and their rows
+//    are not read but zero, as a value there (it may be NaN) would reach every row through 0 * NaN.
 // Measured (28 / 4 heads of 128): prompts of 5 sequences of 2000 to 8000 654 us, 677 TFLOP/s, with the second term
 // 1015 (a large library product: 1265); matrix cores busy in half of the cycles and vector units in 58 %, at 1.8 GHz.
 // Issuing one half block's softmax between the products of its neighbours did not help (659 -> 681 to 730 us): the
 // other wave of the SIMD fills those slots already. 4095 tokens with a window of 1000 and 14 / 2 heads of 64 43 us;
 // 96 drafts of 1 to 3 tokens behind 16384 shared positions 108 us.
 template <int D, bool kShared>
-__device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, int (&lim)[4][2]) {
+__device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
   constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad, kDT = D / 32,
                 kStages = ring_stages<D>();
   const int tid = threadIdx.x, lane = tid & 63;
@@ -539,26 +561,32 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   // limits over the wave's rows and over the tile's: a sequence's positions rise with its rows, the rows of
   // the whole batch need a look at each
   int hi_min, hi_max, lo_min, lo_max, top, low;
+  bool gaps = false;  // there may be positions between the rows' windows that no row sees
   if constexpr (kShared) {
-    hi_min = counts ? hi : INT_MAX, hi_max = hi, lo_min = real ? lo : INT_MAX, lo_max = real ? lo : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      hi_min = min(hi_min, __shfl_xor(hi_min, o, kWave));
-      hi_max = max(hi_max, __shfl_xor(hi_max, o, kWave));
-      lo_min = min(lo_min, __shfl_xor(lo_min, o, kWave));
-      lo_max = max(lo_max, __shfl_xor(lo_max, o, kWave));
-    }
-    hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-    hi_max = __builtin_amdgcn_readfirstlane(hi_max);
-    lo_min = __builtin_amdgcn_readfirstlane(lo_min);
-    lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    // (a row whose window begins past the prefix sees the first tokens of it alone)
+    const int far = a.s.width * a.s.page_size;
+    hi_min = k1 - wave_most(counts ? k1 - hi : 0);
+    hi_max = wave_most(lo < hi ? hi : min(first, hi));
+    lo_min = far - wave_most(real ? far - lo : 0);
+    lo_max = wave_most(real ? lo : 0);
+    if (kh == 0) sh.limits[32 * wv + jq] = make_int2(lo, hi);
     if (lane == 0) {
-      lim[wv][0] = hi_max;
-      lim[wv][1] = lo_min;
+      sh.lim[wv][0] = hi_max;
+      sh.lim[wv][1] = lo_min;
     }
     lds_sync();
-    top = __builtin_amdgcn_readfirstlane(max(max(lim[0][0], lim[1][0]), max(lim[2][0], lim[3][0])));
-    low = __builtin_amdgcn_readfirstlane(min(min(lim[0][1], lim[1][1]), min(lim[2][1], lim[3][1])));
+    top = __builtin_amdgcn_readfirstlane(max(max(sh.lim[0][0], sh.lim[1][0]), max(sh.lim[2][0], sh.lim[3][0])));
+    if (a.window > 0) {  // none if every window begins at or before the first end of one
+      int start = 0, back = 0;
+#pragma unroll
+      for (int u = 0; u < kTileRows; u += kWave) {
+        const int2 x = sh.limits[u + lane];
+        start = max(start, x.x < x.y ? x.x : 0);
+        back = max(back, x.x < x.y ? k1 - x.y : 0);
+      }
+      gaps = wave_most(start) + wave_most(back) > k1;
+    }
+    low = __builtin_amdgcn_readfirstlane(min(min(sh.lim[0][1], sh.lim[1][1]), min(sh.lim[2][1], sh.lim[3][1])));
   } else {
     const int p0 = sp.n - sp.nn;  // of the sequence's first new token; below 0 with more of them than positions
     const int wfirst = p0 + min(wrow, rows - 1) / R, wlast = p0 + min(wrow + 31, rows - 1) / R;
@@ -606,12 +634,27 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     k_off[p] = r * 2 * D + 16u * (ch ^ k_swz(16 * wv + r));
     v_off[p] = r * 2 * D + 16u * (ch ^ v_swz(r));
   }
+  // Bit i: some row of the tile sees position key0 + i, i < 16.
+  auto seen16 = [&](int key0) {
+    auto below = [&](int limit) { return (1u << min(max(limit - key0, 0), 16)) - 1; };
+    uint32_t bits = 0;
+#pragma unroll
+    for (int u = 0; u < kTileRows; u += kWave) {
+      const int2 x = sh.limits[u + lane];
+      bits |= (below(x.y) & ~below(x.x)) | below(min(first, x.y));
+    }
+    return wave_or(bits);
+  };
   auto issue = [&](uint16_t* ks, uint16_t* vs, int j, uint32_t& groups) {
     const int jj = j - j0;
     if ((jj & 15) == 0) refill(j);
     const int e = 4 * (jj & 15);
     groups = (uint32_t)(valid >> e) & 15u;
-    const bool ok = (groups >> wv) & 1;
+    const int key0 = kTileKeys * kb.block(j) + 16 * wv;
+    uint32_t sees = 0xffffu;
+    if constexpr (kShared)
+      if (gaps) sees = seen16(key0);
+    const bool ok = ((groups >> wv) & 1) != 0 && sees != 0;
     const uint64_t off = ok ? (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(offs >> 32), e + wv) << 32 |
                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)offs, e + wv)
                             : 0;
@@ -621,15 +664,15 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
                                                         ok ? 32 * D : 0, 0x00020000);
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) attn_lds_load16(kres, &ks[16 * wv * D + 512 * p], k_off[p], 0);
-    const int key0 = kTileKeys * kb.block(j) + 16 * wv;
-    if (key0 >= k0 && key0 >= low && key0 + 16 <= top) {
+    if (gaps ? sees == 0xffffu : key0 >= k0 && key0 >= low && key0 + 16 <= top) {
 #pragma unroll
       for (int p = 0; p < kLoads; ++p) attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], v_off[p], 0);
     } else {  // value rows that no row of the tile sees are zero, whatever the page holds
 #pragma unroll
       for (int p = 0; p < kLoads; ++p) {
         const int key = key0 + kRowsPerLoad * p + lr;
-        const bool see = (key >= k0) & (key < top) & ((key >= low) | (key < first));
+        const bool see = gaps ? ((sees >> (key - key0)) & 1) != 0
+                              : (key >= k0) & (key < top) & ((key >= low) | (key < first));
         attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], see ? v_off[p] : kOut, 0);
       }
     }
@@ -819,12 +862,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedArgs a) {
   constexpr int kArr = kTileKeys * D, kFour = ring_stages<D>() > 2 ? kArr : 8;
   __shared__ __align__(16) uint16_t k0[kArr], v0[kArr], k1[kArr], v1[kArr], k2[kFour], v2[kFour], k3[kFour], v3[kFour];
   __shared__ float red[2][kOneWaves][16];
-  __shared__ int lim[4][2];
+  __shared__ SharedRows sh;
   const Ring lds{{k0, k1, k2, k3}, {v0, v1, v2, v3}};
   int id = blockIdx.x;
   if constexpr (kWithShared) {
     if (id < a.sh_grid) {
-      tile_body<D, true>(a, id / a.Hk, id % a.Hk, lds, lim);
+      tile_body<D, true>(a, id / a.Hk, id % a.Hk, lds, sh);
       return;
     }
     id -= a.sh_grid;
@@ -832,7 +875,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PagedArgs a) {
   if constexpr (kOne)
     one_body<D>(a, id / a.Hk, id % a.Hk, lds, red);
   else
-    tile_body<D, false>(a, id / a.Hk, id % a.Hk, lds, lim);
+    tile_body<D, false>(a, id / a.Hk, id % a.Hk, lds, sh);
 }
 
 // ------------------------------------------------------------------ merge of the partials

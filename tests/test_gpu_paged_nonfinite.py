@@ -164,3 +164,29 @@ def test_nothing_seen_beside_nan(kernels, Hq, Hk, D):
         got = _attend(kernels, batch, q[:28], Hq, shared).view(28, Hq, D)
         assert bool((got[:4] == 0).all())
         assert bool(torch.isnan(got[4:28:2]).all()) and bool(torch.isfinite(got[5:28:2]).all())
+
+
+# ------------------------------------------------------------------ a shared prefix seen through windows
+# Sequences whose windows end inside the prefix, or begin past it: the positions between them are seen by none.
+@pytest.mark.parametrize("Hq,Hk,D", LAYOUTS)
+@pytest.mark.parametrize("sinks", [0, 3, 70])
+@pytest.mark.parametrize("lens,new,shared", [
+    ([300, 1000], None, 900), ([300, 1000, 650], None, 1000), ([64, 2000, 130, 64], None, 1500),
+    ([300, 1000, 420], [3, 1, 40], 900), ([1300, 200, 700], [1, 4, 30], 1200), ([1000, 990, 1100], None, 900)])
+def test_shared_window_gaps(kernels, lens, new, shared, sinks, Hq, Hk, D):
+    window = 60
+    batch = R.PagedBatch(lens, new, Hk, D, 16, shared=shared, seed=sinks)
+    seen = torch.zeros(max(lens), dtype=torch.bool)
+    for _, b, p in batch.rows():
+        j = torch.arange(max(lens))
+        seen |= (j <= p) & ((j > p - window) | (j < sinks))
+    at = lens.index(max(lens))
+    gone = [j for j in range(min(shared, max(lens))) if not seen[j]]
+    assert gone
+    q = _queries(batch.T, Hq, D, 6)
+    want = formula(batch, q, Hq, window, sinks)
+    for value in (NAN, INF):
+        for j in gone:
+            for pool in (batch.k, batch.v):
+                _set(batch, pool, at, j, value)
+        _check(_attend(kernels, batch, q, Hq, shared, window=window, sinks=sinks), want)
