@@ -190,3 +190,37 @@ def test_shared_window_gaps(kernels, lens, new, shared, sinks, Hq, Hk, D):
             for pool in (batch.k, batch.v):
                 _set(batch, pool, at, j, value)
         _check(_attend(kernels, batch, q, Hq, shared, window=window, sinks=sinks), want)
+
+
+# ------------------------------------------------------------------ padding and bad tables behind a shared prefix
+@pytest.mark.parametrize("Hq,Hk,D", LAYOUTS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 2)])
+@pytest.mark.parametrize("lens,new,shared", [([150, 140, 103], [10, 40, 3], 100), ([700, 650, 640], [2, 1, 0], 640),
+                                             ([3, 90, 2], [8, 20, 5], 64)])
+def test_shared_prefix_with_rows_of_no_sequence(kernels, lens, new, shared, window, sinks, Hq, Hk, D):
+    """Rows behind the last sequence keep what they hold and do not reach the others, also where they are NaN;
+    more new tokens than positions see nothing."""
+    batch = R.PagedBatch(lens, new, Hk, D, 16, shared=shared, seed=1)
+    T = batch.T + 60
+    q = _queries(T, Hq, D, 3)
+    q[batch.T:] = NAN
+    out = torch.full((T, Hq * D), 7.0, dtype=BF16, device="cuda")
+    kernels.paged_attention(q, batch.k, batch.v, batch.table, batch.lens, Hq, q_start=batch.q_start, out=out,
+                            shared=shared, window=window, sinks=sinks)
+    assert bool((out[batch.T:] == 7).all())
+    _check(out[:batch.T], formula(batch, q[:batch.T], Hq, window, sinks))
+
+
+@pytest.mark.parametrize("Hq,Hk,D", LAYOUTS)
+@pytest.mark.parametrize("new", [None, [3, 40, 1]])
+def test_entries_outside_the_pool_in_a_shared_prefix(kernels, new, Hq, Hk, D):
+    """Their positions are left out for every sequence."""
+    batch = R.PagedBatch([300, 350, 290], new, Hk, D, 16, shared=256, seed=5)
+    q = _queries(batch.T, Hq, D, 7)
+    for entry in (-1, batch.k.shape[0], (1 << 31) - 1):
+        for pages in ([0], [3, 4], list(range(16))):
+            table = batch.table.clone()
+            table[:, pages] = entry
+            want = formula(batch, q, Hq, hidden=lambda b, j: torch.isin(j // 16, torch.tensor(pages)))
+            got = kernels.paged_attention(q, batch.k, batch.v, table, batch.lens, Hq, q_start=batch.q_start, shared=256)
+            _check(got, want)
