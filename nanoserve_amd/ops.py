@@ -143,6 +143,12 @@ def _device_of(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
     return here
 
 
+def _int32(n: int) -> int:
+    """n held to 32 bits, for counts where more than every position means no more than that (the library's
+    argument would keep the low bits alone)."""
+    return max(-(1 << 31), min(n, (1 << 31) - 1))
+
+
 def _work_args(work) -> tuple:
     """Address and size of a uint8 workspace as the library takes them, (None, 0) for None. One whose
     elements are strided or repeated (an expanded byte) spans another range than its size says."""
@@ -703,8 +709,8 @@ class Kernels:
         """A uint8 device tensor of the workspace paged_attention uses for these sizes (max_len: table
         width * page_size; ragged: with q_start), or None. Launches that may overlap in time need
         workspaces of their own."""
-        n = int(self.lib.ns_paged_attention_workspace(T, B, n_heads, n_kv_heads, head_dim, max_len,
-                                                      int(ragged), shared))
+        n = int(self.lib.ns_paged_attention_workspace(T, B, n_heads, n_kv_heads, head_dim, _int32(max_len),
+                                                      int(ragged), _int32(shared)))
         return torch.empty(n, dtype=torch.uint8, device=device or "cuda") if n else None
 
     def paged_attention(self, q, k_pages, v_pages, pages, lens, n_heads, q_start=None, shared=0,
@@ -717,9 +723,9 @@ class Kernels:
         ``sinks`` ones. ``shared``: the first ``shared`` positions, as far as a sequence has them, lie in
         the same pages for every sequence (the caller's statement); their keys and values are then read
         once for the whole batch. A token that sees nothing gets zeros, one whose query or seen keys hold
-        NaN gets NaN; rows past the last sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be positive. ``work``: from
-        paged_attention_workspace, allocated here when it is not given. The reference has SDPA over one
-        sequence's cache (qwen.py:124-133)."""
+        NaN gets NaN; rows past the last sequence's are left alone. ``scale`` (default 1 / sqrt(D)) must be
+        positive. ``work``: from paged_attention_workspace, allocated here when it is not given. The
+        reference has SDPA over one sequence's cache (qwen.py:124-133)."""
         here = _device_of(q, "q", torch.bfloat16)
         if q.dim() != 2 or q.stride(1) != 1:
             raise ValueError("q must be [T, Hq * D] with contiguous rows")
@@ -746,7 +752,7 @@ class Kernels:
             q.data_ptr(), q.stride(0) if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
             *strides, n_pages, page_size, *table, lens.data_ptr(),
             None if q_start is None else q_start.data_ptr(), out.data_ptr(),
-            *_work_args(work), T, B, n_heads, Hk, D, shared, window, sinks,
+            *_work_args(work), T, B, n_heads, Hk, D, _int32(shared), _int32(window), _int32(sinks),
             D ** -0.5 if scale is None else scale, _raw_stream(here))
         self._check(rc, "ns_paged_attention")
         return out

@@ -69,3 +69,22 @@ def test_workspace_must_be_contiguous(stub, call, work):
         call(stub, work)
     assert not any(not n.endswith("_workspace") for n in stub.lib.calls)
     call(stub, torch.zeros(1 << 20, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("n,held", [((1 << 31) + 5, (1 << 31) - 1), ((1 << 32) + 16, (1 << 31) - 1),
+                                    (1 << 40, (1 << 31) - 1), (-(1 << 32), -(1 << 31)), (4096, 4096), (0, 0)])
+def test_counts_past_32_bits(stub, n, held):
+    """A window, first tokens or a prefix of more than 32 bits are as many as can be, not their low bits."""
+    _attend(stub, window=n, sinks=n, shared=n)
+    assert stub.lib.calls["ns_paged_attention"][-5:-2] == (held, held, held)
+    assert stub.lib.calls["ns_paged_attention_workspace"][-1] == held
+
+
+def test_negative_counts_past_32_bits_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_require_gpu_tensor", lambda *a: None)
+    monkeypatch.setattr(ops, "_current_device", lambda: -1)
+    monkeypatch.setattr(ops, "_raw_stream", lambda device: 0)
+    work = torch.zeros(1 << 20, dtype=torch.uint8)
+    for kw in (dict(window=-(1 << 32)), dict(sinks=-(1 << 33)), dict(shared=-(1 << 32))):
+        with pytest.raises(RuntimeError, match="-2"):
+            _attend(Kernels(), work=work, **kw)
