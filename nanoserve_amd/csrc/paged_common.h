@@ -59,7 +59,10 @@ inline bool batch_ok(const Batch& s, const Pools& p, int Hk, int D) {
   if (p.page_stride % 8 || p.head_stride % 8 || p.page_stride < 0 || p.head_stride < 0) return false;
   // pages and heads do not overlap, whichever of the two is the outer one
   const long long head = (long long)s.page_size * D;
-  return (Hk == 1 || p.head_stride >= head) && (p.n_pages == 1 || p.page_stride >= head);
+  if ((Hk > 1 && p.head_stride < head) || (p.n_pages > 1 && p.page_stride < head)) return false;
+  if (p.page_stride >> 46 || p.head_stride >> 46) return false;  // past any address
+  return Hk == 1 || p.n_pages == 1 || (__int128)(Hk - 1) * p.head_stride + head <= p.page_stride ||
+         (__int128)(p.n_pages - 1) * p.page_stride + head <= p.head_stride;
 }
 
 }  // namespace ns

@@ -88,3 +88,59 @@ def test_negative_counts_past_32_bits_are_refused(monkeypatch):
     for kw in (dict(window=-(1 << 32)), dict(sinks=-(1 << 33)), dict(shared=-(1 << 32))):
         with pytest.raises(RuntimeError, match="-2"):
             _attend(Kernels(), work=work, **kw)
+
+
+# ------------------------------------------------------------------ entry points, with addresses that are apart
+# 0.25 GiB apart, never dereferenced: the calls that pass the checks end at the missing GPU
+def _address(i):
+    return (i + 1) << 28
+
+
+on_cpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are no memory")
+ATTEND = dict(q=_address(0), qs=512, k=_address(1), v=_address(2), ps=4096, hs=2048, n=8, page=16, tab=_address(3), ts=4,
+              w=4, lens=_address(4), start=None, out=_address(5), work=_address(6), bytes=1 << 20, T=3, B=3, Hq=4, Hk=2,
+              D=128, shared=0, window=0, sinks=0, scale=0.1)
+APPEND = dict(qkv=_address(0), qs=1024, bias=_address(7), inv=_address(8), start=None, lens=_address(4),
+              tab=_address(3), ts=4, w=4, k=_address(1), v=_address(2), ps=4096, hs=2048, n=8, page=16, out=_address(5),
+              T=3, B=3, Hq=4, Hk=2, D=128)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return Kernels().lib
+
+
+def _attention(lib, **kw):
+    a = {**ATTEND, **kw}
+    return lib.ns_paged_attention(
+        a["q"], a["qs"], a["k"], a["v"], a["ps"], a["hs"], a["n"], a["page"], a["tab"], a["ts"], a["w"],
+        a["lens"], a["start"], a["out"], a["work"], a["bytes"], a["T"], a["B"], a["Hq"], a["Hk"], a["D"],
+        a["shared"], a["window"], a["sinks"], a["scale"], None)
+
+
+def _append(lib, **kw):
+    a = {**APPEND, **kw}
+    return lib.ns_paged_append(
+        a["qkv"], a["qs"], a["bias"], a["inv"], a["start"], a["lens"], a["tab"], a["ts"], a["w"], a["k"],
+        a["v"], a["ps"], a["hs"], a["n"], a["page"], a["out"], a["T"], a["B"], a["Hq"], a["Hk"], a["D"], None)
+
+
+# strides in elements for 8 pages and 2 heads of 2048: pages outside, heads outside, either padded; a lone page or
+# head has no stride
+@on_cpu
+@pytest.mark.parametrize("call", [_attention, _append])
+@pytest.mark.parametrize("ok", [
+    dict(), dict(ps=2048, hs=16384), dict(ps=4104), dict(ps=4608, hs=2560), dict(ps=2056, hs=16440), dict(n=1, ps=0),
+    dict(n=1, ps=8), dict(n=1 << 30, ps=1 << 45)], ids=str)
+def test_pool_strides_are_taken(lib, call, ok):
+    assert call(lib, **ok) not in (0, -2)
+
+
+@pytest.mark.parametrize("call", [_attention, _append])
+@pytest.mark.parametrize("bad", [
+    dict(ps=2048), dict(ps=4088), dict(ps=2048, hs=16376), dict(ps=2048, hs=4096), dict(ps=2056),
+    dict(ps=2048, hs=2056), dict(ps=0), dict(hs=0), dict(ps=1 << 50), dict(hs=1 << 62)], ids=str)
+def test_pages_and_heads_that_overlap_are_refused(lib, call, bad):
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are no memory")
+    assert call(lib, **bad) == -2
