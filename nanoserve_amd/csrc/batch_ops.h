@@ -39,7 +39,8 @@ extern "C" {
  * name the same page for a row that both write leave one of the two values of each element there.
  * -2 for D % 16, D > 512, sizes <= 0, page_size % 16, strides that are not a multiple of 8 or shorter
  * than what they span, width * page_size >= 2^30, NULL or misaligned pointers (bf16 16, int 4 bytes),
- * q_start NULL with T != B.
+ * q_start NULL with T != B; pools that share rows with each other, with q_out or with an input, and q_out over an input
+ * (qkv counts from its first value to its last, what lies between its rows included).
  */
 int ns_paged_append(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq,
                     const int* q_start, const int* lens, const int* table, long long table_stride,
@@ -69,7 +70,8 @@ size_t ns_paged_attention_workspace(int T, int B, int Hq, int Hk, int D, int max
  * where the exact result is infinite: the second term of a probability is zero or negative), and may do so to the
  * tokens of the same kv head in its launch tile that do not see it.
  * -2 for D other than 64 and 128, Hq % Hk, negative window, sinks or shared, scale not positive and finite,
- * and as ns_paged_append; work_bytes too small.
+ * and as ns_paged_append (the pools may be one and the same here); work_bytes too small; out and the workspace
+ * over each other or over an input.
  */
 int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool,
                        long long page_stride, long long head_stride, int n_pages, int page_size,
@@ -101,7 +103,8 @@ size_t ns_sample_workspace(int B, int V, int fp32);
  * Weights are held in units of 2^-42 of the largest in 64-bit integers and summed exactly, so the token
  * does not depend on the order of any sum.
  * -2 for B <= 0, B > 65535, V <= 0, V > 2^20, row_stride < V, NULL or misaligned pointers (logits 2 or 4
- * bytes, int and float 4, work 16), work_bytes too small.
+ * bytes, int and float 4, work 16), work_bytes too small, out over the logits (from the first row to the last),
+ * the workspace over anything else.
  */
 int ns_sample(const void* logits, int fp32, long long row_stride, const float* u, const float* temps,
               float temp, const int* top_ks, int top_k, const float* top_ps, float top_p,

@@ -142,6 +142,14 @@ extern "C" int ns_paged_append(const void* qkv, long long qkv_stride, const void
       !ns::aligned(q_out, 16))
     return -2;
   if (qkv_stride % 8 || qkv_stride < (Hq + 2ll * Hk) * D) return -2;
+  const long long head = (long long)page_size * D;
+  const ns::Bytes x = ns::rows_of(qkv, T, qkv_stride, (Hq + 2ll * Hk) * D, 2),
+                  y = ns::bytes_of(q_out, 2 * (size_t)T * Hq * D), w = ns::bytes_of(bias, 2 * (Hq + 2ull * Hk) * D),
+                  f = ns::bytes_of(inv_freq, 2 * (size_t)D);
+  for (const ns::Bytes r : {x, y, w, f, ns::lens_of(a.s), ns::starts_of(a.s), ns::table_of(a.s)})
+    if (!ns::pool_apart(a.p.k, a.p, Hk, head, r) || !ns::pool_apart(a.p.v, a.p, Hk, head, r)) return -2;
+  if (!ns::apart(y, x) || !ns::apart(y, w) || !ns::apart(y, f)) return -2;
+  if (!ns::pools_apart(a.p, Hk, head) || !ns::metadata_apart(a.s, y)) return -2;
   a.qkv = static_cast<const uint16_t*>(qkv);
   a.bias = static_cast<const uint16_t*>(bias);
   a.inv_freq = static_cast<const float*>(inv_freq);

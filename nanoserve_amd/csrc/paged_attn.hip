@@ -1092,6 +1092,13 @@ int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, co
     a.ml = a.shpart + (size_t)p.sh_splits * T * Hq * D;
     a.shml = a.ml + (size_t)p.cap * Hq * 2;
   }
+  const ns::Bytes y = ns::bytes_of(out, 2 * (size_t)T * Hq * D), w = ns::bytes_of(p.bytes ? work : nullptr, p.bytes);
+  for (const ns::Bytes r : {y, w}) {
+    if (!ns::apart(r, ns::rows_of(q, T, q_stride, (long long)Hq * D, 2)) || !ns::metadata_apart(a.s, r)) return -2;
+    for (const uint16_t* pool : {a.p.k, a.p.v})
+      if (!ns::pool_apart(pool, a.p, Hk, (long long)page_size * D, r)) return -2;
+  }
+  if (!ns::apart(y, w)) return -2;
   a.cap = p.cap;
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_stride;

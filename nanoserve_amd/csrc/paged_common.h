@@ -5,6 +5,7 @@
 
 #include <algorithm>
 
+#include "spans.h"
 #include "w4_common.h"
 
 namespace ns {
@@ -63,6 +64,47 @@ inline bool batch_ok(const Batch& s, const Pools& p, int Hk, int D) {
   if (p.page_stride >> 46 || p.head_stride >> 46) return false;  // past any address
   return Hk == 1 || p.n_pages == 1 || (__int128)(Hk - 1) * p.head_stride + head <= p.page_stride ||
          (__int128)(p.n_pages - 1) * p.page_stride + head <= p.head_stride;
+}
+
+// The offsets i * page_stride + j * head_stride, |i| < n_pages and |j| < Hk, hold one in (lo, hi)? All in bytes;
+// i and j from 0 on with `down` false.
+inline bool pool_offset_in(const Pools& p, int Hk, bool down, __int128 lo, __int128 hi) {
+  const __int128 page = 2 * (__int128)p.page_stride, head = 2 * (__int128)p.head_stride;
+  const long long pages = p.n_pages - 1, heads = Hk - 1;
+  const __int128 far = (pages ? pages * page : 0) + (heads ? heads * head : 0);
+  if (lo >= far || hi <= (down ? -far : 0)) return false;  // (where the pools' spans are apart: no loop)
+  for (long long j = down ? -heads : 0; j <= heads; ++j) {
+    const __int128 from = lo - (heads ? j * head : 0), to = hi - (heads ? j * head : 0);
+    __int128 i = 0;
+    if (pages) {  // the first i past `from`
+      i = from / page - (from % page < 0) + 1;
+      i = std::max<__int128>(i, down ? -pages : 0);
+    }
+    const __int128 at = pages ? i * page : 0;
+    if (i <= pages && from < at && at < to) return true;
+  }
+  return false;
+}
+
+// Whether none of the pool's pages lies in a range.
+inline bool pool_apart(const uint16_t* pool, const Pools& p, int Hk, long long head, Bytes x) {
+  const __int128 from = (__int128)x.lo - reinterpret_cast<uintptr_t>(pool), size = 2 * (__int128)head;
+  return x.lo >= x.hi || !pool_offset_in(p, Hk, false, from - size, from + (x.hi - x.lo));
+}
+
+inline Bytes lens_of(const Batch& s) { return bytes_of(s.lens, 4 * (size_t)s.B); }
+inline Bytes starts_of(const Batch& s) { return bytes_of(s.q_start, 4 * ((size_t)s.B + 1)); }
+inline Bytes table_of(const Batch& s) { return rows_of(s.table, s.B, s.table_stride, s.width, 4); }
+// What a call writes (x) against the batch's metadata.
+inline bool metadata_apart(const Batch& s, Bytes x) {
+  return apart(x, lens_of(s)) && apart(x, starts_of(s)) && apart(x, table_of(s));
+}
+
+// Whether K and V share no element: a page of V starts less than a page before or behind one of K nowhere.
+inline bool pools_apart(const Pools& p, int Hk, long long head) {
+  const __int128 d = (__int128)reinterpret_cast<uintptr_t>(p.v) - reinterpret_cast<uintptr_t>(p.k),
+                 size = 2 * (__int128)head;
+  return !pool_offset_in(p, Hk, true, d - size, d + size);
 }
 
 }  // namespace ns

@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #include "batch_ops.h"
+#include "spans.h"
 #include "w4_common.h"
 #include "w4_kernels.h"
 
@@ -1108,6 +1109,13 @@ int ns_sample(const void* logits, int fp32, long long row_stride, const float* u
       !ns::aligned(top_ks, 4) || !ns::aligned(top_ps, 4) || !ns::aligned(min_ps, 4) || !ns::aligned(out, 4))
     return -2;
   if (!work || !ns::aligned(work, 16) || work_bytes < ns_sample_workspace(B, V, fp32)) return -2;
+  const size_t elt = fp32 ? 4 : 2, row = 4 * static_cast<size_t>(B);
+  const ns::Bytes y = ns::bytes_of(out, row), w = ns::bytes_of(work, ns_sample_workspace(B, V, fp32)),
+                  x = ns::rows_of(logits, B, row_stride, V, elt);
+  if (!ns::apart(x, y) || !ns::apart(x, w) || !ns::apart(y, w)) return -2;
+  for (const void* p : {static_cast<const void*>(u), static_cast<const void*>(temps), static_cast<const void*>(top_ks),
+                        static_cast<const void*>(top_ps), static_cast<const void*>(min_ps)})
+    if (!ns::apart(w, ns::bytes_of(p, row))) return -2;
   ns::SampleArgs a{logits, row_stride, u, temps, top_ps, min_ps, top_ks, out, temp, top_p, min_p, top_k, V};
   a.tiles = ns::row_tiles(V);
   a.parts = ns::row_parts(B, V, temps || top_ks || top_ps || min_ps);

@@ -144,3 +144,76 @@ def test_pages_and_heads_that_overlap_are_refused(lib, call, bad):
     if torch.cuda.is_available():
         pytest.skip("the addresses are no memory")
     assert call(lib, **bad) == -2
+
+
+@on_cpu
+def test_tensors_that_are_apart_are_taken(lib):
+    for kw in (dict(), dict(start=_address(9)), dict(out=_address(0) + 3 * 1024), dict(out=_address(0) - 3 * 1024),
+               # pools cut from one buffer: keys and values of a page beside each other, of a head beside each other,
+               # of other layers, one behind the other
+               dict(v=_address(1) + 2 * 4096, ps=8192), dict(v=_address(1) + 2 * 2048, ps=8192, hs=4096),
+               dict(v=_address(1) + 2 * 8192, ps=5 * 4096), dict(v=_address(1) + 2 * 8 * 4096),
+               dict(v=_address(1) + 2 * 16384 * 2, hs=16384, ps=2048), dict(v=_address(1) - 2 * 8 * 4096),
+               # an output between two pages' rows
+               dict(out=_address(1) + 2 * 4096, ps=8192, v=_address(2))):
+        assert _attention(lib, **{k: w for k, w in kw.items()}) not in (0, -2), kw
+        if "out" not in kw:
+            assert _append(lib, **kw) not in (0, -2), kw
+    assert _attention(lib, v=ATTEND["k"]) not in (0, -2)  # reads alone
+    assert _append(lib, out=_address(0) + 3 * 2048) not in (0, -2)
+
+
+K = ATTEND["k"]
+TABLE = dict(w=400, ts=400)  # wide enough that the work may be split
+
+
+@on_cpu
+@pytest.mark.parametrize("bad", [
+    dict(out=_address(0)), dict(out=_address(0) + 3 * 1024 - 16), dict(out=_address(0) - 3 * 1024 + 16), dict(out=K),
+    dict(out=K + 2 * 8 * 4096 - 16), dict(out=K - 16), dict(out=K + 2 * 4096, ps=6144 - 1024, v=_address(2)),
+    dict(out=ATTEND["v"] + 4096), dict(out=ATTEND["tab"]), dict(out=ATTEND["lens"]),
+    dict(out=_address(9), start=_address(9) + 32), dict(out=ATTEND["tab"] + 2 * 400 * 4, **TABLE),
+    dict(work=ATTEND["q"], **TABLE), dict(work=ATTEND["out"] + 16, **TABLE), dict(work=K, **TABLE),
+    dict(work=ATTEND["v"] - 16, **TABLE), dict(work=ATTEND["lens"] - 16, **TABLE), dict(work=ATTEND["tab"] + 16, **TABLE)],
+    ids=str)
+def test_attention_outputs_over_inputs_are_refused(lib, bad):
+    assert _attention(lib, **bad) == -2
+
+
+@on_cpu
+@pytest.mark.parametrize("bad", [
+    dict(v=K), dict(v=K + 16), dict(v=K + 2 * 7 * 4096), dict(v=K - 16), dict(v=K + 2 * 4096 - 16, ps=8192),
+    dict(v=K + 2 * 2048, ps=8192), dict(v=K + 2 * 2048, ps=8192, hs=4096 - 8), dict(out=_address(0)),
+    dict(out=_address(0) + 3 * 2048 - 16), dict(out=APPEND["bias"]), dict(out=APPEND["inv"] - 16), dict(out=K),
+    dict(out=APPEND["v"] + 2 * 5 * 4096), dict(out=APPEND["tab"]), dict(out=APPEND["lens"]),
+    dict(out=_address(9), start=_address(9)), dict(qkv=K), dict(qkv=K - 3 * 2048 + 16), dict(bias=APPEND["v"]),
+    dict(inv=K + 16), dict(lens=K + 16), dict(tab=APPEND["v"] + 4), dict(start=K + 4)], ids=str)
+def test_append_outputs_over_inputs_are_refused(lib, bad):
+    assert _append(lib, **bad) == -2
+
+
+SAMPLE = dict(x=_address(0), fp32=0, rs=100, u=_address(1), T=_address(2), k=_address(3), p=_address(4), m=_address(5),
+              out=_address(6), work=_address(7), bytes=1 << 30, B=2, V=100)
+
+
+def _sample(lib, **kw):
+    a = {**SAMPLE, **kw}
+    return lib.ns_sample(a["x"], a["fp32"], a["rs"], a["u"], a["T"], 1.0, a["k"], 0, a["p"], 1.0, a["m"], 0.0,
+                         a["out"], a["work"], a["bytes"], a["B"], a["V"], None)
+
+
+@on_cpu
+def test_sample_takes_what_is_apart(lib):
+    for kw in (dict(), dict(T=None, k=None, p=None, m=None), dict(fp32=1), dict(out=_address(0) + 400),
+               dict(out=_address(0) - 8)):
+        assert _sample(lib, **kw) not in (0, -2), kw
+
+
+@on_cpu
+@pytest.mark.parametrize("bad", [
+    dict(work=None), dict(work=SAMPLE["work"] + 8), dict(bytes=100), dict(out=SAMPLE["x"]), dict(out=SAMPLE["x"] + 396),
+    dict(out=SAMPLE["x"] + 796, fp32=1), dict(out=SAMPLE["x"] + 300, rs=101, V=50), dict(work=SAMPLE["x"]),
+    dict(work=SAMPLE["out"]), dict(work=SAMPLE["u"] - 16), dict(work=SAMPLE["T"] - 16), dict(work=SAMPLE["k"] - 16),
+    dict(work=SAMPLE["p"]), dict(work=SAMPLE["m"] - 64)], ids=str)
+def test_sample_outputs_over_inputs_are_refused(lib, bad):
+    assert _sample(lib, **bad) == -2

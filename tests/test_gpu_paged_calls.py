@@ -26,3 +26,41 @@ def test_counts_past_32_bits(kernels, new):
     one = R.PagedBatch([700], None if new is None else [1], Hk, D, 16, seed=2)
     q = q[:1]
     assert torch.equal(attend(one, shared=(1 << 32) + 16), attend(one, shared=one.table.shape[1] * 16))
+
+
+@pytest.mark.parametrize("layout", ["pages", "heads", "layers"])
+def test_pools_cut_from_one_buffer(kernels, layout):
+    """Keys and values beside each other per page or per head, or of one layer of a pool of all layers."""
+    Hq, Hk, D, page = 14, 2, 64, 16
+    batch = R.PagedBatch([70, 33, 5], [3, 33, 1], Hk, D, page, seed=1)
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(batch.T, (Hq + 2 * Hk) * D, generator=g).to(BF16).cuda()
+    inv = (1.0 / 1e6 ** (torch.arange(0, D, 2).float() / D)).cuda()
+    n = batch.k.shape[0]
+    if layout == "pages":
+        buf = torch.full((n, 2, Hk, page, D), 9.0, dtype=BF16, device="cuda")
+        k, v = buf[:, 0], buf[:, 1]
+    elif layout == "heads":
+        buf = torch.full((Hk, 2, n, page, D), 9.0, dtype=BF16, device="cuda")
+        k, v = (buf[:, i].transpose(0, 1) for i in (0, 1))
+    else:
+        buf = torch.full((n, 3, 2, Hk, page, D), 9.0, dtype=BF16, device="cuda")
+        k, v = buf[:, 1, 0], buf[:, 1, 1]
+
+    def run(k, v):
+        q = kernels.paged_append(qkv, None, inv, batch.table, batch.lens, k, v, Hq, q_start=batch.q_start)
+        return kernels.paged_attention(q, k, v, batch.table, batch.lens, Hq, q_start=batch.q_start)
+
+    pools = [batch.k.contiguous(), batch.v.contiguous()]
+    k.copy_(pools[0])
+    v.copy_(pools[1])
+    others = buf[:, [0, 2]].clone() if layout == "layers" else None
+    want = run(*pools)
+    got = run(k, v)
+    torch.cuda.synchronize()
+    bits = torch.int16  # (the pools' unused rows are NaN)
+    assert torch.equal(got, want)
+    assert torch.equal(k.contiguous().view(bits), pools[0].view(bits))
+    assert torch.equal(v.contiguous().view(bits), pools[1].view(bits))
+    if others is not None:
+        assert torch.equal(buf[:, [0, 2]], others)
