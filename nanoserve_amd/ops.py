@@ -159,6 +159,12 @@ def _work_args(work) -> tuple:
     return work.data_ptr(), work.numel()
 
 
+def check_setting(name: str, t) -> None:
+    """Raises unless the number t is a setting ``name`` (temperature, top_k, top_p, min_p) of Kernels.sample."""
+    if not t >= 0 or (name in ("top_p", "min_p") and t > 1):
+        raise ValueError(f"{name} is out of range: {t}")
+
+
 def _apart(out: torch.Tensor, t: torch.Tensor, name: str) -> None:
     """Raises if the contiguous out shares memory with t, whose last dimension is contiguous."""
     a, b = out.data_ptr(), t.data_ptr()
@@ -796,8 +802,7 @@ class Kernels:
                     raise ValueError(f"{name} must be a number or a contiguous [{B}] tensor")
                 args += [t.data_ptr(), 0]
             else:
-                if not t >= 0 or (name in ("top_p", "min_p") and t > 1):
-                    raise ValueError(f"{name} is out of range: {t}")
+                check_setting(name, t)
                 args += [None, min(int(t), V) if dtype is torch.int32 else t]
         if out is None:
             out = logits.new_empty(B, dtype=torch.int32)

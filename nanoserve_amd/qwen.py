@@ -42,7 +42,7 @@ import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from . import gptq
-from .ops import Kernels
+from .ops import Kernels, check_setting
 
 # Cache rows per split of the library's decode attention (its workspace grows by one split
 # every ATTN_SPLIT_ROWS rows; tests/test_abi.py checks the two agree).
@@ -524,13 +524,16 @@ class Qwen2Runner:
         [0, 1) (default: torch.rand); -1 stands where a step's logits left nothing to draw, and the
         next step then starts from a zero embedding."""
         T = prompt_ids.shape[0]
-        if not temperature >= 0:
-            raise ValueError(f"temperature is out of range: {temperature}")
+        check_setting("temperature", temperature)
         if temperature > 0:
+            for name, value in (("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+                check_setting(name, value)
             if u is None:
                 u = torch.rand(n_new, device=self.dev)
-            elif tuple(u.shape) != (n_new,):
-                raise ValueError(f"u must hold {n_new} random numbers")
+            elif not isinstance(u, torch.Tensor) or u.dtype != torch.float32:
+                raise TypeError("u must be a float32 tensor")
+            elif tuple(u.shape) != (n_new,) or u.device != self.logits.device:
+                raise ValueError(f"u must hold {n_new} random numbers on {self.logits.device}")
             work = self.k.sample_workspace(1, self.shape.vocab, self.logits.dtype, device=self.dev)
 
         def token(logits, n):
