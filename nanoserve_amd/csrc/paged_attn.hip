@@ -684,7 +684,6 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m = -INFINITY, l = 0.f;
-  bool seen = false;  // the lane's row saw one of the lane's keys
   const float c = a.c;
 
   // transpose-read offsets (elements) of the 32-dim tiles at key row 4 kh + (lane % 16) / 4
@@ -723,7 +722,6 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
           const bool see = (key < hi) & (key >= k0) & ((key >= lo) | (key < first)) &
                            (((groups >> (2 * u + (r >> 3))) & 1) != 0);
           s[u][r] = see ? s[u][r] : -INFINITY;
-          seen |= see;
         }
     } else if (key0 + kTileKeys > hi_min || key0 < lo_max || key0 < k0) {  // positions from, .. to - 1
       const int from = max(lo, k0);
@@ -735,9 +733,6 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
           const uint32_t at = (uint32_t)(key0 + 4 * kh - from + 32 * u + 8 * (r >> 2) + (r & 3));
           s[u][r] = at < span ? s[u][r] : -INFINITY;
         }
-      seen |= max(from, key0) < min(hi, key0 + kTileKeys);
-    } else {
-      seen = true;
     }
     float bm = s[0][0];
 #pragma unroll
@@ -825,9 +820,23 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   }
 
   l += lane_xor32(l);
-  const uint64_t see_lanes = __ballot(seen);  // a row's keys are spread over lanes jq and 32 + jq
-  seen = ((see_lanes >> jq | see_lanes >> (32 + jq)) & 1) != 0;
   if (wrow + jq >= rows) return;
+  // Without a maximum and a sum the row sees none of the range's keys, or scores that are all -inf: then there is
+  // a page among those that it sees.
+  bool seen = m > -INFINITY || l != 0.f;
+  if (!seen) {
+    const int none = min(j0, kb.na), some = min(j1, kb.na), from = max(j0 - kb.na, 0), to = max(j1 - kb.na, 0);
+    const int part[2][2] = {{kTileKeys * (kb.a0 + none), kTileKeys * (kb.a0 + some)},
+                            {kTileKeys * (kb.m0 + from), kTileKeys * (kb.m0 + to)}};
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {  // the first tokens and the rest, in either part of the list
+      int key = max(max(k0, i & 2 ? lo : 0), i & 1 ? part[1][0] : part[0][0]);
+      const int end = min(i & 2 ? hi : min(first, hi), i & 1 ? part[1][1] : part[0][1]);
+#pragma unroll 1
+      for (; key < end && !seen; key = (key / a.s.page_size + 1) * a.s.page_size)
+        seen = (unsigned)table[key / a.s.page_size] < (unsigned)a.p.n_pages;
+    }
+  }
   if (direct) {
     const float inv = seen ? 1.f / l : 0.f;
     uint16_t* op = a.out + ((size_t)t * a.Hq + hq) * D + 4 * kh;

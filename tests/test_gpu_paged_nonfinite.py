@@ -224,3 +224,24 @@ def test_entries_outside_the_pool_in_a_shared_prefix(kernels, new, Hq, Hk, D):
             want = formula(batch, q, Hq, hidden=lambda b, j: torch.isin(j // 16, torch.tensor(pages)))
             got = kernels.paged_attention(q, batch.k, batch.v, table, batch.lens, Hq, q_start=batch.q_start, shared=256)
             _check(got, want)
+
+
+@pytest.mark.parametrize("Hq,Hk,D", LAYOUTS)
+@pytest.mark.parametrize("lens,new,shared", [([300, 700], None, 0), ([300, 700], [40, 300], 0), ([300, 350], [3, 40], 256),
+                                             ([300, 350], None, 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 20)])
+def test_scores_that_are_all_minus_infinity_beside_entries_outside_the_pool(kernels, lens, new, shared, window, sinks,
+                                                                            Hq, Hk, D):
+    """NaN where a page is there, 0 where all that a token would see is outside the pool."""
+    batch = R.PagedBatch(lens, new, Hk, D, 16, shared=shared, seed=5)
+    q = _queries(batch.T, Hq, D, 7)
+    q[:, ::D] = 1.0
+    batch.k[..., 0] = -INF
+    width = batch.table.shape[1]
+    for pages in ([0], [0, 1, 2, 3, 4, 5, 6, 7], list(range(8, 16)), list(range(18)), list(range(width))):
+        table = batch.table.clone()
+        table[:, [p for p in pages if p < width]] = -1
+        want = formula(batch, q, Hq, window, sinks, hidden=lambda b, j: torch.isin(j // 16, torch.tensor(pages)))
+        got = kernels.paged_attention(q, batch.k, batch.v, table, batch.lens, Hq, q_start=batch.q_start, shared=shared,
+                                      window=window, sinks=sinks)
+        _check(got, want)
