@@ -149,14 +149,9 @@ def _int32(n: int) -> int:
     return max(-(1 << 31), min(n, (1 << 31) - 1))
 
 
-def _work_args(work) -> tuple:
-    """Address and size of a uint8 workspace as the library takes them, (None, 0) for None. One whose
-    elements are strided or repeated (an expanded byte) spans another range than its size says."""
-    if work is None:
-        return None, 0
-    if not work.is_contiguous():
-        raise ValueError("work must be contiguous")
-    return work.data_ptr(), work.numel()
+def _strided_work():
+    # elements that are apart or repeated (an expanded byte) span another range than their number says
+    return ValueError("work must be contiguous")
 
 
 def check_setting(name: str, t) -> None:
@@ -310,13 +305,15 @@ class Kernels:
             y = x.new_empty((M or 1, N))
         if work is not None:
             _require_gpu_tensor(work, "work", torch.uint8)
+            if not work.is_contiguous():
+                raise _strided_work()
         if work is None or padded:
             rc = self.lib.ns_w4_linear_rows(x.data_ptr(), Wq.data_ptr(), S.data_ptr(), y.data_ptr(),
                                             max(M, 1), N, K, group, self._stream())
             self._check(rc, "ns_w4_linear")
         else:
             rc = self.lib.ns_w4_linear_ws(x.data_ptr(), Wq.data_ptr(), S.data_ptr(), y.data_ptr(),
-                                          max(M, 1), N, K, group, *_work_args(work),
+                                          max(M, 1), N, K, group, work.data_ptr(), work.numel(),
                                           self._stream())
             self._check(rc, "ns_w4_linear_ws")
         return y if M else y[:0]
@@ -408,11 +405,13 @@ class Kernels:
         _require_gpu_tensor(q, "q", torch.bfloat16)
         _require_gpu_tensor(pos, "pos", torch.int32)
         _require_gpu_tensor(work, "work", torch.uint8)
+        if not work.is_contiguous():
+            raise _strided_work()
         if out is None:
             out = torch.empty((1, n_heads * head_dim), dtype=torch.bfloat16, device=q.device)
         rc = self.lib.ns_decode_attention(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                          pos.data_ptr(), out.data_ptr(), *_work_args(work),
-                                          n_heads, n_kv_heads, head_dim,
+                                          pos.data_ptr(), out.data_ptr(), work.data_ptr(),
+                                          work.numel(), n_heads, n_kv_heads, head_dim,
                                           k_cache.shape[-2], self._stream())
         self._check(rc, "ns_decode_attention")
         return out
@@ -444,6 +443,8 @@ class Kernels:
         _require_gpu_tensor(inv_freq, "inv_freq", torch.float32)
         _require_gpu_tensor(pos, "pos", torch.int32)
         _require_gpu_tensor(work, "work", torch.uint8)
+        if not work.is_contiguous():
+            raise _strided_work()
         for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
             _require_gpu_tensor(t, n, torch.bfloat16)
             if not t.is_contiguous():
@@ -457,7 +458,7 @@ class Kernels:
         rc = self.lib.ns_decode_qkv_attention(
             qkv.data_ptr(), None if bias is None else bias.data_ptr(), inv_freq.data_ptr(),
             pos.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
-            *_work_args(work), n_heads, n_kv_heads, head_dim, k_cache.shape[-2],
+            work.data_ptr(), work.numel(), n_heads, n_kv_heads, head_dim, k_cache.shape[-2],
             1 if merge else 0, None if rot is None else _rot_ptr(rot, head_dim), self._stream())
         self._check(rc, "ns_decode_qkv_attention")
         return out
@@ -492,13 +493,15 @@ class Kernels:
         split partials are merged while the activation is loaded."""
         _require_gpu_tensor(attn_out, "attn_out", torch.bfloat16)
         _require_gpu_tensor(work, "work", torch.uint8)
+        if not work.is_contiguous():
+            raise _strided_work()
         _require_gpu_tensor(pos, "pos", torch.int32)
         _require_gpu_tensor(Wq, "Wq", torch.int32)
         _require_gpu_tensor(S, "S", torch.bfloat16)
         N, K = Wq.shape[0], Wq.shape[1] * 8
         if out is None:
             out = torch.empty((1, N), dtype=torch.bfloat16, device=Wq.device)
-        rc = self.lib.ns_w4_gemv_decode_attn(attn_out.data_ptr(), _work_args(work)[0],
+        rc = self.lib.ns_w4_gemv_decode_attn(attn_out.data_ptr(), work.data_ptr(),
                                              pos.data_ptr(), max_len, n_heads, Wq.data_ptr(),
                                              S.data_ptr(), out.data_ptr(), N, K, group,
                                              self._stream())
@@ -625,9 +628,12 @@ class Kernels:
             _require_gpu_tensor(out, "out", torch.bfloat16)
             if tuple(out.shape) != (T, n_heads * 128) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{T}, {n_heads * 128}] tensor")
+        if work is not None and not work.is_contiguous():
+            raise _strided_work()
         rc = self.lib.ns_prompt_attention(
             q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(1), k.stride(0),
-            out.data_ptr(), *_work_args(work), T, n_heads, Hk, pos0, self._stream())
+            out.data_ptr(), None if work is None else work.data_ptr(),
+            0 if work is None else work.numel(), T, n_heads, Hk, pos0, self._stream())
         self._check(rc, "ns_prompt_attention")
         return out
 
@@ -749,17 +755,21 @@ class Kernels:
             _apart(out, q, "q")
         if T == 0 or B == 0:
             return out
+        if (shared | window | sinks) >> 31:  # one below 0 or past 32 bits
+            shared, window, sinks = _int32(shared), _int32(window), _int32(sinks)
         if work is None:
             work = self.paged_attention_workspace(T, B, n_heads, Hk, D, table[2] * page_size,
                                                   q_start is not None, shared, device=q.device)
         else:
             _require_here(work, "work", torch.uint8, here)
+            if not work.is_contiguous():
+                raise _strided_work()
         rc = self.lib.ns_paged_attention(
             q.data_ptr(), q.stride(0) if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
             *strides, n_pages, page_size, *table, lens.data_ptr(),
             None if q_start is None else q_start.data_ptr(), out.data_ptr(),
-            *_work_args(work), T, B, n_heads, Hk, D, _int32(shared), _int32(window), _int32(sinks),
-            D ** -0.5 if scale is None else scale, _raw_stream(here))
+            None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
+            Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
         self._check(rc, "ns_paged_attention")
         return out
 
@@ -816,8 +826,11 @@ class Kernels:
             work = self.sample_workspace(B, V, logits.dtype, device=logits.device)
         else:
             _require_here(work, "work", torch.uint8, here)
+            if not work.is_contiguous():
+                raise _strided_work()
         rc = self.lib.ns_sample(logits.data_ptr(), int(fp32), logits.stride(0) if B > 1 else V, u.data_ptr(),
-                                *args, out.data_ptr(), *_work_args(work), B, V, _raw_stream(here))
+                                *args, out.data_ptr(), None if work is None else work.data_ptr(),
+                                0 if work is None else work.numel(), B, V, _raw_stream(here))
         self._check(rc, "ns_sample")
         return out
 
