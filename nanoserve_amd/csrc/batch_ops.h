@@ -66,11 +66,12 @@ size_t ns_paged_attention_workspace(int T, int B, int Hq, int Hk, int D, int max
  * shared > 0: the caller states that positions 0 .. shared - 1, as far as a sequence has them, lie in the
  * same pages for every sequence; they are read through the row of the longest one, once for the batch.
  * A head's output is NaN for NaN in its query or in a key that it sees, for a score of +inf and for scores that are
- * all -inf. Keys and values (NaN and infinities among them) in positions that no token sees have no effect. A NaN or infinite value that a token sees leaves that dimension of its output NaN or infinite (NaN also
- * where the exact result is infinite: the second term of a probability is zero or negative), and may do so to the
- * tokens of the same kv head in its launch tile that do not see it.
- * -2 for D other than 64 and 128, Hq % Hk, negative window, sinks or shared, scale not positive and finite,
- * and as ns_paged_append (the pools may be one and the same here); work_bytes too small; out and the workspace
+ * all -inf. Keys and values (NaN and infinities among them) in positions that no token sees have no effect. A NaN
+ * or infinite value that a token sees leaves that dimension of its output NaN or infinite (NaN also where the exact
+ * result is infinite: the second term of a probability is zero or negative), and may do so to the tokens of the same
+ * kv head in its launch tile that do not see it.
+ * -2 for D other than 64 and 128, Hq % Hk, T * Hq >= 2^30, negative window, sinks or shared, scale not positive and
+ * finite, and as ns_paged_append (the pools may be one and the same here); work_bytes too small; out and the workspace
  * over each other or over an input.
  */
 int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, const void* v_pool,

@@ -45,8 +45,12 @@ struct PagedArgs {
 };
 
 // LDS of a workgroup: 64 KiB (D = 128: two stages of 64 rows of K and of V; D = 64: four). Separate arrays,
-// not one: a read of a stage then provably does not alias the loads in flight into another, so the
-// compiler puts no wait for those before it.
+// not one: where a read of a stage provably does not alias the loads in flight into another, the compiler puts
+// no wait for those before it. It still puts some, which hold the ring below its depth: in the one-token kernel
+// before the reads of stage 0 (vmcnt 1 before K, 0 before V; with two stages the other's loads are then drained in every
+// second block), and in tiles of four stages in every block, behind the loads just sent out (vmcnt 3 to 0 before
+// the scores: the query fragments, loaded before the ring, may for all it knows be in flight behind the ring's
+// conditional waits). Tiles of two stages, whose wait is for all loads, have none.
 template <int D>
 constexpr int ring_stages() {
   return D == 128 ? 2 : 4;
@@ -496,10 +500,11 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
 //    sequences over the shared prefix may lie apart: the positions between them stay in the list, and their rows
 //    are not read but zero, as a value there (it may be NaN) would reach every row through 0 * NaN.
 // Measured (28 / 4 heads of 128): prompts of 5 sequences of 2000 to 8000 654 us, 677 TFLOP/s, with the second term
-// 1015 (a large library product: 1265); matrix cores busy in half of the cycles and vector units in 58 %, at 1.8 GHz.
-// Issuing one half block's softmax between the products of its neighbours did not help (659 -> 681 to 730 us): the
-// other wave of the SIMD fills those slots already. 4095 tokens with a window of 1000 and 14 / 2 heads of 64 43 us;
-// 96 drafts of 1 to 3 tokens behind 16384 shared positions 108 us.
+// 1015 (a large library product: 1265); matrix cores busy in half of the cycles and vector units in 58 %, at 1.8 GHz,
+// so that products and softmax still take turns for much of the time. Issuing one half block's softmax between the
+// products of its neighbours did not help (659 -> 681 to 730 us). 4095 tokens with a window of 1000 and 14 / 2 heads of
+// 64 43 us. 96 drafts of 1 to 3 tokens behind 16384 shared positions 100 to 104 us back to back, 108 to 117 among
+// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD.
 template <int D, bool kShared>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
   constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad, kDT = D / 32,
@@ -1004,6 +1009,9 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
   Plan p{};
   const int R = Hq / Hk;
   shared = std::min(shared, max_len);
+  // Token counts are device values, so with q_start single tokens go in tiles too. us without and with it (28 / 4
+  // heads of 128; 14 / 2 of 64): one of 700 10.1, 15.1; 9.0, 13.3. 64 of 1000 to 8000 113, 146; 34, 60. 64 such
+  // beside a prompt of 512 at 4000 184 in one call, 108 + 80 in two.
   p.one = !ragged && R <= 16;
   // Least range 64 keys (a block per wave) and 256. us with half, this and twice it: one token at 4000 13.2, 11.8,
   // 11.4; at 700 9.4, 9.5, 9.9; 20 tokens after 4000 19.4, 19.8, 23.8.
@@ -1015,7 +1023,7 @@ Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, in
     const long long st = ((long long)T * R + kTileRows - 1) / kTileRows;
     const int blocks = (shared + kTileKeys - 1) / kTileKeys;
     // One workgroup per CU, which leaves the other half of its LDS to the sequences' own keys. us for one, one and
-    // a half, two and three: 96 sequences (194 tokens) behind 16384 99.6, 108.8, 116.5, 126.8.
+    // a half, two and three, back to back: 96 sequences (194 tokens) behind 16384 99.6, 108.8, 116.5, 126.8.
     const long long want = cus / (st * Hk);
     // at least four blocks each, two where that leaves fewer than eight splits (8 sequences behind 1024: 14.4 ->
     // 11.8 us; always two: 32 behind 4096 23.3 -> 26.5)

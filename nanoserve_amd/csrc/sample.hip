@@ -3,7 +3,7 @@
 //
 // The kept tokens are a beginning of the order by falling logit, so they are those above a cut: a 32-bit
 // order-preserving key of the logit, and the index up to which tokens at exactly that key are kept. The row is
-// never sorted. It is read up to three times, by several workgroups per row, in launches of their own:
+// never sorted. It is read up to four times, by several workgroups per row, in launches of their own:
 //   max   the largest logit, and that of every tile of 512
 //   hist  a histogram, linear in the logit, of counts for top-k and of weights for top-p: 2048 bins over
 //         the logits whose weight is not zero. The cut lies in one bin. Not for a top-k of at most as many
@@ -14,9 +14,13 @@
 //         the tiles' sums and then within one tile
 // hist is left out where no row needs it. top-p of a top-k longer than the list takes scan and
 // end twice. hist and scan skip tiles whose maximum does not matter to them. A bin with more tokens than
-// the list holds (flat rows, rows of few values) is cut by `end` alone, digit by digit of the key.
+// the list holds (flat rows, rows of few values) is cut by `end` alone, digit by digit of the key: one workgroup reads
+// the row five times (three digits, the level tokens, the sums), eight times with both top-k and top-p.
 // Measured: one row of 152064 bf16 with top-k 20 and top-p 0.8 16 us (max 3.4, scan 8, end 5: latency); 256 rows of
-// 151936 fp32 with settings of their own 158 to 167 us (max 25, at 6.3 TB/s, hist 33, scan 39, end 21, second scan 22, end 20).
+// 151936 fp32 with settings of their own 160 us, 167 to 174 among other launches (max 25, at 6.3 TB/s, hist 33, scan 39,
+// end 21, second scan 22, end 20). Crowded rows of 152064, top-p 0.9, one row and 256: T = 20 280 and 375 us (end alone
+// 268), logits of whole numbers 312 and 436, T = 20 with a top-k of a third of the row in fp32 372 and 509; spread
+// rows 31 and 148.
 //  * Launches, each with little code, and not one kernel with a counter that finds a row's last workgroup:
 //    the fences that its data needs between the XCDs' L2 caches cost more (256 rows without a cut 407 us).
 //  * Weights exp((l - max) / T) are rounded to multiples of 2^-42 and summed as integers: sums do not
@@ -1060,7 +1064,9 @@ int row_tiles(int V) { return (V + 8 * kTileVecs - 1) / (8 * kTileVecs); }
 // Workgroups per row, each with at least eight tiles: two per CU where all rows have the same settings and end
 // together, six where rows have their own, so that the long ones spread. us with two, four, six and eight per CU:
 // 128 rows of 152064 with top-k 20 31, 37, 42, 48; 16 with top-p 33, 38, 38, 38; 256 mixed 234, 174, 158, 154, 64
-// mixed 95, 85, 91, 93.
+// mixed 95, 85, 91, 93. Settings in device arrays count as the rows' own whatever they hold, and an array of top-k
+// with any top-p brings all launches: top-k 20 and top-p 0.8 for every row of 152064 take, as numbers and as arrays, 16.5
+// and 21.4 us for one row, 30 and 47 for 128, 39 and 55 for 256.
 int row_parts(int B, int V, bool mixed) {
   int cus = 256;  // (a failed query leaves MI355X's count; the launch reports the error)
   if (cached_cu_count(&cus) != hipSuccess || cus <= 0) cus = 256;

@@ -789,7 +789,9 @@ class Kernels:
         the ones of at least ``min_p`` times the largest probability; the token is the first, by index,
         at which the running sum of the kept probabilities exceeds u times their sum. Temperature 0:
         the largest logit. A setting is a number or a tensor [B] (float32, top_k int32) with one for
-        each row. NaN logits are never drawn, nor is -inf; a row without any other gives -1. The same
+        each row. Numbers out of range are refused; a tensor's are read on the device, where a top_k
+        below 1 keeps all tokens, a temperature not above 0 is 0, a top_p from 1 on keeps all and a
+        min_p above 1 is 1. NaN logits are never drawn, nor is -inf; a row without any other gives -1. The same
         arguments give the same token, eager or replayed, whatever else is in the batch. ``work``: from
         sample_workspace, allocated here when it is not given. The reference decodes greedily
         (qwen.py:166-177)."""
