@@ -66,24 +66,28 @@ inline bool batch_ok(const Batch& s, const Pools& p, int Hk, int D) {
          (__int128)(p.n_pages - 1) * p.page_stride + head <= p.head_stride;
 }
 
-// The offsets i * page_stride + j * head_stride, |i| < n_pages and |j| < Hk, hold one in (lo, hi)? All in bytes;
-// i and j from 0 on with `down` false.
-inline bool pool_offset_in(const Pools& p, int Hk, bool down, __int128 lo, __int128 hi) {
-  const __int128 page = 2 * (__int128)p.page_stride, head = 2 * (__int128)p.head_stride;
-  const long long pages = p.n_pages - 1, heads = Hk - 1;
-  const __int128 far = (pages ? pages * page : 0) + (heads ? heads * head : 0);
-  if (lo >= far || hi <= (down ? -far : 0)) return false;  // (where the pools' spans are apart: no loop)
+// The offsets i * page + j * head, |i| <= pages and |j| <= heads, hold one in (lo, hi)? i and j from 0 on with
+// `down` false. A stride of a lone page or head is 0.
+template <typename W>
+inline bool offset_in(W page, W head, long long pages, long long heads, bool down, W lo, W hi) {
   for (long long j = down ? -heads : 0; j <= heads; ++j) {
-    const __int128 from = lo - (heads ? j * head : 0), to = hi - (heads ? j * head : 0);
-    __int128 i = 0;
-    if (pages) {  // the first i past `from`
-      i = from / page - (from % page < 0) + 1;
-      i = std::max<__int128>(i, down ? -pages : 0);
-    }
-    const __int128 at = pages ? i * page : 0;
-    if (i <= pages && from < at && at < to) return true;
+    const W from = lo - j * head, to = hi - j * head;
+    // the first i past `from`
+    const W i = pages ? std::max<W>(from / page - (from % page < 0) + 1, down ? -pages : 0) : 0;
+    if (i <= pages && from < i * page && i * page < to) return true;
   }
   return false;
+}
+
+// The same for a pool's strides, in bytes.
+inline bool pool_offset_in(const Pools& p, int Hk, bool down, __int128 lo, __int128 hi) {
+  const long long pages = p.n_pages - 1, heads = Hk - 1;
+  const long long page = pages ? 2 * p.page_stride : 0, head = heads ? 2 * p.head_stride : 0;
+  const __int128 far = (__int128)pages * page + (__int128)heads * head;
+  if (lo >= far || hi <= (down ? -far : 0)) return false;  // (where the pools' spans are apart: no loop)
+  const __int128 most = (__int128)1 << 60;  // what the loop's values stay within, eight times
+  if (far < most && lo > -most && hi < most) return offset_in<long long>(page, head, pages, heads, down, lo, hi);
+  return offset_in<__int128>(page, head, pages, heads, down, lo, hi);
 }
 
 // Whether none of the pool's pages lies in a range.
