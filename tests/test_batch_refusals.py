@@ -98,11 +98,11 @@ def _address(i):
 
 on_cpu = pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are no memory")
 ATTEND = dict(q=_address(0), qs=512, k=_address(1), v=_address(2), ps=4096, hs=2048, n=8, page=16, tab=_address(3), ts=4,
-              w=4, lens=_address(4), start=None, out=_address(5), work=_address(6), bytes=1 << 20, T=3, B=3, Hq=4, Hk=2,
+              w=4, lens=_address(4), start=None, out=_address(5), work=_address(6), bytes=1 << 20, T=5, B=5, Hq=4, Hk=2,
               D=128, shared=0, window=0, sinks=0, scale=0.1)
 APPEND = dict(qkv=_address(0), qs=1024, bias=_address(7), inv=_address(8), start=None, lens=_address(4),
               tab=_address(3), ts=4, w=4, k=_address(1), v=_address(2), ps=4096, hs=2048, n=8, page=16, out=_address(5),
-              T=3, B=3, Hq=4, Hk=2, D=128)
+              T=5, B=5, Hq=4, Hk=2, D=128)
 
 
 @pytest.fixture(scope="module")
@@ -148,7 +148,7 @@ def test_pages_and_heads_that_overlap_are_refused(lib, call, bad):
 
 @on_cpu
 def test_tensors_that_are_apart_are_taken(lib):
-    for kw in (dict(), dict(start=_address(9)), dict(out=_address(0) + 3 * 1024), dict(out=_address(0) - 3 * 1024),
+    for kw in (dict(), dict(start=_address(9)), dict(out=_address(0) + 5 * 1024), dict(out=_address(0) - 5 * 1024),
                # pools cut from one buffer: keys and values of a page beside each other, of a head beside each other,
                # of other layers, one behind the other
                dict(v=_address(1) + 2 * 4096, ps=8192), dict(v=_address(1) + 2 * 2048, ps=8192, hs=4096),
@@ -160,7 +160,7 @@ def test_tensors_that_are_apart_are_taken(lib):
         if "out" not in kw:
             assert _append(lib, **kw) not in (0, -2), kw
     assert _attention(lib, v=ATTEND["k"]) not in (0, -2)  # reads alone
-    assert _append(lib, out=_address(0) + 3 * 2048) not in (0, -2)
+    assert _append(lib, out=_address(0) + 5 * 2048) not in (0, -2)
 
 
 K = ATTEND["k"]
@@ -169,7 +169,7 @@ TABLE = dict(w=400, ts=400)  # wide enough that the work may be split
 
 @on_cpu
 @pytest.mark.parametrize("bad", [
-    dict(out=_address(0)), dict(out=_address(0) + 3 * 1024 - 16), dict(out=_address(0) - 3 * 1024 + 16), dict(out=K),
+    dict(out=_address(0)), dict(out=_address(0) + 5 * 1024 - 16), dict(out=_address(0) - 5 * 1024 + 16), dict(out=K),
     dict(out=K + 2 * 8 * 4096 - 16), dict(out=K - 16), dict(out=K + 2 * 4096, ps=6144 - 1024, v=_address(2)),
     dict(out=ATTEND["v"] + 4096), dict(out=ATTEND["tab"]), dict(out=ATTEND["lens"]),
     dict(out=_address(9), start=_address(9) + 32), dict(out=ATTEND["tab"] + 2 * 400 * 4, **TABLE),
@@ -184,9 +184,9 @@ def test_attention_outputs_over_inputs_are_refused(lib, bad):
 @pytest.mark.parametrize("bad", [
     dict(v=K), dict(v=K + 16), dict(v=K + 2 * 7 * 4096), dict(v=K - 16), dict(v=K + 2 * 4096 - 16, ps=8192),
     dict(v=K + 2 * 2048, ps=8192), dict(v=K + 2 * 2048, ps=8192, hs=4096 - 8), dict(out=_address(0)),
-    dict(out=_address(0) + 3 * 2048 - 16), dict(out=APPEND["bias"]), dict(out=APPEND["inv"] - 16), dict(out=K),
+    dict(out=_address(0) + 5 * 2048 - 16), dict(out=APPEND["bias"]), dict(out=APPEND["inv"] - 16), dict(out=K),
     dict(out=APPEND["v"] + 2 * 5 * 4096), dict(out=APPEND["tab"]), dict(out=APPEND["lens"]),
-    dict(out=_address(9), start=_address(9)), dict(qkv=K), dict(qkv=K - 3 * 2048 + 16), dict(bias=APPEND["v"]),
+    dict(out=_address(9), start=_address(9)), dict(qkv=K), dict(qkv=K - 5 * 2048 + 16), dict(bias=APPEND["v"]),
     dict(inv=K + 16), dict(lens=K + 16), dict(tab=APPEND["v"] + 4), dict(start=K + 4)], ids=str)
 def test_append_outputs_over_inputs_are_refused(lib, bad):
     assert _append(lib, **bad) == -2
