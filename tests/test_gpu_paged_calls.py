@@ -64,3 +64,58 @@ def test_pools_cut_from_one_buffer(kernels, layout):
     assert torch.equal(v.contiguous().view(bits), pools[1].view(bits))
     if others is not None:
         assert torch.equal(buf[:, [0, 2]], others)
+
+
+@pytest.mark.parametrize("Hq,Hk,D,shared,window,sinks", [(28, 4, 128, 0, 0, 0), (14, 2, 64, 0, 50, 3), (28, 4, 128, 64, 0, 0),
+                                                         (14, 2, 64, 64, 40, 2)])
+def test_a_captured_step_of_any_batch(kernels, Hq, Hk, D, shared, window, sinks):
+    """One captured step of append and attention with q_start, replayed for other lengths, other numbers of tokens per
+    sequence, sequences without any and padded rows; eager work between the replays."""
+    page, B, T, width = 16, 4, 64, 30
+    g = torch.Generator().manual_seed(D + shared)
+    n_pages = B * width
+    order = torch.randperm(n_pages, generator=g).view(B, width).to(torch.int32)
+    order[:, :shared // page] = order[0, :shared // page]
+    table = order.cuda()
+    # (the shared rows are written once; every sequence's own follow)
+    k, v = (torch.randn(n_pages, Hk, page, D, generator=g).to(BF16).cuda() for _ in range(2))
+    qkv = torch.zeros(T, (Hq + 2 * Hk) * D, dtype=BF16, device="cuda")
+    inv = (1.0 / 1e6 ** (torch.arange(0, D, 2).float() / D)).cuda()
+    lens, start = torch.ones(B, dtype=torch.int32, device="cuda"), torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    q, out = (torch.zeros(T, Hq * D, dtype=BF16, device="cuda") for _ in range(2))
+    work = kernels.paged_attention_workspace(T, B, Hq, Hk, D, width * page, ragged=True, shared=shared)
+
+    def step(q, out, work):
+        kernels.paged_append(qkv, None, inv, table, lens, k, v, Hq, q_start=start, out=q)
+        kernels.paged_attention(q, k, v, table, lens, Hq, q_start=start, shared=shared, window=window, sinks=sinks,
+                                work=work, out=out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(q, out, work)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(q, out, work)
+    for new, total in (([1, 1, 1, 1], [100, 470, 65, 300]), ([40, 0, 3, 1], [480, 0, 70, 90]), ([0, 0, 64, 0], [90, 80, 130, 65]),
+                       ([1, 1, 1, 1], [480, 480, 480, 480]), ([16, 16, 16, 16], [80, 300, 81, 479]), ([0, 0, 0, 0], [5, 6, 7, 8])):
+        qkv.copy_(torch.randn(qkv.shape, generator=g).to(BF16))
+        lens.copy_(torch.tensor(total, dtype=torch.int32))
+        start.copy_(torch.tensor([0] + new).cumsum(0).to(torch.int32))
+        q.fill_(7.0)
+        out.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        rows = sum(new)
+        assert bool((out[rows:] == 7).all()) and bool((q[rows:] == 7).all())
+        again, mine = torch.full_like(out, 7.0), torch.full_like(q, 7.0)
+        step(mine, again, None)
+        assert torch.equal(again, out) and torch.equal(mine, q)
+        batch = R.PagedBatch([1], None, Hk, D, page)  # (the reference's view of these pools)
+        batch.host_lens, batch.new, batch.T = total, new, rows
+        batch.k, batch.v, batch.cpu_table = k, v, order
+        if rows:
+            want = R.attention(batch, q[:rows], Hq, window, sinks)
+            err = (out[:rows].cpu().double().view_as(want) - want).abs()
+            assert bool((err <= want.abs() * 2.0 ** -8 + 2.0 ** -13 * 8.0).all())
