@@ -44,9 +44,17 @@ struct Batch {
 
 struct Pools {
   uint16_t *k, *v;
-  long long page_stride, head_stride;
+  long long page_stride, head_stride;  // in elements
   int n_pages;
+  int size = 2;  // bytes of an element: 1 for a cache in 8 bits, whose addresses k and v hold all the same
 };
+
+// The scales of a cache in 8 bits: one byte e, for 2^(e - 127), per 16 rows of a page and head.
+struct Scales {
+  uint8_t *k, *v;
+  long long page_stride, head_stride;
+};
+constexpr int kScaleRows = 16;
 
 // Host checks common to the entry points.
 inline bool batch_ok(const Batch& s, const Pools& p, int Hk, int D) {
@@ -57,7 +65,8 @@ inline bool batch_ok(const Batch& s, const Pools& p, int Hk, int D) {
   if (!s.q_start && s.T != s.B) return false;
   if (!s.lens || !s.table || !p.k || !p.v) return false;
   if (!al(s.lens, 4) || !al(s.table, 4) || !al(s.q_start, 4) || !al(p.k, 16) || !al(p.v, 16)) return false;
-  if (p.page_stride % 8 || p.head_stride % 8 || p.page_stride < 0 || p.head_stride < 0) return false;
+  const int per16 = 16 / p.size;
+  if (p.page_stride % per16 || p.head_stride % per16 || p.page_stride < 0 || p.head_stride < 0) return false;
   // pages and heads do not overlap, whichever of the two is the outer one
   const long long head = (long long)s.page_size * D;
   if ((Hk > 1 && p.head_stride < head) || (p.n_pages > 1 && p.page_stride < head)) return false;
@@ -82,7 +91,7 @@ inline bool offset_in(W page, W head, long long pages, long long heads, bool dow
 // The same for a pool's strides, in bytes.
 inline bool pool_offset_in(const Pools& p, int Hk, bool down, __int128 lo, __int128 hi) {
   const long long pages = p.n_pages - 1, heads = Hk - 1;
-  const long long page = pages ? 2 * p.page_stride : 0, head = heads ? 2 * p.head_stride : 0;
+  const long long page = pages ? p.size * p.page_stride : 0, head = heads ? p.size * p.head_stride : 0;
   const __int128 far = (__int128)pages * page + (__int128)heads * head;
   if (lo >= far || hi <= (down ? -far : 0)) return false;  // (where the pools' spans are apart: no loop)
   const __int128 most = (__int128)1 << 60;  // what the loop's values stay within, eight times
@@ -92,7 +101,7 @@ inline bool pool_offset_in(const Pools& p, int Hk, bool down, __int128 lo, __int
 
 // Whether none of the pool's pages lies in a range.
 inline bool pool_apart(const uint16_t* pool, const Pools& p, int Hk, long long head, Bytes x) {
-  const __int128 from = (__int128)x.lo - reinterpret_cast<uintptr_t>(pool), size = 2 * (__int128)head;
+  const __int128 from = (__int128)x.lo - reinterpret_cast<uintptr_t>(pool), size = p.size * (__int128)head;
   return x.lo >= x.hi || !pool_offset_in(p, Hk, false, from - size, from + (x.hi - x.lo));
 }
 
@@ -107,8 +116,47 @@ inline bool metadata_apart(const Batch& s, Bytes x) {
 // Whether K and V share no element: a page of V starts less than a page before or behind one of K nowhere.
 inline bool pools_apart(const Pools& p, int Hk, long long head) {
   const __int128 d = (__int128)reinterpret_cast<uintptr_t>(p.v) - reinterpret_cast<uintptr_t>(p.k),
-                 size = 2 * (__int128)head;
+                 size = p.size * (__int128)head;
   return !pool_offset_in(p, Hk, true, d - size, d + size);
+}
+
+// Host checks of the scales that go with a pool: strides by which pages and heads do not overlap.
+inline bool scales_ok(const Scales& f, const Pools& p, int Hk, int page_size) {
+  const long long head = page_size / kScaleRows;
+  if (!f.k || !f.v || f.page_stride < 0 || f.head_stride < 0 || f.page_stride >> 46 || f.head_stride >> 46) return false;
+  if ((Hk > 1 && f.head_stride < head) || (p.n_pages > 1 && f.page_stride < head)) return false;
+  return Hk == 1 || p.n_pages == 1 || (__int128)(Hk - 1) * f.head_stride + head <= f.page_stride ||
+         (__int128)(p.n_pages - 1) * f.page_stride + head <= f.head_stride;
+}
+
+// The scales as pools of one byte per element, for the checks above.
+inline Pools scale_pools(const Scales& f, int n_pages) {
+  return Pools{reinterpret_cast<uint16_t*>(f.k), reinterpret_cast<uint16_t*>(f.v), f.page_stride, f.head_stride, n_pages, 1};
+}
+
+// Whether a pool's pages (heads of `x` bytes) and another's (of `y`) share no byte. Exact where pages are equally far
+// apart in both; else their spans have to be apart.
+inline bool sets_apart(const void* a, const Pools& p, long long x, const void* b, const Pools& r, long long y, int Hk) {
+  const long long pages = p.n_pages - 1, heads = Hk - 1;
+  const __int128 ap = pages ? (__int128)p.size * p.page_stride : 0, ah = heads ? (__int128)p.size * p.head_stride : 0;
+  const __int128 bp = pages ? (__int128)r.size * r.page_stride : 0, bh = heads ? (__int128)r.size * r.head_stride : 0;
+  const __int128 d = (__int128)reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a);
+  if (d >= pages * ap + heads * ah + x || -d >= pages * bp + heads * bh + y) return true;
+  if (ap != bp) return false;
+  for (int i = 0; i < Hk; ++i)
+    for (int j = 0; j < Hk; ++j) {
+      // pages m of b and n of a overlap where (m - n) * ap lies in (-y - at, x - at)
+      const __int128 at = d + j * bh - i * ah;
+      if (pages == 0) {
+        if (at > -(__int128)y && at < x) return false;
+        continue;
+      }
+      const __int128 lo = -(__int128)y - at, hi = x - at;
+      __int128 k = lo / ap - (lo % ap < 0) + 1;  // the first k with k * ap > lo
+      if (k < -pages) k = -pages;
+      if (k <= pages && k * ap < hi) return false;
+    }
+  return true;
 }
 
 }  // namespace ns
