@@ -82,6 +82,40 @@ int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, co
                        void* stream);
 
 /*
+ * The same over a cache in 8 bits. Pools of e4m3 codes (strides in bytes, multiples of 16), and beside them scales: one
+ * byte e per 16 rows of a page and head, for 2^(e - 127), at k_scales + page * scale_page_stride + head *
+ * scale_head_stride + row / 16, v_scales alike. A value is code times scale.
+ *
+ * ns_paged_append_fp8: y as ns_paged_append's, in fp32. For the new rows of a block of 16 positions of one sequence and
+ * kv head, K and V apart, t their largest finite magnitude: e' = the least with t <= 448 * 2^e', held to [-110, 119]; where
+ * the block has rows from before (its first new position is no multiple of 16) the larger of that and the scale
+ * there (held to the same), and those rows' codes become e4m3(code * 2^(e - e')). Codes are e4m3(y / 2^e'), rounded to
+ * nearest even, held to 448; NaN and infinities become NaN. D 64 or 128, T * Hk < 2^29; -2 also for scales over anything
+ * else, or over pages (where neither the spans are apart nor the page strides the same).
+ * Two sequences that append to one page leave one of the two values of each element and scale, which need not
+ * belong together.
+ *
+ * ns_paged_attention_fp8: ns_paged_attention over the values. The query enters the first product as two e4m3
+ * terms under a power of two per head: exact down to 2^-14 of the head's largest magnitude, within 2^-22 of it below,
+ * held to 448 * 2^119; infinities in it become NaN. A scale byte of 255 counts as 254.
+ */
+int ns_paged_append_fp8(const void* qkv, long long qkv_stride, const void* bias, const void* inv_freq,
+                        const int* q_start, const int* lens, const int* table, long long table_stride,
+                        int width, void* k_pool, void* v_pool, long long page_stride,
+                        long long head_stride, void* k_scales, void* v_scales,
+                        long long scale_page_stride, long long scale_head_stride, int n_pages,
+                        int page_size, void* q_out, int T, int B, int Hq, int Hk, int D, void* stream);
+size_t ns_paged_attention_fp8_workspace(int T, int B, int Hq, int Hk, int D, int max_len, int ragged,
+                                        int shared);
+int ns_paged_attention_fp8(const void* q, long long q_stride, const void* k_pool, const void* v_pool,
+                           long long page_stride, long long head_stride, const void* k_scales,
+                           const void* v_scales, long long scale_page_stride, long long scale_head_stride,
+                           int n_pages, int page_size, const int* table, long long table_stride, int width,
+                           const int* lens, const int* q_start, void* out, void* work, size_t work_bytes,
+                           int T, int B, int Hq, int Hk, int D, int shared, int window, int sinks,
+                           float scale, void* stream);
+
+/*
  * Bytes of workspace ns_sample uses for these sizes, 0 for none or for sizes it rejects. Launches that
  * may overlap in time need workspaces of their own.
  */

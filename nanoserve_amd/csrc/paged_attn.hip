@@ -209,46 +209,7 @@ __device__ __forceinline__ void one_body(const PagedArgs& a, int item, int g, co
   l += lane_xor32(l);
   m = seen_max(m, seen);
 
-  // ---- merge of the waves through their (then free) first stages: fp32, heads 0 .. 7 in the K half and
-  // 8 .. 15 in the V half
-  auto (&red_m) = red[0];
-  auto (&red_l) = red[1];
-  float *ok = reinterpret_cast<float*>(lds.k[0]), *ov_ = reinterpret_cast<float*>(lds.v[0]);
-  float* half = (grp < 2 ? ok : ov_) + wv * kBlk / 2 + (4 * grp & 7) * D;
-#pragma unroll
-  for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) half[r * D + 16 * d + r16] = o[d][r];
-  if (grp == 0) {
-    red_m[wv][r16] = m;
-    red_l[wv][r16] = l;
-  }
-  lds_sync();
-  for (int i = tid; i < R * D; i += kOneWaves * kWave) {
-    const int hh = i / D, d = i % D;
-    float mt = red_m[0][hh];
-#pragma unroll
-    for (int k = 1; k < kOneWaves; ++k) mt = fmaxf(mt, red_m[k][hh]);
-    const float mz = mt == -INFINITY ? 0.f : mt;
-    float ov = 0.f, lt = 0.f;
-#pragma unroll
-    for (int k = 0; k < kOneWaves; ++k) {
-      const float f = exp2f(red_m[k][hh] - mz);  // 0 for a wave without keys
-      ov = fmaf(f, (hh < 8 ? ok : ov_)[k * kBlk / 2 + (hh & 7) * D + d], ov);
-      lt = fmaf(f, red_l[k][hh], lt);
-    }
-    const int h = g * R + hh;
-    if (direct) {
-      a.out[((size_t)b * a.Hq + h) * D + d] =
-          static_cast<uint16_t>(f32_to_bf16_rne(mt == -INFINITY ? 0.f : ov / lt));
-    } else {
-      const size_t row = (size_t)(slot + split) * a.Hq + h;
-      a.opart[row * D + d] = ov;
-      if (d == 0) *reinterpret_cast<float2*>(&a.ml[row * 2]) = make_float2(mt, lt);
-    }
-  }
-  // (also where the result is final, so that the merge does not read an older launch's entry)
-  if (a.rows && split == 0 && g == 0 && tid == 0) a.rows[b] = make_int4((int)slot, 1, sp.splits, 0);
+  one_finish<D>(a, lds, red, o, m, l, b, g, split, slot, sp.splits, direct);
 }
 
 // The launch: workgroups of the shared keys first (kWithShared), then those of the sequences' own keys. Both in

@@ -240,6 +240,152 @@ __device__ __forceinline__ void wait_loads(int n) {
 // divide 0 by 0 alone.
 __device__ __forceinline__ float seen_max(float m, bool seen) { return seen ? fmaxf(m, -FLT_MAX) : -INFINITY; }
 
+// The end of the one-token kernels: merge of the waves through their (then free) first stages, fp32, heads 0 .. 7
+// in the K half and 8 .. 15 in the V half. o: heads 4 grp + r at dim 16 d + r16 of a wave; m, l: of head r16.
+template <int D>
+__device__ __forceinline__ void one_finish(const PagedArgs& a, const Ring& lds, float (&red)[2][kOneWaves][16],
+                                           const f32x4_t (&o)[D / 16], float m, float l, int b, int g, int split,
+                                           long long slot, int splits, bool direct) {
+  constexpr int kBlk = 16 * D;  // a wave's part of a stage, in units of 2 bytes
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, grp = lane >> 4, R = a.R;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto (&red_m) = red[0];
+  auto (&red_l) = red[1];
+  float *ok = reinterpret_cast<float*>(lds.k[0]), *ov_ = reinterpret_cast<float*>(lds.v[0]);
+  float* half = (grp < 2 ? ok : ov_) + wv * kBlk / 2 + (4 * grp & 7) * D;
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) half[r * D + 16 * d + r16] = o[d][r];
+  if (grp == 0) {
+    red_m[wv][r16] = m;
+    red_l[wv][r16] = l;
+  }
+  lds_sync();
+  for (int i = tid; i < R * D; i += kOneWaves * kWave) {
+    const int hh = i / D, d = i % D;
+    float mt = red_m[0][hh];
+#pragma unroll
+    for (int k = 1; k < kOneWaves; ++k) mt = fmaxf(mt, red_m[k][hh]);
+    const float mz = mt == -INFINITY ? 0.f : mt;
+    float ov = 0.f, lt = 0.f;
+#pragma unroll
+    for (int k = 0; k < kOneWaves; ++k) {
+      const float f = exp2f(red_m[k][hh] - mz);  // 0 for a wave without keys
+      ov = fmaf(f, (hh < 8 ? ok : ov_)[k * kBlk / 2 + (hh & 7) * D + d], ov);
+      lt = fmaf(f, red_l[k][hh], lt);
+    }
+    const int h = g * R + hh;
+    if (direct) {
+      a.out[((size_t)b * a.Hq + h) * D + d] =
+          static_cast<uint16_t>(f32_to_bf16_rne(mt == -INFINITY ? 0.f : ov / lt));
+    } else {
+      const size_t row = (size_t)(slot + split) * a.Hq + h;
+      a.opart[row * D + d] = ov;
+      if (d == 0) *reinterpret_cast<float2*>(&a.ml[row * 2]) = make_float2(mt, lt);
+    }
+  }
+  // (also where the result is final, so that the merge does not read an older launch's entry)
+  if (a.rows && split == 0 && g == 0 && tid == 0) a.rows[b] = make_int4((int)slot, 1, splits, 0);
+}
+
+// ------------------------------------------------------------------ caches in 8 bits
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ i32x8_t join(const u32x4_t& a, const u32x4_t& b) {
+  return (i32x8_t){(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
+// The scales of the 16 rows of a page and head that hold position `key`, K's in bits 0 .. 7 and V's in 8 .. 15; one for
+// what is no page. 255, no power of two and never written by an append, counts as the one below it: rows that
+// nobody sees are zeros times their scale. The value is waited for here, or the compiler would wait at every use,
+// behind the ring's loads.
+constexpr int kNoScales = 127 | 127 << 8;
+__device__ __forceinline__ int group_scales(const PagedArgs& a, int id, int g, int key) {
+  int s = kNoScales;
+  if ((unsigned)id < (unsigned)a.p.n_pages) {
+    const size_t at = (size_t)id * a.f.page_stride + (size_t)g * a.f.head_stride + key % a.s.page_size / kScaleRows;
+    s = min((int)a.f.k[at], 254) | min((int)a.f.v[at], 254) << 8;
+  }
+  asm volatile("" : "+v"(s));
+  return s;
+}
+
+// Eight codes as bf16, exact: the first four times one scale, the others times another (powers of two).
+__device__ __forceinline__ bf16x8_t f8_values(u32x2_t x, float s0, float s1) {
+  u32x4_t v;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float s = i ? s1 : s0;
+    v[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[i], s, false));
+    v[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[i], s, true));
+  }
+  return __builtin_bit_cast(bf16x8_t, v);
+}
+
+// ds_read_b64_tr_b8: the 16 lanes of a group read 8 rows of 16 bytes, lane l half l % 2 of row l / 2, and lane l
+// receives byte l of each row, in order.
+__device__ __forceinline__ u32x2_t lds_read_tr8(const uint16_t* p) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                         (__attribute__((address_space(3))) i32x2_t*)const_cast<uint16_t*>(p)));
+}
+
+// s + A B for 32 keys and 32 queries over 64 dims of e4m3, with a power of two per row of either: bytes `ka` of
+// ks and `qa` of qs.
+__device__ __forceinline__ f32x16_t scaled_product(const i32x8_t& k, const i32x8_t& q, const f32x16_t& s, int ka, int ks,
+                                                   int qa, int qs) {
+  if (ka == 0)
+    return qa == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 0, ks, 0, qs)
+                   : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 0, ks, 1, qs);
+  return qa == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 1, ks, 0, qs)
+                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 1, ks, 1, qs);
+}
+
+// A query head's values as two e4m3 terms, x = 2^e (hi + lo / 16). bf16 has the 8 significant bits of two
+// e4m3: lo, what hi's rounding left times 16, is at most 8 of its units, so the terms are exact for values down to 2^-14 of
+// the head's largest, and within 2^-22 of that below. NaN and infinities become NaN.
+// The head's exponent e; a lane holds N * 8 of the values (bf16), the lanes l ^ 32 (and l ^ 16, kOver16) the others.
+template <int N, bool kOver16>
+__device__ __forceinline__ int query_exponent(const u32x4_t (&q)[N]) {
+  uint32_t top = 0;  // of the magnitudes, as bf16 bits << 16; infinities and NaN do not count
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t m = (i & 1 ? q[s][i / 2] : q[s][i / 2] << 16) & 0x7fff0000u;
+      top = max(top, m < 0x7f800000u ? m : 0u);
+    }
+  float t = __uint_as_float(top);
+  t = fmaxf(t, lane_xor32(t));
+  if constexpr (kOver16) t = fmaxf(t, lane_xor16(t));
+  return scale_exponent(t);
+}
+
+// Eight of the values.
+__device__ __forceinline__ void query_terms(const u32x4_t& q, int e, u32x2_t& hi, u32x2_t& lo) {
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  auto fit = [&](uint32_t bits) {
+    return (bits & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u) : held448(__uint_as_float(bits) * inv);
+  };
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    uint32_t h = 0, l = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = fit(q[2 * w + i] << 16), y = fit(q[2 * w + i] & 0xffff0000u);
+      const int b = __builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false);
+      const auto back = __builtin_amdgcn_cvt_pk_f32_fp8(b, false);
+      const int r = __builtin_amdgcn_cvt_pk_fp8_f32((x - back[0]) * 16.f, (y - back[1]) * 16.f, 0, false);
+      h |= (uint32_t)(b & 0xffff) << (16 * i);
+      l |= (uint32_t)(r & 0xffff) << (16 * i);
+    }
+    hi[w] = h;
+    lo[w] = l;
+  }
+}
+
 // ------------------------------------------------------------------ tiles of query rows
 // Bound by the matrix cores and the softmax's VALU work beside them. The rows of a kv head's problem are its R query heads'
 // tokens, token-major (row = token * R + head): one K / V tile serves all heads of the group. kShared:
@@ -263,10 +409,11 @@ __device__ __forceinline__ float seen_max(float m, bool seen) { return seen ? fm
 // products of its neighbours did not help (659 -> 681 to 730 us). 4095 tokens with a window of 1000 and 14 / 2 heads of
 // 64 43 us. 96 drafts of 1 to 3 tokens behind 16384 shared positions 100 to 104 us back to back, 108 to 117 among
 // other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD.
-template <int D, bool kShared>
+template <int D, bool kShared, bool kF8 = false>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
-  constexpr int kChunks = D / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad, kDT = D / 32,
-                kStages = ring_stages<D>();
+  // (kRow: a row of the cache in units of 2 bytes)
+  constexpr int kRow = kF8 ? D / 2 : D, kChunks = kRow / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad,
+                kDT = D / 32, kStages = ring_stages<D>();
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = a.R;
@@ -364,9 +511,27 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   const int j0 = (int)((long long)kb.count() * split / splits);
   const int j1 = (int)((long long)kb.count() * (split + 1) / splits);
 
-  // B operand of the scores: this lane's query at dims 16 s + 8 kh ..
+  // B operand of the scores: this lane's query at dims 16 s + 8 kh .. (8 bits: 64 s + 32 kh .., in two terms)
   u32x4_t qf[D / 16];
-  {
+  int qe = 0;  // the exponents of the terms' scales, a byte each
+  if constexpr (kF8) {
+    const uint16_t* qp = a.q + (size_t)t * a.q_stride + (size_t)hq * D + 32 * kh;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(qp + 64 * (s / 4) + 8 * (s % 4));
+    const int e = query_exponent<D / 16, false>(qf);
+    qe = (e + 127) | (e - 4 + 127) << 8;
+#pragma unroll
+    for (int s = 0; s < D / 16; s += 4) {  // 32 values: two vectors of hi, two of lo
+      u32x2_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) query_terms(qf[s + i], e, hi[i], lo[i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        qf[s + i] = (u32x4_t){hi[2 * i][0], hi[2 * i][1], hi[2 * i + 1][0], hi[2 * i + 1][1]};
+        qf[s + 2 + i] = (u32x4_t){lo[2 * i][0], lo[2 * i][1], lo[2 * i + 1][0], lo[2 * i + 1][1]};
+      }
+    }
+  } else {
     const uint16_t* qp = a.q + (size_t)t * a.q_stride + (size_t)hq * D + 8 * kh;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const u32x4_t*>(qp + 16 * s);
@@ -375,27 +540,33 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   // lane i: offset in the pools of 16-row group i % 4 of block j0 + 16 (.. / 16) + i / 4 of the list
   const int* table = a.s.table + (size_t)b * a.s.table_stride;
   uint64_t offs = 0, valid = 0;
+  int scales = kNoScales;  // of the lane's group
   auto refill = [&](int j) {
     const int v = j + (lane >> 2);
-    int id = -1;
+    int id = -1, key = 0;
     if (v < j1) {
-      const int key = kTileKeys * kb.block(v) + 16 * (lane & 3);
+      key = kTileKeys * kb.block(v) + 16 * (lane & 3);
       if (key < top) id = table[key / a.s.page_size];
-      offs = 2 * ((uint64_t)(uint32_t)id * a.p.page_stride + (uint64_t)g * a.p.head_stride +
-                  (uint64_t)(key % a.s.page_size) * D);
+      offs = (kF8 ? 1 : 2) * ((uint64_t)(uint32_t)id * a.p.page_stride + (uint64_t)g * a.p.head_stride +
+                              (uint64_t)(key % a.s.page_size) * D);
     }
     valid = __ballot((unsigned)id < (unsigned)a.p.n_pages);
+    if constexpr (kF8) scales = group_scales(a, id, g, key);
   };
-  auto k_swz = [](int r) { return D == 128 ? r & 15 : (r >> 1) & 7; };
-  auto v_swz = [](int r) { return D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; };
+  // (16-byte chunks of a row lie in the order c ^ swz(row), so that the rows of one read hit distinct banks)
+  auto k_swz = [](int r) { return kF8 ? (D == 128 ? (r >> 1) & 7 : (r >> 2) & 3) : D == 128 ? r & 15 : (r >> 1) & 7; };
+  auto v_swz = [](int r) {
+    return kF8 ? (D == 128 ? 2 * ((r >> 1 & 1) | (r >> 2 & 2)) : 2 * (r >> 3 & 1))
+               : D == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
+  };
   uint32_t k_off[kLoads], v_off[kLoads];  // of this lane's 16 bytes in a group
   const int lr = lane / kChunks;
 #pragma unroll
   for (int p = 0; p < kLoads; ++p) {
     const int r = kRowsPerLoad * p + lr;
     const uint32_t ch = lane % kChunks;
-    k_off[p] = r * 2 * D + 16u * (ch ^ k_swz(16 * wv + r));
-    v_off[p] = r * 2 * D + 16u * (ch ^ v_swz(r));
+    k_off[p] = r * 2 * kRow + 16u * (ch ^ k_swz(16 * wv + r));
+    v_off[p] = r * 2 * kRow + 16u * (ch ^ v_swz(r));
   }
   // Bit i: some row of the tile sees position key0 + i, i < 16.
   auto seen16 = [&](int key0) {
@@ -408,11 +579,14 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     }
     return wave_or(bits);
   };
-  auto issue = [&](uint16_t* ks, uint16_t* vs, int j, uint32_t& groups) {
+  auto issue = [&](uint16_t* ks, uint16_t* vs, int j, uint32_t& groups, int (&sc)[4]) {
     const int jj = j - j0;
     if ((jj & 15) == 0) refill(j);
     const int e = 4 * (jj & 15);
     groups = (uint32_t)(valid >> e) & 15u;
+    if constexpr (kF8)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) sc[u] = __builtin_amdgcn_readlane(scales, e + u);
     const int key0 = kTileKeys * kb.block(j) + 16 * wv;
     uint32_t sees = 0xffffu;
     if constexpr (kShared)
@@ -422,21 +596,21 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)offs, e + wv)
                             : 0;
     const auto kres = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(a.p.k) + off, (short)0,
-                                                        ok ? 32 * D : 0, 0x00020000);
+                                                        ok ? 32 * kRow : 0, 0x00020000);
     const auto vres = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<char*>(a.p.v) + off, (short)0,
-                                                        ok ? 32 * D : 0, 0x00020000);
+                                                        ok ? 32 * kRow : 0, 0x00020000);
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) attn_lds_load16(kres, &ks[16 * wv * D + 512 * p], k_off[p], 0);
+    for (int p = 0; p < kLoads; ++p) attn_lds_load16(kres, &ks[16 * wv * kRow + 512 * p], k_off[p], 0);
     if (gaps ? sees == 0xffffu : key0 >= k0 && key0 >= low && key0 + 16 <= top) {
 #pragma unroll
-      for (int p = 0; p < kLoads; ++p) attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], v_off[p], 0);
+      for (int p = 0; p < kLoads; ++p) attn_lds_load16(vres, &vs[16 * wv * kRow + 512 * p], v_off[p], 0);
     } else {  // value rows that no row of the tile sees are zero, whatever the page holds
 #pragma unroll
       for (int p = 0; p < kLoads; ++p) {
         const int key = key0 + kRowsPerLoad * p + lr;
         const bool see = gaps ? ((sees >> (key - key0)) & 1) != 0
                               : (key >= k0) & (key < top) & ((key >= low) | (key < first));
-        attn_lds_load16(vres, &vs[16 * wv * D + 512 * p], see ? v_off[p] : kOut, 0);
+        attn_lds_load16(vres, &vs[16 * wv * kRow + 512 * p], see ? v_off[p] : kOut, 0);
       }
     }
   };
@@ -449,23 +623,44 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   float m = -INFINITY, l = 0.f;
   const float c = a.c;
 
-  // transpose-read offsets (elements) of the 32-dim tiles at key row 4 kh + (lane % 16) / 4
+  // transpose-read offsets (in units of 2 bytes) of the 32-dim tiles at key row 4 kh + (lane % 16) / 4; 8 bits: at
+  // the key rows of the probabilities' order, 4 kh .. + 3 and 8 + 4 kh .. + 3, two lanes to a row
   int vt[kDT];
-  {
+  if constexpr (kF8) {
+    const int i = lane & 15, rr = 4 * kh + ((i >> 1) & 3) + 8 * (i >> 3);
+#pragma unroll
+    for (int d = 0; d < kDT; ++d)
+      vt[d] = rr * kRow + 8 * ((2 * d + ((lane >> 4) & 1)) ^ v_swz(rr)) + 4 * (lane & 1);
+  } else {
     const int rr = 4 * kh + ((lane & 15) >> 2);
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
       vt[d] = rr * D + 8 * ((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swz(rr)) + 4 * (lane & 1);
   }
 
-  auto compute = [&](const uint16_t* kt, const uint16_t* vb, int j, uint32_t groups) {
+  auto compute = [&](const uint16_t* kt, const uint16_t* vb, int j, uint32_t groups, const int (&sc)[4]) {
     const int key0 = kTileKeys * kb.block(j);
     if (key0 >= hi_max || (key0 + kTileKeys <= lo_min && key0 >= first)) return;  // no row sees it
     f32x16_t s[2];
+    // (scale bytes of this lane's key: of its group in the first 32 keys, then in the second 32)
+    const int kscale = kF8 ? (jq & 16 ? sc[1] & 0xff : sc[0] & 0xff) | (jq & 16 ? sc[3] & 0xff : sc[2] & 0xff) << 8 : 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+      if constexpr (kF8) {
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) {
+          const int kr = 32 * u + jq;
+          const u32x4_t k0 = *reinterpret_cast<const u32x4_t*>(&kt[kr * kRow + 8 * ((4 * d + 2 * kh) ^ k_swz(kr))]);
+          const u32x4_t k1 = *reinterpret_cast<const u32x4_t*>(&kt[kr * kRow + 8 * ((4 * d + 2 * kh + 1) ^ k_swz(kr))]);
+          const i32x8_t kf = join(k0, k1);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)  // the query's terms
+            s[u] = scaled_product(kf, join(qf[4 * d + 2 * i], qf[4 * d + 2 * i + 1]), s[u], u, kscale, i, qe);
+        }
+        continue;
+      }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) {
         const int kr = 32 * u + jq;
@@ -531,8 +726,14 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       bf16x8_t vf[kDT];
+      if constexpr (kF8) {
+        const float scale = __uint_as_float((uint32_t)(sc[u] >> 8) << 23);
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) vf[d] = f8_values(lds_read_tr8(&vb[vt[d] + 16 * u * kRow]), scale, scale);
+      }
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
+        if constexpr (kF8) break;
         const u32x2_t v0 = lds_read_tr16(&vb[vt[d] + 16 * u * D]);
         const u32x2_t v1 = lds_read_tr16(&vb[vt[d] + (16 * u + 8) * D]);
         vf[d] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v0[0], v0[1], v1[0], v1[1]});
@@ -549,9 +750,10 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   // in flight), and past the barrier nobody reads block j - 1, whose stage is loaded next: each wave waits for
   // its loads of j and its reads of j - 1.
   uint32_t gr[kStages];
+  int sg[kStages][4];
   auto fill = [&](auto stage, int j) {
     constexpr int S = decltype(stage)::value;
-    if (j < j1) issue(lds.k[S], lds.v[S], j, gr[S]);
+    if (j < j1) issue(lds.k[S], lds.v[S], j, gr[S], sg[S]);
   };
   auto step = [&](auto stage, auto last, int j) {
     constexpr int S = decltype(stage)::value;
@@ -559,7 +761,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     wait_loads(2 * kLoads * min(j1 - 1 - j, kStages - 2));
     lds_sync();
     fill(last, j + kStages - 1);
-    compute(lds.k[S], lds.v[S], j, gr[S]);
+    compute(lds.k[S], lds.v[S], j, gr[S], sg[S]);
   };
   using S0 = std::integral_constant<int, 0>;
   using S1 = std::integral_constant<int, 1>;

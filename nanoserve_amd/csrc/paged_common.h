@@ -55,6 +55,15 @@ struct Scales {
   long long page_stride, head_stride;
 };
 constexpr int kScaleRows = 16;
+// Of a scale: the least e with t <= 448 * 2^e, between these two (so that every code times its scale is a normal bf16,
+// or 0: 2^-9 * 2^-110 and 448 * 2^119). t finite and not negative.
+constexpr int kLeastScale = -110, kMostScale = 119;
+__device__ __forceinline__ int scale_exponent(float t) {
+  const uint32_t b = __float_as_uint(t);  // 448 = 1.75 * 2^8
+  return min(max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u), kLeastScale), kMostScale);
+}
+// Held to e4m3's range, 448 (the conversion would make NaN of what lies past 464); NaN stays.
+__device__ __forceinline__ float held448(float x) { return fabsf(x) > 448.f ? copysignf(448.f, x) : x; }
 
 // Host checks common to the entry points.
 inline bool batch_ok(const Batch& s, const Pools& p, int Hk, int D) {

@@ -52,7 +52,7 @@ SIGNATURES["ns_probe_linear_loop"] = [_VP] * 7 + [_I32, _I32, _VP]
 RESTYPES = {"ns_decode_attention_workspace": _SZ, "ns_w4_gptq_workspace": _SZ,
             "ns_w4_linear_workspace": _SZ, "ns_prompt_attention_workspace": _SZ,
             "ns_w4_linear_swiglu_rows_workspace": _SZ, "ns_paged_attention_workspace": _SZ,
-            "ns_sample_workspace": _SZ}
+            "ns_sample_workspace": _SZ, "ns_paged_attention_fp8_workspace": _SZ}
 # Entry points of this package's own callers (csrc/internal_ops.h, csrc/batch_ops.h), not part of the
 # public ABI.
 INTERNAL_SIGNATURES = {
@@ -69,6 +69,11 @@ INTERNAL_SIGNATURES = {
     "ns_paged_attention_workspace": [_I32] * 8,
     "ns_paged_attention": [_VP, _I64, _VP, _VP, _I64, _I64, _I32, _I32, _VP, _I64, _I32, _VP, _VP, _VP,
                            _VP, _SZ] + [_I32] * 8 + [_F32, _VP],
+    "ns_paged_append_fp8": [_VP, _I64] + [_VP] * 5 + [_I64, _I32, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _I64,
+                                                      _I32, _I32, _VP] + [_I32] * 5 + [_VP],
+    "ns_paged_attention_fp8_workspace": [_I32] * 8,
+    "ns_paged_attention_fp8": [_VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _I32, _I32, _VP, _I64, _I32,
+                               _VP, _VP, _VP, _VP, _SZ] + [_I32] * 8 + [_F32, _VP],
     "ns_sample_workspace": [_I32] * 3,
     "ns_sample": [_VP, _I32, _I64, _VP, _VP, _F32, _VP, _I32, _VP, _F32, _VP, _F32, _VP, _VP, _SZ, _I32,
                   _I32, _VP],
@@ -639,12 +644,12 @@ class Kernels:
 
     # ------------------------------------------------------------------ a batch over a paged cache
     @staticmethod
-    def _batch_args(T, pages, lens, k_pages, v_pages, q_start, here):
+    def _batch_args(T, pages, lens, k_pages, v_pages, q_start, here, dtype=torch.bfloat16):
         """Checks of a batch's metadata and pools; returns them as the C entry points take them."""
         _require_here(pages, "pages", torch.int32, here)
         _require_here(lens, "lens", torch.int32, here)
-        _require_here(k_pages, "k_pages", torch.bfloat16, here)
-        _require_here(v_pages, "v_pages", torch.bfloat16, here)
+        _require_here(k_pages, "k_pages", dtype, here)
+        _require_here(v_pages, "v_pages", dtype, here)
         shape, strides = k_pages.shape, k_pages.stride()
         if len(shape) != 4 or strides[3] != 1 or strides[2] != shape[3]:
             raise ValueError("k_pages must be [n_pages, Hk, page_size, D] with contiguous heads")
@@ -771,6 +776,114 @@ class Kernels:
             None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
             Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
         self._check(rc, "ns_paged_attention")
+        return out
+
+    @staticmethod
+    def _scale_args(k_scales, v_scales, n_pages, Hk, page_size, here):
+        """Checks of the scales of a cache in 8 bits; returns them as the C entry points take them."""
+        _require_here(k_scales, "k_scales", torch.float8_e8m0fnu, here)
+        _require_here(v_scales, "v_scales", torch.float8_e8m0fnu, here)
+        blocks = page_size // 16
+        strides = k_scales.stride()
+        if tuple(k_scales.shape) != (n_pages, Hk, blocks) or (blocks > 1 and strides[2] != 1):
+            raise ValueError("k_scales must be [n_pages, Hk, page_size / 16] with contiguous heads")
+        if v_scales.shape != k_scales.shape or v_scales.stride() != strides:
+            raise ValueError("k_scales and v_scales must be alike")
+        return (k_scales.data_ptr(), v_scales.data_ptr(), strides[0] if n_pages > 1 else 0,
+                strides[1] if Hk > 1 else 0)
+
+    def paged_append_fp8(self, qkv, bias, inv_freq, pages, lens, k_pages, v_pages, k_scales, v_scales, n_heads,
+                         q_start=None, out=None):
+        """paged_append to a cache in 8 bits: k_pages, v_pages [n_pages, Hk, page_size, D] float8_e4m3fn (head
+        size 64 or 128), k_scales, v_scales [n_pages, Hk, page_size / 16] float8_e8m0fnu, one power of two for each
+        16 positions and kv head; a value is its code times its scale. Returns the q heads [T, Hq * D], bf16.
+
+        The scale is the least with which the block's largest magnitude fits (448 of it), in 2^-110 .. 2^119; with rows of
+        the block from before it rises where new ones need it and never falls, and their codes are rounded to the new
+        scale (for most values exact: the exponent moves). A block of which no earlier position is the sequence's
+        starts anew, whatever its scale held. NaN and infinities are stored as NaN and do not count for the scale.
+        Everything else as paged_append; rows of the pages that no new token writes keep their values."""
+        here = _device_of(qkv, "qkv", torch.bfloat16)
+        _require_here(inv_freq, "inv_freq", torch.float32, here)
+        if qkv.dim() != 2 or qkv.stride(1) != 1:
+            raise ValueError("qkv must be [T, (Hq + 2Hk) * D] with contiguous rows")
+        T, columns = qkv.shape
+        B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
+                                                                        q_start, here, torch.float8_e4m3fn)
+        scales = self._scale_args(k_scales, v_scales, n_pages, Hk, page_size, here)
+        if columns != (n_heads + 2 * Hk) * D:
+            raise ValueError("qkv must hold n_heads + 2 Hk heads of D values per row")
+        if inv_freq.numel() != D // 2 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be contiguous with head_dim / 2 elements")
+        if bias is not None:
+            _require_here(bias, "bias", torch.bfloat16, here)
+            if bias.numel() != columns or not bias.is_contiguous():
+                raise ValueError("bias must be contiguous with one value per column of qkv")
+        if out is None:
+            out = qkv.new_empty((T, n_heads * D))
+        else:
+            _require_here(out, "out", torch.bfloat16, here)
+            if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
+            _apart(out, qkv, "qkv")
+        if T == 0 or B == 0:
+            return out
+        rc = self.lib.ns_paged_append_fp8(
+            qkv.data_ptr(), qkv.stride(0) if T > 1 else columns,
+            None if bias is None else bias.data_ptr(), inv_freq.data_ptr(),
+            None if q_start is None else q_start.data_ptr(), lens.data_ptr(), *table, k_pages.data_ptr(),
+            v_pages.data_ptr(), *strides, *scales, n_pages, page_size, out.data_ptr(), T, B, n_heads, Hk, D,
+            _raw_stream(here))
+        self._check(rc, "ns_paged_append_fp8")
+        return out
+
+    def paged_attention_fp8_workspace(self, T, B, n_heads, n_kv_heads, head_dim, max_len, ragged=False,
+                                      shared=0, device=None):
+        """paged_attention_workspace for paged_attention_fp8."""
+        n = int(self.lib.ns_paged_attention_fp8_workspace(T, B, n_heads, n_kv_heads, head_dim, _int32(max_len),
+                                                          int(ragged), _int32(shared)))
+        return torch.empty(n, dtype=torch.uint8, device=device or "cuda") if n else None
+
+    def paged_attention_fp8(self, q, k_pages, v_pages, k_scales, v_scales, pages, lens, n_heads, q_start=None,
+                            shared=0, window=0, sinks=0, scale=None, work=None, out=None):
+        """paged_attention over a cache in 8 bits (pools and scales as paged_append_fp8 writes them): the result of
+        paged_attention over a bf16 cache that holds code times scale, but for infinities in a query, which count as NaN,
+        query magnitudes above 448 * 2^119, which are held to it, and those below 2^-14 of their head's largest, which are
+        held to 2^-22 of it. ``work``: from paged_attention_fp8_workspace."""
+        here = _device_of(q, "q", torch.bfloat16)
+        if q.dim() != 2 or q.stride(1) != 1:
+            raise ValueError("q must be [T, Hq * D] with contiguous rows")
+        T, columns = q.shape
+        B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
+                                                                        q_start, here, torch.float8_e4m3fn)
+        scales = self._scale_args(k_scales, v_scales, n_pages, Hk, page_size, here)
+        if columns != n_heads * D:
+            raise ValueError("q must hold n_heads heads of D values per row")
+        if out is None:
+            out = q.new_empty((T, columns))
+        else:
+            _require_here(out, "out", torch.bfloat16, here)
+            if tuple(out.shape) != (T, columns) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{T}, {columns}] tensor")
+            _apart(out, q, "q")
+        if T == 0 or B == 0:
+            return out
+        if (shared | window | sinks) >> 31:  # one below 0 or past 32 bits
+            shared, window, sinks = _int32(shared), _int32(window), _int32(sinks)
+        if work is None:
+            work = self.paged_attention_fp8_workspace(T, B, n_heads, Hk, D, table[2] * page_size,
+                                                      q_start is not None, shared, device=q.device)
+        else:
+            _require_here(work, "work", torch.uint8, here)
+            if not work.is_contiguous():
+                raise _strided_work()
+        rc = self.lib.ns_paged_attention_fp8(
+            q.data_ptr(), q.stride(0) if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
+            *strides, *scales, n_pages, page_size, *table, lens.data_ptr(),
+            None if q_start is None else q_start.data_ptr(), out.data_ptr(),
+            None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
+            Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
+        self._check(rc, "ns_paged_attention_fp8")
         return out
 
     # ------------------------------------------------------------------ the next token
