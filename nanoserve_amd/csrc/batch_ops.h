@@ -116,6 +116,71 @@ int ns_paged_attention_fp8(const void* q, long long q_stride, const void* k_pool
                            float scale, void* stream);
 
 /*
+ * Table entries, first rows and slot map of a step, from its sequences' new lengths: sequence b has lens[b] positions
+ * (held to 0 .. width * page_size) and gets add[b] more, or gives back -add[b] of them. In place:
+ *   lens [B]       becomes max(lens + add, 0)
+ *   table          entries ceil(old / page_size) .. ceil(new / page_size) - 1 of a sequence that grows are taken from
+ *                  the stack, in the order of the sequences and entries, its top first. The entries of one that shrinks
+ *                  from ceil(new / page_size) on go back to it (and stay in the table), the last one first: what one call
+ *                  took and a later one gives back lies there as before. Pages given back count for the same call.
+ *   free, n_free   the stack: pages free[0 .. n_free[0] - 1], the top last, room for `capacity`
+ * Written: q_start [B + 1], the running sum of max(add, 0) from 0 on; slots [rows], of each new token in that order
+ * page * page_size + row, -1 where the table's entry is below 0 and behind the last sequence's (rows -1: no slot map, slots
+ * unused); shorts [1]: 0.
+ * A call that does not go through as a whole changes nothing: q_start is all 0 (rows of no sequence, on which the operators
+ * here do nothing), slots are -1, and shorts is the number of pages that are missing, or -1 where a sequence would pass its
+ * table row, more than `rows` tokens are new, or the stack would pass its capacity.
+ * Entries given back must not be in use by other rows. -2 for sizes <= 0 (B >= 2^24, rows < -1, capacity < 0 or >= 2^31),
+ * page_size % 16, width * page_size >= 2^30, table_stride < width, NULL or misaligned pointers (slots 8, others 4
+ * bytes), and any two of the arrays over each other.
+ */
+int ns_paged_reserve(const int* add, int* lens, int* table, long long table_stride, int width, int* free_pages,
+                     long long capacity, int* n_free, int* q_start, long long* slots, int rows, int* shorts,
+                     int B, int page_size, void* stream);
+
+/*
+ * Bytes of workspace ns_beam_select uses for these sizes, 0 for sizes it rejects. Launches that may overlap in time need
+ * workspaces of their own.
+ */
+size_t ns_beam_select_workspace(int R, int beams, int V, int n);
+
+/*
+ * The n best continuations of each of R requests with `beams` beams. logits: R * beams rows (request-major) row_stride apart of V
+ * values (bf16, or fp32 with fp32 != 0); scores [R][beams], what a beam has so far. With l the logits
+ *   c[i][v] = scores[i] + l[i][v] - log(sum over v of exp(l[i][v]))
+ * out_scores, out_tokens, out_parents [R][n] are the n largest c with their v and i, falling; within a beam in the order of
+ * the logits, equal ones by rising v, between beams in that of c in 64 bits, equal ones by rising i. The exponentials are 32
+ * bits wide, which moves a beam's c as a whole by 2^-22 or so: beams whose c lie closer may come in either order. NaN logits and scores count as -inf, +inf as the largest fp32; a score of
+ * -inf is a beam that does not count, a logit of -inf is never taken. Where fewer than n are left: -inf, -1, -1.
+ * -2 for sizes <= 0, beams or n above 64, R * beams > 65535, V > 2^20, row_stride < V, NULL or misaligned pointers (logits 2
+ * or 4 bytes, work 16, others 4), work_bytes too small, outputs and the workspace over an input or each other.
+ */
+int ns_beam_select(const void* logits, int fp32, long long row_stride, const float* scores, float* out_scores,
+                   int* out_tokens, int* out_parents, void* work, size_t work_bytes, int R, int beams, int V, int n,
+                   void* stream);
+
+/*
+ * The pages of R requests' beams after a selection: beam i of a request goes on from beam parents[i] (rows parent_stride apart;
+ * one that is not 0 .. beams - 1 counts as i). table and lens are those of the R * beams sequences, request-major; the
+ * beams of a request have the same length n. out [R * beams][width] receives, per beam, with w = n / page_size whole
+ * pages: entries 0 .. w - 1 of its parent; where n % page_size is not 0 entry w of a page of its own, which holds
+ * the parent's rows; behind that the beam's own entries. Of a parent's children the parent itself, or else the first one,
+ * keeps the parent's page w; the k-th of the others gets page w of the k-th beam that no one goes on from, into which the
+ * n % page_size rows of every layer and head are copied in both pools, and the scales of their blocks (k_scales and
+ * v_scales NULL: a cache without). The last, partly filled pages of a request must be the beams' own. table is not changed,
+ * so a repeated call gives the same; entries outside [0, n_pages) are moved and not copied from or to.
+ * Pools: + layer * layer_stride + page * page_stride + head * head_stride + row * row_bytes (bytes, multiples of 16); scales
+ * alike, one byte per 16 rows. -2 for sizes <= 0, beams > 64, R * beams >= 2^24, page_size % 16, width * page_size
+ * >= 2^30, page_size * row_bytes * Hk >= 2^31, strides by which layers, pages and heads overlap, NULL or misaligned pointers
+ * (pools 16, int 4 bytes), pages over each other (as in ns_paged_append_fp8), out or an input within the pools' spans, out over an input.
+ */
+int ns_paged_reorder(const int* parents, long long parent_stride, const int* table, long long table_stride, int width,
+                     const int* lens, int* out, void* k_pool, void* v_pool, long long layer_stride,
+                     long long page_stride, long long head_stride, void* k_scales, void* v_scales,
+                     long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride, int layers,
+                     int n_pages, int page_size, int row_bytes, int R, int beams, int Hk, void* stream);
+
+/*
  * Bytes of workspace ns_sample uses for these sizes, 0 for none or for sizes it rejects. Launches that
  * may overlap in time need workspaces of their own.
  */

@@ -1,0 +1,224 @@
+// Pages of the beams that go on (gfx950; contract in batch_ops.h): table rows of the parents, and copies of the last,
+// partly filled page where a beam goes on more than once. The reference keeps one sequence and has no counterpart.
+//
+// Whole pages are never written again, so beams share them by their tables alone. The last page has to be a beam's own:
+// of a parent's children one keeps it, and the others take over the last pages of beams that ended, of which there are as
+// many. Sources are thus pages that stay and destinations pages that nobody reads: all copies and tables go in one launch, and
+// a second run of the call gives the same. Bound by HBM for many layers (each copied row read once and written once),
+// by the latency of parents -> page ids -> rows for few.
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "batch_ops.h"
+#include "paged_common.h"
+
+namespace ns {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMostBeams = 64;
+
+struct ReorderArgs {
+  const int *parents, *table, *lens;
+  long long parent_stride, table_stride;
+  int* out;  // [rows][width]
+  uint8_t *pool[2], *scale[2];  // K and V; scales null: a cache without
+  long long layer, page, head, s_layer, s_page, s_head;  // strides in bytes
+  int beams, width, page_size, row_bytes, n_pages, Hk, layers, table_grid;
+};
+
+// Beam i's parent and the beam whose last page it gets, of the request whose lanes hold the parents (lane = beam).
+// Every lane of the wave takes part.
+struct Way {
+  int parent, place;
+};
+__device__ __forceinline__ Way way_of(const ReorderArgs& a, long long request, int beam) {
+  const int lane = __lane_id();
+  int p = -1;
+  if (lane < a.beams) {
+    p = a.parents[request * a.parent_stride + lane];
+    if ((unsigned)p >= (unsigned)a.beams) p = lane;  // no parent: goes on as it is
+  }
+  // the child that keeps the parent's page: the parent itself, or else the first one
+  const unsigned long long stays = __ballot(p == lane);
+  unsigned long long goes_on = 0, keeps = 0;
+  for (int q = 0; q < a.beams; ++q) {
+    const unsigned long long children = __ballot(p == q);
+    if (!children) continue;
+    goes_on |= 1ull << q;
+    keeps |= stays >> q & 1 ? 1ull << q : children & -children;
+  }
+  const unsigned long long all = a.beams == 64 ? ~0ull : (1ull << a.beams) - 1;
+  unsigned long long ended = all & ~goes_on, copied = all & ~keeps;
+  Way w;
+  w.parent = __builtin_amdgcn_readlane(p, beam);
+  w.place = w.parent;
+  if (copied >> beam & 1) {  // the k-th copy goes to the k-th ended beam's page
+    for (int k = __popcll(copied & ((1ull << beam) - 1)); k > 0; --k) ended &= ended - 1;
+    w.place = __builtin_ctzll(ended);
+  }
+  return w;
+}
+
+__global__ void __launch_bounds__(kThreads) reorder_kernel(ReorderArgs a) {
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < a.table_grid) {  // a workgroup per table row
+    const long long row = blockIdx.x, request = row / a.beams;
+    const int beam = (int)(row % a.beams);
+    const Way w = way_of(a, request, beam);
+    const long long from = request * a.beams + w.parent;
+    const int len = min(max(a.lens[from], 0), a.width * a.page_size), whole = len / a.page_size;
+    for (int j = tid; j < a.width; j += kThreads) {
+      const long long src = j < whole ? from : j == whole && len % a.page_size ? request * a.beams + w.place : row;
+      a.out[row * a.width + j] = a.table[src * a.table_stride + j];
+    }
+    return;
+  }
+  // a workgroup per beam, layer and one of K and V: the rows of all heads
+  long long id = blockIdx.x - a.table_grid;
+  const int kv = (int)(id & 1);
+  id >>= 1;
+  const int layer = (int)(id % a.layers);
+  const long long row = id / a.layers, request = row / a.beams;
+  const Way w = way_of(a, request, (int)(row % a.beams));
+  if (w.place == w.parent) return;
+  const long long from = request * a.beams + w.parent;
+  const int len = min(max(a.lens[from], 0), a.width * a.page_size), part = len % a.page_size;
+  if (part == 0) return;
+  const int at = len / a.page_size;
+  const int src = a.table[from * a.table_stride + at], dst = a.table[(request * a.beams + w.place) * a.table_stride + at];
+  if ((unsigned)src >= (unsigned)a.n_pages || (unsigned)dst >= (unsigned)a.n_pages) return;
+  const uint8_t* s = a.pool[kv] + layer * a.layer + src * a.page;
+  uint8_t* d = a.pool[kv] + layer * a.layer + dst * a.page;
+  const int chunks = part * a.row_bytes / 16, total = chunks * a.Hk;  // of 16 bytes
+  constexpr int kAtOnce = 4;
+  for (int i0 = tid; i0 < total; i0 += kAtOnce * kThreads) {
+    uint4 v[kAtOnce];
+    long long off[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int i = min(i0 + u * kThreads, total - 1);
+      off[u] = i / chunks * a.head + i % chunks * 16ll;
+      v[u] = *reinterpret_cast<const uint4*>(s + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      if (i0 + u * kThreads < total) *reinterpret_cast<uint4*>(d + off[u]) = v[u];
+  }
+  if (!a.scale[kv]) return;
+  const int blocks = (part + kScaleRows - 1) / kScaleRows;
+  const uint8_t* ss = a.scale[kv] + layer * a.s_layer + src * a.s_page;
+  uint8_t* sd = a.scale[kv] + layer * a.s_layer + dst * a.s_page;
+  for (int i = tid; i < blocks * a.Hk; i += kThreads) {
+    const long long off = i / blocks * a.s_head + i % blocks;
+    sd[off] = ss[off];
+  }
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Pages, heads and layers of pieces of `piece` bytes: whether no two share a byte, whichever of the dimensions is the
+// outer one (each stride spans what the smaller ones span together).
+bool nested(long long piece, long long layers, long long layer, long long pages, long long page, long long heads,
+            long long head) {
+  std::pair<long long, long long> dims[] = {{layer, layers}, {page, pages}, {head, heads}};
+  std::sort(std::begin(dims), std::end(dims));
+  __int128 span = piece;
+  for (const auto& d : dims) {
+    if (d.second == 1) continue;
+    if (d.first < span) return false;
+    span += (__int128)d.first * (d.second - 1);
+  }
+  return true;
+}
+
+}  // namespace
+}  // namespace ns
+
+extern "C" int ns_paged_reorder(const int* parents, long long parent_stride, const int* table, long long table_stride,
+                                int width, const int* lens, int* out, void* k_pool, void* v_pool, long long layer_stride,
+                                long long page_stride, long long head_stride, void* k_scales, void* v_scales,
+                                long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride,
+                                int layers, int n_pages, int page_size, int row_bytes, int R, int beams, int Hk,
+                                void* stream) {
+  if (R <= 0 || beams <= 0 || beams > ns::kMostBeams || (long long)R * beams >= (1 << 24)) return -2;
+  if (width <= 0 || page_size <= 0 || page_size % 16 || (long long)width * page_size >= (1ll << 30)) return -2;
+  if (layers <= 0 || n_pages <= 0 || Hk <= 0 || row_bytes <= 0 || row_bytes % 16) return -2;
+  if ((long long)page_size * row_bytes * Hk >= (1ll << 31)) return -2;
+  if (parent_stride < beams || parent_stride >> 46 || table_stride < width || table_stride >> 46) return -2;
+  if (!parents || !table || !lens || !out || !k_pool || !v_pool || !k_scales != !v_scales) return -2;
+  for (const void* p : {(const void*)parents, (const void*)table, (const void*)lens, (const void*)out})
+    if (!ns::aligned(p, 4)) return -2;
+  if (!ns::aligned(k_pool, 16) || !ns::aligned(v_pool, 16)) return -2;
+  for (const long long s : {layer_stride, page_stride, head_stride})
+    if (s < 0 || s % 16 || s >> 46) return -2;
+  for (const long long s : {scale_layer_stride, scale_page_stride, scale_head_stride})
+    if (s < 0 || s >> 46) return -2;
+  const long long piece = (long long)page_size * row_bytes, marks = page_size / ns::kScaleRows, rows = (long long)R * beams;
+  if (!ns::nested(piece, layers, layer_stride, n_pages, page_stride, Hk, head_stride)) return -2;
+  if (k_scales && !ns::nested(marks, layers, scale_layer_stride, n_pages, scale_page_stride, Hk, scale_head_stride))
+    return -2;
+  if (rows * (2ll * layers + 1) >= (1ll << 31)) return -2;
+  const ns::Bytes y = ns::bytes_of(out, 4 * (size_t)rows * width), z[] = {ns::rows_of(parents, R, parent_stride, beams, 4),
+                                                                        ns::rows_of(table, rows, table_stride, width, 4),
+                                                                        ns::bytes_of(lens, 4 * (size_t)rows)};
+  for (const ns::Bytes& r : z)
+    if (!ns::apart(y, r)) return -2;
+  // what lies between the pools' pages counts as theirs here
+  auto span = [&](const void* p, long long x, long long layer, long long page, long long head) {
+    return ns::bytes_of(p, (layers - 1) * layer + (n_pages - 1) * page + (Hk - 1) * head + x);
+  };
+  const ns::Bytes pools[] = {span(k_pool, piece, layer_stride, page_stride, head_stride),
+                             span(v_pool, piece, layer_stride, page_stride, head_stride),
+                             span(k_scales, marks, scale_layer_stride, scale_page_stride, scale_head_stride),
+                             span(v_scales, marks, scale_layer_stride, scale_page_stride, scale_head_stride)};
+  for (const ns::Bytes& p : pools)
+    if (!ns::apart(p, y) || !ns::apart(p, z[0]) || !ns::apart(p, z[1]) || !ns::apart(p, z[2])) return -2;
+  // but K's, V's and the scales' pages may lie between each other's
+  auto layer_of = [](const void* p, long long l, long long stride) {
+    return reinterpret_cast<uint16_t*>(reinterpret_cast<uintptr_t>(p) + l * stride);
+  };
+  const ns::Pools f{nullptr, nullptr, page_stride, head_stride, n_pages, 1},
+      g{nullptr, nullptr, scale_page_stride, scale_head_stride, n_pages, 1};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j) {
+      if (ns::apart(pools[i], pools[j])) continue;
+      for (int l = 0; l < layers; ++l)
+        for (int m = 0; m < layers; ++m) {
+          const void* all[] = {k_pool, v_pool, k_scales, v_scales};
+          if (!ns::sets_apart(layer_of(all[i], l, i < 2 ? layer_stride : scale_layer_stride), i < 2 ? f : g,
+                              i < 2 ? piece : marks, layer_of(all[j], m, j < 2 ? layer_stride : scale_layer_stride),
+                              j < 2 ? f : g, j < 2 ? piece : marks, Hk))
+            return -2;
+        }
+    }
+  ns::ReorderArgs a{};
+  a.parents = parents;
+  a.table = table;
+  a.lens = lens;
+  a.parent_stride = parent_stride;
+  a.table_stride = table_stride;
+  a.out = out;
+  a.pool[0] = static_cast<uint8_t*>(k_pool);
+  a.pool[1] = static_cast<uint8_t*>(v_pool);
+  a.scale[0] = static_cast<uint8_t*>(k_scales);
+  a.scale[1] = static_cast<uint8_t*>(v_scales);
+  a.layer = layer_stride;
+  a.page = page_stride;
+  a.head = head_stride;
+  a.s_layer = scale_layer_stride;
+  a.s_page = scale_page_stride;
+  a.s_head = scale_head_stride;
+  a.beams = beams;
+  a.width = width;
+  a.page_size = page_size;
+  a.row_bytes = row_bytes;
+  a.n_pages = n_pages;
+  a.Hk = Hk;
+  a.layers = layers;
+  a.table_grid = (int)rows;
+  const auto st = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(ns::reorder_kernel, dim3((unsigned)(rows * (2ll * layers + 1))), dim3(ns::kThreads), 0, st, a);
+  return static_cast<int>(hipGetLastError());
+}

@@ -52,7 +52,8 @@ SIGNATURES["ns_probe_linear_loop"] = [_VP] * 7 + [_I32, _I32, _VP]
 RESTYPES = {"ns_decode_attention_workspace": _SZ, "ns_w4_gptq_workspace": _SZ,
             "ns_w4_linear_workspace": _SZ, "ns_prompt_attention_workspace": _SZ,
             "ns_w4_linear_swiglu_rows_workspace": _SZ, "ns_paged_attention_workspace": _SZ,
-            "ns_sample_workspace": _SZ, "ns_paged_attention_fp8_workspace": _SZ}
+            "ns_sample_workspace": _SZ, "ns_paged_attention_fp8_workspace": _SZ,
+            "ns_beam_select_workspace": _SZ}
 # Entry points of this package's own callers (csrc/internal_ops.h, csrc/batch_ops.h), not part of the
 # public ABI.
 INTERNAL_SIGNATURES = {
@@ -74,6 +75,10 @@ INTERNAL_SIGNATURES = {
     "ns_paged_attention_fp8_workspace": [_I32] * 8,
     "ns_paged_attention_fp8": [_VP, _I64, _VP, _VP, _I64, _I64, _VP, _VP, _I64, _I64, _I32, _I32, _VP, _I64, _I32,
                                _VP, _VP, _VP, _VP, _SZ] + [_I32] * 8 + [_F32, _VP],
+    "ns_paged_reserve": [_VP, _VP, _VP, _I64, _I32, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _I32, _I32, _VP],
+    "ns_beam_select_workspace": [_I32] * 4,
+    "ns_beam_select": [_VP, _I32, _I64] + [_VP] * 5 + [_SZ] + [_I32] * 4 + [_VP],
+    "ns_paged_reorder": [_VP, _I64, _VP, _I64, _I32] + [_VP] * 4 + [_I64] * 3 + [_VP] * 2 + [_I64] * 3 + [_I32] * 7 + [_VP],
     "ns_sample_workspace": [_I32] * 3,
     "ns_sample": [_VP, _I32, _I64, _VP, _VP, _F32, _VP, _I32, _VP, _F32, _VP, _F32, _VP, _VP, _SZ, _I32,
                   _I32, _VP],
@@ -885,6 +890,179 @@ class Kernels:
             Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
         self._check(rc, "ns_paged_attention_fp8")
         return out
+
+    def paged_reserve(self, new, lens, pages, free, n_free, page_size, rows=None, out=None):
+        """Room for a step's tokens, on the device: sequence b gets new[b] more positions (int32 [B]; below 0: gives
+        back as many). lens [B] and pages [B, width] (int32, as paged_append reads them), the stack of free pages free
+        [capacity] and its height n_free [1] are changed in place: pages of sequences that shrink are pushed, those that
+        growing ones need are popped, in the order of the sequences. Returns (q_start [B + 1], slots, short [1]):
+        the first token row of each sequence, and with ``rows`` an int64 [rows] map of every new token to page * page_size +
+        its row there (an index into a pool's positions; -1 for rows behind the last sequence's). ``out``: the three of
+        them (slots None without ``rows``), for a captured step.
+
+        The call goes through as a whole or changes nothing: then q_start is 0 throughout, so that the operators on
+        the batch have no rows to work on, and short[0] is the number of pages that were missing, or -1 where a sequence
+        would pass its table row, more tokens are new than rows, or the stack would pass its capacity; else 0. A later
+        call that gives back what this one took restores the stack as it was. Pages that another sequence still
+        reads (a shared prefix, beams) must not be given back. The reference keeps one sequence in one cache
+        (qwen.py:103-111)."""
+        here = _device_of(new, "new", torch.int32)
+        for name, t in (("lens", lens), ("pages", pages), ("free", free), ("n_free", n_free)):
+            _require_here(t, name, torch.int32, here)
+        if new.dim() != 1 or not new.is_contiguous():
+            raise ValueError("new must be a contiguous [B] tensor")
+        B = new.shape[0]
+        if tuple(lens.shape) != (B,) or not lens.is_contiguous():
+            raise ValueError(f"lens must be a contiguous [{B}] tensor")
+        if pages.dim() != 2 or pages.shape[0] != B or pages.stride(1) != 1:
+            raise ValueError("pages must be [B, width] with contiguous rows")
+        if free.dim() != 1 or not free.is_contiguous() or n_free.numel() != 1:
+            raise ValueError("free must be a contiguous [capacity] tensor and n_free hold one value")
+        if rows is not None and rows < 0:
+            raise ValueError("rows must not be negative")
+        if out is None:
+            out = (new.new_empty(B + 1), None if rows is None else new.new_empty(rows, dtype=torch.int64), new.new_empty(1))
+        q_start, slots, short = out
+        _require_here(q_start, "q_start", torch.int32, here)
+        _require_here(short, "short", torch.int32, here)
+        if tuple(q_start.shape) != (B + 1,) or not q_start.is_contiguous() or short.numel() != 1:
+            raise ValueError(f"q_start must be a contiguous [{B + 1}] tensor and short hold one value")
+        if rows is not None:
+            _require_here(slots, "slots", torch.int64, here)
+            if tuple(slots.shape) != (rows,) or not slots.is_contiguous():
+                raise ValueError(f"slots must be a contiguous [{rows}] tensor")
+        elif slots is not None:
+            raise ValueError("slots without rows")
+        if B == 0:
+            raise ValueError("the batch has no sequence")
+        width = pages.shape[1]
+        rc = self.lib.ns_paged_reserve(
+            new.data_ptr(), lens.data_ptr(), pages.data_ptr(), pages.stride(0) if B > 1 else width, width,
+            free.data_ptr(), free.shape[0], n_free.data_ptr(), q_start.data_ptr(),
+            None if slots is None else slots.data_ptr(), -1 if rows is None else rows, short.data_ptr(), B, page_size,
+            _raw_stream(here))
+        self._check(rc, "ns_paged_reserve")
+        return out
+
+    def paged_reorder(self, parents, pages, lens, k_pages, v_pages, k_scales=None, v_scales=None, out=None):
+        """The pages of beam search's sequences after a selection: beam i of request r goes on from beam parents[r, i]
+        (int32 [R, beams], rows may be strided, e.g. beam_select's first columns; -1: stays). pages [R * beams, width] and
+        lens [R * beams] are the batch's, request by request; the beams of a request have one length. Returns the new
+        pages [R * beams, width] (contiguous, not pages itself).
+
+        Whole pages are shared by the tables. Of the last, partly filled pages, which have to be the beams' own, one child
+        keeps its parent's; for the others its rows are copied, in every layer, to the pages of beams that ended. So
+        neither pages nor copies are needed beyond the beams' own, and entries behind the last position stay each
+        beam's. k_pages, v_pages: bf16 [n_pages, Hk, page_size, D] or all layers' [layers, n_pages, Hk, page_size,
+        D] (strides as in paged_append), or float8_e4m3fn with k_scales, v_scales as in paged_append_fp8. A repeated call
+        with the same arguments gives the same. The reference serves one sequence (qwen.py:166-177)."""
+        here = _device_of(parents, "parents", torch.int32)
+        _require_here(pages, "pages", torch.int32, here)
+        _require_here(lens, "lens", torch.int32, here)
+        fp8 = k_scales is not None
+        dtype = torch.float8_e4m3fn if fp8 else torch.bfloat16
+        _require_here(k_pages, "k_pages", dtype, here)
+        _require_here(v_pages, "v_pages", dtype, here)
+        if parents.dim() != 2 or (parents.shape[1] > 1 and parents.stride(1) != 1):
+            raise ValueError("parents must be [R, beams] with contiguous rows")
+        R, beams = parents.shape
+        rows = R * beams
+        if pages.dim() != 2 or pages.shape[0] != rows or pages.stride(1) != 1:
+            raise ValueError(f"pages must be [{rows}, width] with contiguous rows")
+        if tuple(lens.shape) != (rows,) or not lens.is_contiguous():
+            raise ValueError(f"lens must be a contiguous [{rows}] tensor")
+        shape, strides = tuple(k_pages.shape), k_pages.stride()
+        if len(shape) not in (4, 5) or strides[-1] != 1 or strides[-2] != shape[-1]:
+            raise ValueError("k_pages must be [n_pages, Hk, page_size, D], or that for all layers, with contiguous heads")
+        if v_pages.shape != k_pages.shape or v_pages.stride() != strides:
+            raise ValueError("k_pages and v_pages must be alike")
+        if len(shape) == 4:
+            shape, strides = (1, *shape), (0, *strides)
+        layers, n_pages, Hk, page_size, D = shape
+        size = 1 if fp8 else 2
+        by = tuple(size * s if n > 1 else 0 for s, n in zip(strides[:3], shape[:3]))
+        marks = (None, None, 0, 0, 0)
+        if fp8:
+            _require_here(k_scales, "k_scales", torch.float8_e8m0fnu, here)
+            _require_here(v_scales, "v_scales", torch.float8_e8m0fnu, here)
+            strides = k_scales.stride()
+            if tuple(k_scales.shape) != (*k_pages.shape[:-2], page_size // 16) or (page_size > 16 and strides[-1] != 1):
+                raise ValueError("k_scales must be [n_pages, Hk, page_size / 16] (for all layers, as the pages) with "
+                                 "contiguous heads")
+            if v_scales.shape != k_scales.shape or v_scales.stride() != strides:
+                raise ValueError("k_scales and v_scales must be alike")
+            if len(strides) == 3:
+                strides = (0, *strides)
+            marks = (k_scales.data_ptr(), v_scales.data_ptr(),
+                     *(s if n > 1 else 0 for s, n in zip(strides[:3], shape[:3])))
+        elif v_scales is not None:
+            raise ValueError("v_scales without k_scales")
+        width = pages.shape[1]
+        if out is None:
+            out = pages.new_empty((rows, width))
+        else:
+            _require_here(out, "out", torch.int32, here)
+            if tuple(out.shape) != (rows, width) or not out.is_contiguous():
+                raise ValueError(f"out must be a contiguous [{rows}, {width}] tensor")
+        if rows == 0:
+            return out
+        rc = self.lib.ns_paged_reorder(
+            parents.data_ptr(), parents.stride(0) if R > 1 else beams, pages.data_ptr(),
+            pages.stride(0) if rows > 1 else width, width, lens.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), *by, *marks, layers, n_pages, page_size, size * D, R, beams, Hk, _raw_stream(here))
+        self._check(rc, "ns_paged_reorder")
+        return out
+
+    # ------------------------------------------------------------------ beam search
+    def beam_select_workspace(self, R, beams, vocab, n, dtype=torch.bfloat16, device=None):
+        """A uint8 device tensor of the workspace beam_select uses for these sizes. Launches that may overlap in time need
+        workspaces of their own."""
+        size = int(self.lib.ns_beam_select_workspace(R, beams, vocab, n))
+        return torch.empty(size, dtype=torch.uint8, device=device or "cuda") if size else None
+
+    def beam_select(self, logits, scores, n, work=None, out=None):
+        """The n best continuations (at most 64) of R requests with up to 64 beams each: logits [R * beams, vocab] (bf16 or
+        float32, request by request, rows may be strided, vocab at most 2^20), scores [R, beams] float32, the beams' sums of log
+        probabilities so far. Returns (scores float32, tokens int32, parents int32), each [R, n]: the largest scores[r, i] +
+        log softmax(logits[r, i])[v], falling, with their v and i; equal ones by beam, then by token. A beam whose score is -inf
+        does not count (after the prompt: all but one). NaN counts as -inf and is never taken, +inf as the largest float32;
+        where fewer than n are left, -inf, -1 and -1. Scores are compared in float64; the sum below a logarithm is good to
+        some 2^-22, and beams whose scores lie closer than that may come in either order.
+        ``work``: from beam_select_workspace, allocated here when it is not given; ``out``: the three results. The
+        reference decodes one sequence greedily (qwen.py:166-177)."""
+        if not isinstance(logits, torch.Tensor):
+            raise TypeError("logits must be a torch.Tensor")
+        fp32 = logits.dtype is torch.float32
+        here = _device_of(logits, "logits", torch.float32 if fp32 else torch.bfloat16)
+        _require_here(scores, "scores", torch.float32, here)
+        if scores.dim() != 2 or not scores.is_contiguous():
+            raise ValueError("scores must be a contiguous [R, beams] tensor")
+        R, beams = scores.shape
+        if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] != R * beams:
+            raise ValueError(f"logits must be [{R * beams}, vocab] with contiguous rows")
+        V = logits.shape[1]
+        if out is None:
+            out = (scores.new_empty((R, n)), scores.new_empty((R, n), dtype=torch.int32),
+                   scores.new_empty((R, n), dtype=torch.int32))
+        else:
+            for t, name, dtype in zip(out, ("scores", "tokens", "parents"), (torch.float32, torch.int32, torch.int32)):
+                _require_here(t, "out " + name, dtype, here)
+                if tuple(t.shape) != (R, n) or not t.is_contiguous():
+                    raise ValueError(f"out {name} must be a contiguous [{R}, {n}] tensor")
+        if R == 0:
+            return out
+        if work is None:
+            work = self.beam_select_workspace(R, beams, V, n, logits.dtype, device=logits.device)
+        else:
+            _require_here(work, "work", torch.uint8, here)
+            if not work.is_contiguous():
+                raise _strided_work()
+        rc = self.lib.ns_beam_select(logits.data_ptr(), int(fp32), logits.stride(0) if R * beams > 1 else V,
+                                     scores.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+                                     None if work is None else work.data_ptr(), 0 if work is None else work.numel(), R,
+                                     beams, V, n, _raw_stream(here))
+        self._check(rc, "ns_beam_select")
+        return tuple(out)
 
     # ------------------------------------------------------------------ the next token
     def sample_workspace(self, B, vocab, dtype=torch.bfloat16, device=None):
