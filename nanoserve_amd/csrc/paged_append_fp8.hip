@@ -26,7 +26,7 @@ struct Append8Args {
   Pools p;
   Scales f;
   int Hq, Hk;
-  int q_grid, parts;  // workgroups of the query heads; workgroups per 16 token rows
+  int kv_grid, parts;  // workgroups of the key and value heads, and how many of them per 16 token rows
 };
 
 // cos and sin of position * frequency, reduced to a fraction of a turn in fp64.
@@ -71,6 +71,38 @@ __device__ __forceinline__ uint2 codes8(const float (&x)[8], float inv) {
   return make_uint2(w[0], w[1]);
 }
 
+// Sixteen codes times a power of two, rounded again where they leave the normal range.
+__device__ __forceinline__ u32x4_t rescaled(u32x4_t v, float f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i], true);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(held448(lo[0] * f), held448(lo[1] * f), 0, false);
+    v[i] = __builtin_amdgcn_cvt_pk_fp8_f32(held448(hi[0] * f), held448(hi[1] * f), w, true);
+  }
+  return v;
+}
+
+// The largest of a group of N lanes (4 or 8, aligned; values not negative), in all of them: DPP within rows of 16.
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
+  auto from = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value,
+                                                                 0xf, 0xf, false));
+  };
+  v = fmaxf(v, from(v, std::integral_constant<int, 0xb1>{}));   // lane ^ 1
+  v = fmaxf(v, from(v, std::integral_constant<int, 0x4e>{}));   // lane ^ 2
+  if constexpr (N == 8) v = fmaxf(v, from(v, std::integral_constant<int, 0x141>{}));  // mirrored within 8
+  return v;
+}
+
+// The largest of the wave's values, none below 0.
+__device__ __forceinline__ float wave_top(float v) {
+  v = lanes_max<8>(v);
+  v = fmaxf(v, lane_xor8(v));
+  v = fmaxf(v, lane_xor16(v));
+  return fmaxf(v, lane_xor32(v));
+}
+
 // The codes of one of K and V for `count` new rows of a block behind `held` older ones. x, y: of the rows
 // kRows * p + lane / kLanes.
 template <int D, int kPasses>
@@ -87,7 +119,7 @@ __device__ __forceinline__ void store_block(uint8_t* block, uint8_t* scale, int 
       const float u = fabsf(x[p][e]), v = fabsf(y[p][e]);
       if (kRows * p + r < count) top = fmaxf(top, fmaxf(u <= FLT_MAX ? u : 0.f, v <= FLT_MAX ? v : 0.f));
     }
-  int e = scale_exponent(wave_max(top));
+  int e = scale_exponent(wave_top(top));
   if (held > 0) e = max(e, min(max(old - 127, kLeastScale), kMostScale));
   e = __builtin_amdgcn_readfirstlane(e);
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -109,14 +141,7 @@ __device__ __forceinline__ void store_block(uint8_t* block, uint8_t* scale, int 
     const int row = kRows * p + r;
     if (row < held) {
       u32x4_t* at = reinterpret_cast<u32x4_t*>(block + row * D + 16 * c);
-      u32x4_t v = *at;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)v[i], true);
-        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(held448(lo[0] * f), held448(lo[1] * f), 0, false);
-        v[i] = __builtin_amdgcn_cvt_pk_fp8_f32(held448(hi[0] * f), held448(hi[1] * f), w, true);
-      }
-      *at = v;
+      *at = rescaled(*at, f);
     }
   }
 }
@@ -125,10 +150,10 @@ template <int D, int kHeads>
 __global__ void __launch_bounds__(256) paged_append_fp8_kernel(Append8Args a) {
   constexpr int kLanes = D / 16, kRows = kWave / kLanes, kPasses = kTile / kRows;
   const int H = a.Hq;
-  if ((int)blockIdx.x < a.q_grid) {
+  if ((int)blockIdx.x >= a.kv_grid) {
     // a thread: elements 8 c .. with their partners in up to kHeads query heads of a token
     const int nblk = (H + kHeads - 1) / kHeads;
-    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, tb = id / kLanes;
+    const long long id = (long long)(blockIdx.x - a.kv_grid) * 256 + threadIdx.x, tb = id / kLanes;
     if (tb / nblk >= a.s.T) return;
     const int c = (int)(id % kLanes), t = (int)(tb / nblk), h0 = (int)(tb % nblk) * kHeads;
     const int b = a.s.sequence(t);
@@ -159,7 +184,7 @@ __global__ void __launch_bounds__(256) paged_append_fp8_kernel(Append8Args a) {
   }
   // Blocks that begin among the workgroup's 16 token rows: those of a sequence's first new token or of a multiple of 16.
   // Every wave finds them all and takes its share of them times the kv heads.
-  const int id = blockIdx.x - a.q_grid, tile = id / a.parts;
+  const int id = blockIdx.x, tile = id / a.parts;
   const int lane = __lane_id(), wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int t = tile * kTile + (lane & 15);
   int page = -1, pos = -1, count = 0, at = 0;
@@ -180,37 +205,116 @@ __global__ void __launch_bounds__(256) paged_append_fp8_kernel(Append8Args a) {
   unsigned long long todo = __ballot(count > 0 && (unsigned)page < (unsigned)a.p.n_pages);
   for (int n = 0; todo; todo &= todo - 1) {
     const int src = __builtin_ctzll(todo);
-    for (int g = 0; g < a.Hk; ++g, ++n) {
+    for (int h = 0; h < 2 * a.Hk; ++h, ++n) {
       if (n % (4 * a.parts) != (id % a.parts) * 4 + wv) continue;
+      const bool is_k = h < a.Hk;
+      const int g = is_k ? h : h - a.Hk;
       const int rows = __builtin_amdgcn_readlane(count, src), p0 = __builtin_amdgcn_readlane(pos, src);
       const int in = __builtin_amdgcn_readlane(at, src), held = in % kScaleRows;
       const size_t pg = (size_t)__builtin_amdgcn_readlane(page, src);
       const size_t off = pg * a.p.page_stride + (size_t)g * a.p.head_stride + (size_t)(in - held) * D;
       const size_t soff = pg * a.f.page_stride + (size_t)g * a.f.head_stride + in / kScaleRows;
       const int c = lane % kLanes, r = lane / kLanes;
-      float x[kPasses][8], y[kPasses][8], u[kPasses][8], w[kPasses][8];
+      float x[kPasses][8], y[kPasses][8];
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {  // (rows past the last repeat it, unstored)
         const uint16_t* row = a.qkv + (size_t)(tile * kTile + src + min(kRows * p + r, rows - 1)) * a.qkv_stride;
-        load_pair<D>(a, row, a.Hq + g, c, x[p], y[p]);
-        load_pair<D>(a, row, a.Hq + a.Hk + g, c, u[p], w[p]);
+        load_pair<D>(a, row, a.Hq + h, c, x[p], y[p]);
       }
+      if (is_k) {
 #pragma unroll
-      for (int p = 0; p < kPasses; ++p) {
-        if (kRows * p >= rows) break;
+        for (int p = 0; p < kPasses; ++p) {
+          if (kRows * p >= rows) break;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float sn, cs;
-          turn(p0 + kRows * p + r, a.inv_freq[8 * c + e], sn, cs);
-          const float k = x[p][e], v = y[p][e];
-          x[p][e] = k * cs - v * sn;
-          y[p][e] = v * cs + k * sn;
+          for (int e = 0; e < 8; ++e) {
+            float sn, cs;
+            turn(p0 + kRows * p + r, a.inv_freq[8 * c + e], sn, cs);
+            const float k = x[p][e], v = y[p][e];
+            x[p][e] = k * cs - v * sn;
+            y[p][e] = v * cs + k * sn;
+          }
         }
       }
-      store_block<D, kPasses>(reinterpret_cast<uint8_t*>(a.p.k) + off, a.f.k + soff, held, rows, x, y);
-      store_block<D, kPasses>(reinterpret_cast<uint8_t*>(a.p.v) + off, a.f.v + soff, held, rows, u, w);
+      store_block<D, kPasses>(reinterpret_cast<uint8_t*>(is_k ? a.p.k : a.p.v) + off, (is_k ? a.f.k : a.f.v) + soff, held,
+                              rows, x, y);
     }
   }
+}
+
+// One new token per sequence: a thread takes elements 8 c .. with their partners in one head of a token, D / 16 lanes a
+// head, so the values' loads need not wait for the length and the page. Where a block's exponent rises, those lanes
+// also rewrite its older rows.
+template <int D>
+__global__ void __launch_bounds__(256) paged_append_fp8_one_kernel(Append8Args a) {
+  constexpr int kLanes = D / 16;
+  const int H = a.Hq + 2 * a.Hk;
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, th = id / kLanes;
+  if (th / H >= a.s.T) return;  // (whole groups of kLanes lanes)
+  const int c = (int)(id % kLanes), b = (int)(th / H), h = (int)(th % H);
+  const int pos = a.s.positions(b) - 1;
+  float x[8], y[8], frq[8];
+  load_pair<D>(a, a.qkv + (size_t)b * a.qkv_stride, h, c, x, y);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) frq[e] = a.inv_freq[8 * c + e];
+  const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hk;
+  const int g = h - a.Hq - (is_k ? 0 : a.Hk);
+  int page = -1;
+  if (!is_q && pos >= 0) page = a.s.table[(size_t)b * a.s.table_stride + pos / a.s.page_size];
+  const bool stored = (unsigned)page < (unsigned)a.p.n_pages;
+  const int at = max(pos, 0) % a.s.page_size, held = at % kScaleRows;
+  uint8_t* scale = nullptr;
+  int old = 0;
+  if (stored) {
+    scale = (is_k ? a.f.k : a.f.v) + (size_t)page * a.f.page_stride + (size_t)g * a.f.head_stride + at / kScaleRows;
+    if (held > 0) old = *scale;
+  }
+  if (h < a.Hq + a.Hk) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float sn, cs;
+      turn(pos, frq[e], sn, cs);
+      const float p = x[e], q = y[e];
+      x[e] = p * cs - q * sn;
+      y[e] = q * cs + p * sn;
+    }
+  }
+  if (is_q) {
+    uint16_t* dst = a.q_out + ((size_t)b * a.Hq + h) * D + 8 * c;
+    *reinterpret_cast<u32x4_t*>(dst) = pack8(x);
+    *reinterpret_cast<u32x4_t*>(dst + D / 2) = pack8(y);
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float u = fabsf(x[e]), v = fabsf(y[e]);
+    top = fmaxf(top, fmaxf(u <= FLT_MAX ? u : 0.f, v <= FLT_MAX ? v : 0.f));
+  }
+  top = lanes_max<kLanes>(top);
+  if (!stored) return;
+  int e = scale_exponent(top);
+  if (held > 0) e = max(e, min(max(old - 127, kLeastScale), kMostScale));
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  uint8_t* block = reinterpret_cast<uint8_t*>(is_k ? a.p.k : a.p.v) + (size_t)page * a.p.page_stride +
+                   (size_t)g * a.p.head_stride + (size_t)(at - held) * D;
+  uint8_t* dst = block + held * D + 8 * c;
+  *reinterpret_cast<uint2*>(dst) = codes8(x, inv);
+  *reinterpret_cast<uint2*>(dst + D / 2) = codes8(y, inv);
+  if (c == 0) *scale = (uint8_t)(e + 127);
+  if (held == 0 || e + 127 == old) return;
+  const float f = ldexpf(1.f, old - 127 - e);
+  u32x4_t v[kScaleRows - 1];
+#pragma unroll
+  for (int r = 0; r < kScaleRows - 1; ++r)
+    if (r < held) v[r] = *reinterpret_cast<const u32x4_t*>(block + r * D + 16 * c);
+#pragma unroll
+  for (int r = 0; r < kScaleRows - 1; ++r)
+    if (r < held) *reinterpret_cast<u32x4_t*>(block + r * D + 16 * c) = rescaled(v[r], f);
+}
+
+template <int D>
+void launch_one(const Append8Args& a, hipStream_t st) {
+  const long long threads = a.s.T * (a.Hq + 2ll * a.Hk) * (D / 16);
+  hipLaunchKernelGGL(paged_append_fp8_one_kernel<D>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a);
 }
 
 template <int D, int kHeads>
@@ -219,9 +323,9 @@ void launch(Append8Args& a, hipStream_t st) {
   const long long tiles = (a.s.T + kTile - 1) / kTile;
   // about one block and head to a wave: a tile of 16 rows begins one block or two, and one more for each sequence
   const long long blocks = std::min<long long>(kTile, 1 + (long long)kTile * a.s.B / a.s.T);
-  a.parts = (int)((blocks * a.Hk + 3) / 4);
-  a.q_grid = (int)((threads + 255) / 256);
-  hipLaunchKernelGGL((paged_append_fp8_kernel<D, kHeads>), dim3((unsigned)(a.q_grid + tiles * a.parts)), dim3(256), 0,
+  a.parts = (int)((blocks * 2 * a.Hk + 3) / 4);
+  a.kv_grid = (int)(tiles * a.parts);
+  hipLaunchKernelGGL((paged_append_fp8_kernel<D, kHeads>), dim3((unsigned)(a.kv_grid + (threads + 255) / 256)), dim3(256), 0,
                      st, a);
 }
 
@@ -274,6 +378,11 @@ extern "C" int ns_paged_append_fp8(const void* qkv, long long qkv_stride, const 
   // (both parts of the grid within 2^30 workgroups)
   if ((long long)T * Hq * (D / 16) >= (1ll << 38) || (long long)T * Hk >= (1ll << 29)) return -2;
   const auto st = static_cast<hipStream_t>(stream);
+  if (!q_start) {
+    if ((long long)T * (Hq + 2ll * Hk) * (D / 16) >= (1ll << 38)) return -2;
+    D == 64 ? ns::launch_one<64>(a, st) : ns::launch_one<128>(a, st);
+    return static_cast<int>(hipGetLastError());
+  }
   const bool small = (long long)T * Hq * (D / 16) <= ns::kSmall;
   if (D == 64)
     small ? ns::launch<64, 1>(a, st) : ns::launch<64, 4>(a, st);

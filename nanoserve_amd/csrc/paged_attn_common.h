@@ -300,16 +300,16 @@ __device__ __forceinline__ i32x8_t join(const u32x4_t& a, const u32x4_t& b) {
 
 // The scales of the 16 rows of a page and head that hold position `key`, K's in bits 0 .. 7 and V's in 8 .. 15; one for
 // what is no page. 255, no power of two and never written by an append, counts as the one below it: rows that
-// nobody sees are zeros times their scale. The value is waited for here, or the compiler would wait at every use,
-// behind the ring's loads.
+// nobody sees are zeros times their scale. `landed` waits for the value: without it the compiler would wait at every
+// use, behind the ring's loads.
 constexpr int kNoScales = 127 | 127 << 8;
+__device__ __forceinline__ void landed(int& s) { asm volatile("" : "+v"(s)); }
 __device__ __forceinline__ int group_scales(const PagedArgs& a, int id, int g, int key) {
   int s = kNoScales;
   if ((unsigned)id < (unsigned)a.p.n_pages) {
     const size_t at = (size_t)id * a.f.page_stride + (size_t)g * a.f.head_stride + key % a.s.page_size / kScaleRows;
     s = min((int)a.f.k[at], 254) | min((int)a.f.v[at], 254) << 8;
   }
-  asm volatile("" : "+v"(s));
   return s;
 }
 
@@ -551,7 +551,10 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
                               (uint64_t)(key % a.s.page_size) * D);
     }
     valid = __ballot((unsigned)id < (unsigned)a.p.n_pages);
-    if constexpr (kF8) scales = group_scales(a, id, g, key);
+    if constexpr (kF8) {
+      scales = group_scales(a, id, g, key);
+      landed(scales);
+    }
   };
   // (16-byte chunks of a row lie in the order c ^ swz(row), so that the rows of one read hit distinct banks)
   auto k_swz = [](int r) { return kF8 ? (D == 128 ? (r >> 1) & 7 : (r >> 2) & 3) : D == 128 ? r & 15 : (r >> 1) & 7; };

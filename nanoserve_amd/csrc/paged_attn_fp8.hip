@@ -106,13 +106,16 @@ __device__ __forceinline__ void one8_body(const PagedArgs& a, int item, int g, c
     bool has[2], whole;
   };
   auto issue = [&](uint16_t* ks, uint16_t* vs, int i, At& at) {
-    if (i > 0 && (i & 31) == 0) refill(i);
+    if (i > 0 && (i & 31) == 0) {
+      refill(i);
+      landed(scales);
+    }
     const int e = 2 * (i & 31);
     at.key0 = kOneRows * kb.block(j0 + wv + kOneWaves * i);
     at.whole = at.key0 >= k0 && at.key0 >= lo && at.key0 + kOneRows <= n;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      at.sc[u] = __builtin_amdgcn_readlane(scales, e + u);
+      if (i >= kStages) at.sc[u] = __builtin_amdgcn_readlane(scales, e + u);
       at.has[u] = __builtin_amdgcn_readlane(keys, e + u) >= 0;
       at.whole &= at.has[u];
     }
@@ -196,7 +199,7 @@ __device__ __forceinline__ void one8_body(const PagedArgs& a, int item, int g, c
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
-        const float p0 = exp2f(sr[u][r] - mz), p1 = exp2f(sr[u][r + 1] - mz);
+        const float p0 = __builtin_amdgcn_exp2f(sr[u][r] - mz), p1 = __builtin_amdgcn_exp2f(sr[u][r + 1] - mz);
         l += p0 + p1;  // this lane's keys; the lanes are added at the end
         const uint32_t term = pack_bf16x2_rne(p0, p1);
         ph[2 * u + r / 2] = term;
@@ -236,6 +239,11 @@ __device__ __forceinline__ void one8_body(const PagedArgs& a, int item, int g, c
     if (cnt > 2) start(S2{}, 2);
     if (cnt > 3) start(S3{}, 3);
   }
+  landed(scales);  // (of the first refill: behind the first blocks' loads)
+#pragma unroll
+  for (int k = 0; k < kStages; ++k)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) at[k].sc[u] = __builtin_amdgcn_readlane(scales, 2 * k + u);
   for (int i = 0; i < cnt; i += kStages) {
     step(S0{}, i);
     if (i + 1 < cnt) step(S1{}, i + 1);
