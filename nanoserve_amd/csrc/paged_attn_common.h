@@ -138,8 +138,9 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // Item `item` of the batch: its sequence, the number within it, and the sequence's first partial (a
-// token slot). False past the last item. Uniform over the workgroup's waves.
-template <int BLK, int ROWS>
+// token slot). False past the last item. Uniform over the workgroup's waves. kSorted: up to 64 sequences go by falling
+// length, so that what starts last is short.
+template <int BLK, int ROWS, bool kSorted = false>
 __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, Span& sp, int& within,
                                           long long& slot) {
   const int lane = __lane_id(), B = a.s.B;
@@ -152,13 +153,19 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
     tiles += (float)x.tiles;
   }
   total = wave_sum(total);
-  const int share = __builtin_amdgcn_readfirstlane((int)ceilf(total * a.per_target));
+  // Tiles of a cache in 8 bits: half as many workgroups aimed at (one per CU) once there are four tiles to five CUs, as a
+  // range then costs more in partials than it gains. us with all and half of them, on 256 CUs: 2000 tokens of 8
+  // sequences of 1000 to 4000 (476 tiles) 163, 111; 1000 tokens (220) 46.2, 41.3; 800 after 3000 (176) 88.7, 99.1; 2 x
+  // 300 after 8000 (160) 125, 210; 512 after 3000 (112) 54.5, 61.6.
+  float per_target = a.per_target;
+  if (kSorted && wave_sum(tiles) * per_target > 0.4f) per_target *= 2.f;
+  const int share = __builtin_amdgcn_readfirstlane((int)ceilf(total * per_target));
   int per = max(a.unit, (share + a.unit - 1) / a.unit * a.unit);
   // Sequences end inside a share: where that makes more items than workgroups aimed at, the last ones would
   // start when the others end. Larger shares then, a few times at most, if the items can be that few at all
   // (us without and with: 64 sequences of 1000 to 8000 positions 118.7, 110.0; 20 of 1000 to 4000 with 8 kv
   // heads 41.9, 38.5; 200 of up to 1000, whose 800 items are more anyway, 51.6, 59.0).
-  const bool fits = B <= 4 * kWave && wave_sum(tiles) * a.per_target < 0.9f;
+  const bool fits = B <= 4 * kWave && wave_sum(tiles) * per_target < 0.9f;
 #pragma unroll 1
   for (int step = 0; step < 3 && fits; ++step) {
     int items = 0;
@@ -169,11 +176,26 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
       }
       items += x.nn > 0 ? x.tiles * max(1, (x.blocks + per - 1) / per) : 0;
     }
-    const float over = (float)__builtin_amdgcn_readlane(wave_scan(items), kWave - 1) * a.per_target;
+    const float over = (float)__builtin_amdgcn_readlane(wave_scan(items), kWave - 1) * per_target;
     if (over <= 1.f) break;
     per = ((int)((float)per * fminf(over, 2.f)) / a.unit + 1) * a.unit;
   }
 
+  int from = lane;  // the lane's sequence
+  if (kSorted && B > 1 && B <= kWave) {
+    int rank = 0;
+    for (int i = 0; i < B; ++i) {
+      const int other = __builtin_amdgcn_readlane(x.blocks, i);
+      rank += (other > x.blocks) | ((other == x.blocks) & (i < lane));
+    }
+    // (lanes past the last sequence keep their place)
+    from = __builtin_amdgcn_ds_permute(4 * (lane < B ? rank : lane), lane);
+    x.n = __builtin_amdgcn_ds_bpermute(4 * from, x.n);
+    x.row0 = __builtin_amdgcn_ds_bpermute(4 * from, x.row0);
+    x.nn = __builtin_amdgcn_ds_bpermute(4 * from, x.nn);
+    x.tiles = __builtin_amdgcn_ds_bpermute(4 * from, x.tiles);
+    x.blocks = __builtin_amdgcn_ds_bpermute(4 * from, x.blocks);
+  }
   int seen = 0;
   slot = 0;
   for (int base = 0; base < B; base += kWave) {
@@ -186,7 +208,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
     const int upto = wave_scan(items), all = __builtin_amdgcn_readlane(upto, kWave - 1);
     if (item < seen + all) {
       const int src = __builtin_ctzll(__ballot(seen + upto > item));
-      b = base + src;
+      b = kSorted && B <= kWave ? __builtin_amdgcn_readlane(from, src) : base + src;
       within = item - seen - __builtin_amdgcn_readlane(upto - items, src);
       sp.n = __builtin_amdgcn_readlane(x.n, src);
       sp.row0 = __builtin_amdgcn_readlane(x.row0, src);
@@ -413,7 +435,7 @@ template <int D, bool kShared, bool kF8 = false>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
   // (kRow: a row of the cache in units of 2 bytes)
   constexpr int kRow = kF8 ? D / 2 : D, kChunks = kRow / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad,
-                kDT = D / 32, kStages = ring_stages<D>();
+                kDT = D / 32, kStages = ring_stages<D>(), kTerms = kF8 ? 1 : 2;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = a.R;
@@ -434,7 +456,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     b = longest(a);
   } else {
     int within;
-    if (!find_item<kTileKeys, kTileRows>(a, item, b, sp, within, slot)) return;
+    if (!find_item<kTileKeys, kTileRows, kF8>(a, item, b, sp, within, slot)) return;
     splits = sp.splits;
     split = within % splits;
     r0 = (sp.tiles - 1 - within / splits) * kTileRows;  // longest tiles first
@@ -713,18 +735,23 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
     const float mc = m == -INFINITY ? 0.f : m * c;
-    u32x4_t pt[2][4];  // B operands of the four 16-key steps
+    u32x4_t pt[kTerms][4];  // B operands of the four 16-key steps
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -mc));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][r + 1], c, -mc));
-        l += p0 + p1;
         const uint32_t term = pack_bf16x2_rne(p0, p1);
         pt[0][2 * u + (r >> 3)][(r & 7) >> 1] = term;
-        pt[1][2 * u + (r >> 3)][(r & 7) >> 1] = pack_bf16x2_rne(p0 - __uint_as_float(term << 16),
-                                                                p1 - __uint_as_float(term & 0xffff0000u));
+        if constexpr (kTerms == 1) {  // the sum of what enters the product
+          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, term), __builtin_bit_cast(bf16x2_t, 0x3f803f80u),
+                                              l, false);
+        } else {
+          l += p0 + p1;
+          pt[1][2 * u + (r >> 3)][(r & 7) >> 1] = pack_bf16x2_rne(p0 - __uint_as_float(term << 16),
+                                                                  p1 - __uint_as_float(term & 0xffff0000u));
+        }
       }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -742,7 +769,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
         vf[d] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v0[0], v0[1], v1[0], v1[1]});
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < kTerms; ++i)
 #pragma unroll
         for (int d = 0; d < kDT; ++d)
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d], __builtin_bit_cast(bf16x8_t, pt[i][u]), o[d], 0, 0, 0);
@@ -944,7 +971,8 @@ inline bool sizes_ok(int T, int B, int Hq, int Hk, int D, int max_len, int share
 }
 
 // one_rows: cache rows per block of the one-token kernel.
-inline Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, int shared, int one_rows) {
+inline Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool ragged, int shared, int one_rows,
+                      bool fp8 = false) {
   int cus = 256;  // (a failed query leaves MI355X's count; the launch reports the error)
   if (cached_cu_count(&cus) != hipSuccess || cus <= 0) cus = 256;
   Plan p{};
@@ -959,7 +987,7 @@ inline Plan make_plan(int T, int B, int Hq, int Hk, int D, int max_len, bool rag
   p.unit = 4;
   // As many workgroups as run at once; tiles: one and a half per CU, since a range of few blocks costs a partial of
   // 128 rows (us with one, one and a half, two: 1000 tokens 42.3, 42.9, 49.5; 512 after 3000 68.1, 67.1, 59.8).
-  p.target = p.one ? 2 * cus : 3 * cus / 2;
+  p.target = p.one || fp8 ? 2 * cus : 3 * cus / 2;
   if (shared > 0) {
     const long long st = ((long long)T * R + kTileRows - 1) / kTileRows;
     const int blocks = (shared + kTileKeys - 1) / kTileKeys;
@@ -1018,7 +1046,7 @@ inline bool plan_call(PagedArgs& a, Plan& p, void* work, size_t work_bytes, int 
   if (window < 0 || sinks < 0 || !(scale > 0.f) || !(scale < INFINITY)) return false;
   if (!a.q || !a.out || !aligned(a.q, 16) || !aligned(a.out, 16)) return false;
   if (a.q_stride % 8 || a.q_stride < (long long)Hq * D) return false;
-  p = make_plan(T, B, Hq, Hk, D, max_len, a.s.q_start != nullptr, shared, one_rows);
+  p = make_plan(T, B, Hq, Hk, D, max_len, a.s.q_start != nullptr, shared, one_rows, a.p.size == 1);
   if ((p.items + p.sh_items) * Hk >= (1ll << 31) || p.cap >= (1ll << 31)) return false;
   if (p.bytes > 0) {
     if (!work || !aligned(work, 16) || work_bytes < p.bytes) return false;

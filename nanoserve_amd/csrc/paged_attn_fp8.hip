@@ -5,8 +5,11 @@
 //  * Scores: the query's 8 significant bits are exactly two e4m3 terms, so q . k runs on the 8-bit matrix
 //    instructions with the codes as they lie in the cache, at the price of one product in bf16.
 //  * Values: a code times its scale is a bf16 value without rounding (v_cvt_scalef32_pk_bf16_fp8, two per
-//    instruction), and the second product is the bf16 cache's, with probabilities in two bf16 terms.
-// So the result is that of the bf16 kernels over a cache that holds the same values.
+//    instruction), and the second product is the bf16 cache's.
+//  * Probabilities of single tokens, which are bound by HBM, are two bf16 terms, as over the bf16 cache. Tiles are bound by
+//    products and softmax in turn and take one (16 bits of weight for values that a 4-bit significand stands for cost
+//    a third of the products): prompts of 5 sequences of 2000 to 8000 684 -> 537 us, at a 2-norm error against 64 bits of
+//    0.0019 where two terms have 0.0017, the rounding of the result. Their sum is that of the rounded ones.
 #include "paged_attn_common.h"
 
 namespace ns {
@@ -299,7 +302,7 @@ extern "C" {
 size_t ns_paged_attention_fp8_workspace(int T, int B, int Hq, int Hk, int D, int max_len, int ragged,
                                         int shared) {
   if (!ns::sizes_ok(T, B, Hq, Hk, D, max_len, shared)) return 0;
-  return ns::make_plan(T, B, Hq, Hk, D, max_len, ragged != 0, shared, ns::kOneRows).bytes;
+  return ns::make_plan(T, B, Hq, Hk, D, max_len, ragged != 0, shared, ns::kOneRows, true).bytes;
 }
 
 int ns_paged_attention_fp8(const void* q, long long q_stride, const void* k_pool, const void* v_pool,
