@@ -25,10 +25,12 @@ namespace ns {
 namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
-constexpr int kVecs = 2, kPer = 8 * kVecs;       // vectors and logits of a thread in a tile
-constexpr int kTile = kThreads * kPer;           // logits of a tile
+constexpr int kMostVecs = 4;                     // vectors of 8 logits of a thread in a tile
 constexpr int kMostBeams = 64, kMostKept = 64;   // a list to a lane, and a bound from 64 lane maxima
 constexpr int kMostParts = 64;
+constexpr int kSlack = 8;                        // lanes of equal largest logits that a bound may reach beyond n
+constexpr int kAtOnce = 8;                       // comparisons whose operands are loaded together
+static_assert(kWaves == 4, "the end of beam_rows_kernel");
 constexpr int kMostKeys = 12288;                 // keys of all parts of a request in the merge's LDS
 
 struct BeamArgs {
@@ -39,7 +41,7 @@ struct BeamArgs {
   double2* sums;     // [rows][parts]: maximum, sum of exp(l - maximum)
   float* out_scores;
   int *out_tokens, *out_parents;
-  int V, beams, n, parts, tiles;
+  int V, beams, n, parts, tiles;  // (tiles of a row)
 };
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
@@ -56,107 +58,164 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// A key that n of the wave's lanes reach, and no more than n (all that are not 0, if they are fewer): keys differ.
-__device__ __forceinline__ uint64_t nth_bound(uint64_t key, int n) {
-  if (__popcll(__ballot(key != 0)) <= n) return 1;
-  uint64_t at = 0;
+// The largest `at` that n of the wave's lanes reach (0: fewer than n are not 0), and how many reach it. Searched from
+// the highest bit in which lanes differ.
+__device__ __forceinline__ uint32_t nth_value(uint32_t high, int n, int& reach) {
+  reach = __popcll(__ballot(high != 0));
+  if (reach < n) return 0;
+  const uint32_t most = wave_umax(high), least = ~wave_umax(~high);
+  int bit = most == least ? -1 : 31 - __builtin_clz(most ^ least);
+  uint32_t at = bit < 0 ? most : most & ~((2u << bit) - 1u);
+  reach = kWave;
 #pragma unroll 1
-  for (int half = 1; half >= 0; --half) {
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint64_t next = at | 1ull << (32 * half + bit);
-      const int reach = __popcll(__ballot(key >= next));
-      if (reach >= n) at = next;
-      if (reach == n) return at;
-    }
+  for (; bit >= 0; --bit) {
+    const uint32_t next = at | 1u << bit;
+    const int k = __popcll(__ballot(high >= next));
+    if (k < n) continue;
+    at = next;
+    reach = k;
+    if (k == n) break;
   }
   return at;
 }
 
-template <typename E>
+// Of lanes whose keys differ in the low half: a key that n lanes reach, and no more than n, where more than n reach `at`.
+__device__ __forceinline__ uint64_t nth_key(uint64_t key, uint32_t at, int n) {
+  const uint32_t high = (uint32_t)(key >> 32);
+  const int more = __popcll(__ballot(high > at));
+  uint32_t low = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = low | 1u << bit;
+    if (more + __popcll(__ballot(high == at && (uint32_t)key >= next)) >= n) low = next;
+  }
+  return (uint64_t)at << 32 | low;
+}
+
+// The sum over the wave's lanes, in lane 63, by DPP (row shifts, then row broadcasts).
+__device__ __forceinline__ double wave_total(double v) {
+  auto add = [](double x, auto ctrl, auto rows) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    auto part = [](uint32_t w) {
+      return (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    return x + __longlong_as_double((long long)(part((uint32_t)(u >> 32)) << 32 | part((uint32_t)u)));
+  };
+  using M = std::integral_constant<int, 0xf>;
+  v = add(v, std::integral_constant<int, 0x111>{}, M{});
+  v = add(v, std::integral_constant<int, 0x112>{}, M{});
+  v = add(v, std::integral_constant<int, 0x114>{}, M{});
+  v = add(v, std::integral_constant<int, 0x118>{}, M{});
+  v = add(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  return add(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+}
+
+template <typename E, int kVecs>
 __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
-  extern __shared__ uint64_t list[];  // n kept before + kWaves * n * kPer
+  extern __shared__ uint64_t list[];  // n kept before + kWaves * (n + kSlack) * 8 kVecs, and kAtOnce of 0
   __shared__ uint64_t bounds[kWaves], kept[kMostKept];
-  __shared__ float red_m[kWaves];
+  __shared__ uint32_t tops[kWaves];
   __shared__ double red_s[kWaves];
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long r = blockIdx.y;
   const int part = blockIdx.x, n = a.n;
   uint64_t* out = a.keys + (r * a.parts + part) * n;
+  const Row<E> row{static_cast<const E*>(a.logits) + r * a.row_stride, a.V};
+  const int t0 = (int)((long long)a.tiles * part / a.parts), t1 = (int)((long long)a.tiles * (part + 1) / a.parts);
+  typename Row<E>::Raw raw[kVecs];
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) raw[j] = row.fetch((t * kVecs + j) * kThreads + tid);
+  };
   const float score = a.scores[r];
+  fetch(t0);
   if (!(score > -INFINITY)) {  // a beam that does not count
     if (tid < n) out[tid] = 0;
     if (tid == 0) a.sums[r * a.parts + part] = make_double2(-INFINITY, 0.);
     return;
   }
-  const Row<E> row{static_cast<const E*>(a.logits) + r * a.row_stride, a.V};
-  const int t0 = (int)((long long)a.tiles * part / a.parts), t1 = (int)((long long)a.tiles * (part + 1) / a.parts);
-  float m = -INFINITY;  // of this wave
-  double sum = 0.;      // of this lane, in units of exp(m)
-  int have = 0;         // keys in `kept`, descending
+  float m = -INFINITY;
+  double sum = 0.;  // of this lane, in units of exp(m)
+  int have = 0;     // keys in `kept`, descending
   for (int t = t0; t < t1; ++t) {
-    typename Row<E>::Raw raw[kVecs];
-    const int v0 = t * (kTile / 8) + tid;
-#pragma unroll
-    for (int j = 0; j < kVecs; ++j) raw[j] = row.fetch(v0 + j * kThreads);
+    const int v0 = t * kVecs * kThreads + tid;
     float x[kVecs][8], top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
-      row.read(raw[j], v0 + j * kThreads, x[j]);
+      // (NaN -> -inf, +inf -> the largest finite value; -0 may stay)
+      row.read(raw[j], v0 + j * kThreads, x[j], [](float v) { return fminf(fmaxf(v, -INFINITY), FLT_MAX); });
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, x[j][e]);
     }
-    // the lane's largest, its first place
-    uint64_t best = 0;
-    if (top > -INFINITY) {
-      uint32_t at = 0;
+    if (t + 1 < t1) fetch(t + 1);
+    auto key_at = [&](int j, int e) {
+      return (uint64_t)key_of(x[j][e] + 0.f) << 32 | ~(uint32_t)(row.first(v0 + j * kThreads) + e);
+    };
+    const uint32_t high = top > -INFINITY ? key_of(top + 0.f) : 0;
+    int reach;
+    uint64_t bound = (uint64_t)nth_value(high, n, reach) << 32;
+    if (reach > n + kSlack) {  // many equal ones: by index too, from each lane's largest at its first place
+      uint64_t best = 0;
 #pragma unroll
-      for (int j = kVecs - 1; j >= 0; --j)
+      for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-        for (int e = 7; e >= 0; --e)
-          if (x[j][e] == top) at = row.first(v0 + j * kThreads) + e;
-      best = (uint64_t)key_of(top) << 32 | ~at;
+        for (int e = 0; e < 8; ++e) best = max(best, x[j][e] == top ? key_at(j, e) : 0);
+      bound = nth_key(top > -INFINITY ? best : 0, (uint32_t)(bound >> 32), n);
     }
-    const uint32_t high = wave_umax((uint32_t)(best >> 32));
-    if (high != 0) {
-      const float mt = fmaxf(m, value_of(high));
+    if (have == n) bound = max(bound, kept[n - 1] + 1);
+    const uint32_t wave_top = wave_umax(high);
+    if (lane == 0) {
+      bounds[wv] = bound;
+      tops[wv] = wave_top;
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+    uint32_t most = 0;
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+      bound = max(bound, bounds[k]);
+      most = max(most, tops[k]);
+    }
+    const float least = bound >> 32 ? value_of((uint32_t)(bound >> 32)) : -FLT_MAX;
+    if (top >= least) {
+#pragma unroll
+      for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (x[j][e] >= least) {
+            const uint64_t key = key_at(j, e);
+            if (key >= bound) list[atomicAdd(&count, 1)] = key;
+          }
+    }
+    if (most != 0) {
+      const float mt = fmaxf(m, value_of(most));
+      if (mt != m) {
+        sum = m == -INFINITY ? 0. : sum * exp((double)m - mt);
+        m = mt;
+      }
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < kVecs; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) s += __expf(x[j][e] - mt);
-      sum = (mt == m ? sum : sum * (double)__expf(m - mt)) + (double)s;
-      m = mt;
-    }
-    uint64_t bound = nth_bound(best, n);
-    if (have == n) bound = max(bound, kept[n - 1] + 1);
-    if (lane == 0) bounds[wv] = bound;
-    if (tid == 0) count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) bound = max(bound, bounds[k]);
-    if (best >= bound) {
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint64_t key = (uint64_t)key_of(x[j][e]) << 32 | ~(uint32_t)(row.first(v0 + j * kThreads) + e);
-          if (x[j][e] > -INFINITY && key >= bound) list[atomicAdd(&count, 1)] = key;
-        }
+      sum += (double)s;
     }
     __syncthreads();
     const int fresh = count;
     if (fresh > 0) {
       // ranks among the new ones and those kept before (which need not reach the bound)
-      uint64_t old = tid < have ? kept[tid] : 0;
       const int all = fresh + have;
-      if (tid < have) list[fresh + tid] = old;
+      if (tid < have) list[fresh + tid] = kept[tid];
+      if (tid < kAtOnce) list[all + tid] = 0;
       __syncthreads();
       for (int i = tid; i < all; i += kThreads) {
         const uint64_t key = list[i];
         int rank = 0;
-        for (int k = 0; k < all; ++k) rank += list[k] > key;
+        for (int k = 0; k < all; k += kAtOnce) {
+#pragma unroll
+          for (int u = 0; u < kAtOnce; ++u) rank += list[k + u] > key;
+        }
         if (rank < n) kept[rank] = key;
       }
       have = min(all, n);
@@ -164,22 +223,10 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
     __syncthreads();
   }
   if (tid < n) out[tid] = tid < have ? kept[tid] : 0;
-  // the waves' sums, in a fixed order
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) sum += __shfl_xor(sum, d, kWave);
-  if (lane == 0) {
-    red_m[wv] = m;
-    red_s[wv] = sum;
-  }
+  sum = wave_total(sum);
+  if (lane == 63) red_s[wv] = sum;
   __syncthreads();
-  if (tid == 0) {
-    float mt = red_m[0];
-    for (int k = 1; k < kWaves; ++k) mt = fmaxf(mt, red_m[k]);
-    double s = 0.;
-    for (int k = 0; k < kWaves; ++k)
-      if (red_m[k] > -INFINITY) s += red_s[k] * exp((double)red_m[k] - mt);
-    a.sums[r * a.parts + part] = make_double2(mt, s);
-  }
+  if (tid == 0) a.sums[r * a.parts + part] = make_double2(m, (red_s[0] + red_s[1]) + (red_s[2] + red_s[3]));
 }
 
 // The lane with the largest key, the first of several; every lane's value of it. -1: all are 0.
@@ -202,58 +249,133 @@ __device__ __forceinline__ uint64_t order_of(double x) {
 }
 
 constexpr int kMergeThreads = 512;
+constexpr int kMostRanked = kMergeThreads;  // continuations that are ordered by rank, one to a thread
+constexpr int kEach = kMostKeys / kMergeThreads;
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   extern __shared__ uint64_t lds[];  // [beams][parts][n], then [beams][n]
   __shared__ double base[kMostBeams];
+  __shared__ uint64_t bounds[kMergeThreads / kWave];
+  // the sum's order, and what decides between equal sums: beam (6 bits, complement), logit key (32), index (20, complement)
+  __shared__ __align__(16) ulonglong2 found[kMostRanked + kAtOnce];
+  __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = a.n, lists = a.beams * a.parts;
+  const int n = a.n, lists = a.beams * a.parts, all = lists * n;
   const long long r0 = (long long)blockIdx.x * a.beams;
-  uint64_t* best = lds + (size_t)lists * n;
   const uint64_t* keys = a.keys + r0 * a.parts * n;
-  for (int i = tid; i < lists * n; i += kMergeThreads) lds[i] = keys[i];
-  __syncthreads();
+  uint64_t first[2], key_at[kEach];  // of the lane's lists; of its share of all keys
+#pragma unroll
+  for (int u = 0; u < 2; ++u) first[u] = tid + u * kMergeThreads < lists ? keys[(size_t)(tid + u * kMergeThreads) * n] : 0;
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    if (u * kMergeThreads >= all) break;
+    key_at[u] = tid + u * kMergeThreads < all ? keys[tid + u * kMergeThreads] : 0;
+  }
+  if (tid == 0) count = 0;
   for (int b = wv; b < a.beams; b += kMergeThreads / kWave) {
     const double2 ms = lane < a.parts ? a.sums[(r0 + b) * a.parts + lane] : make_double2(-INFINITY, 0.);
+    const float score = a.scores[r0 + b];
     const double m = value_of(wave_umax(key_of((float)ms.x)));
-    double s = ms.x > -INFINITY ? ms.y * exp(ms.x - m) : 0.;
+    const double s = wave_total(ms.x > -INFINITY ? ms.y * exp(ms.x - m) : 0.);
+    if (lane == 63) base[b] = (double)fminf(score, FLT_MAX) - (m + log(s));
+  }
+  __syncthreads();
+  auto total = [&](uint64_t key, int b) { return key ? order_of(base[b] + value_of((uint32_t)(key >> 32))) : 0; };
+
+  // A bound that n continuations reach: of the lists' first ones, a list to a lane (or several: their largest)
+  uint64_t head = 0;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) s += __shfl_xor(s, d, kWave);
-    if (lane == 0) base[b] = (double)fminf(a.scores[r0 + b], FLT_MAX) - (m + log(s));
-    // the parts' lists, each descending, a list to a lane
-    const uint64_t* mine = lds + ((size_t)b * a.parts + min(lane, a.parts - 1)) * n;
-    uint64_t head = lane < a.parts ? mine[0] : 0;
+  for (int u = 0; u < 2; ++u)
+    if (first[u]) head = max(head, total(first[u], (tid + u * kMergeThreads) / a.parts));
+  for (int i = tid + 2 * kMergeThreads; i < lists; i += kMergeThreads) head = max(head, total(keys[(size_t)i * n], i / a.parts));
+  int reach;
+  const uint64_t mine = (uint64_t)nth_value((uint32_t)(head >> 32), n, reach) << 32;
+  if (lane == 0) bounds[wv] = mine;
+  __syncthreads();
+  uint64_t bound = 1;
+#pragma unroll
+  for (int k = 0; k < kMergeThreads / kWave; ++k) bound = max(bound, bounds[k]);
+#pragma unroll
+  for (int u = 0; u < kEach; ++u) {
+    if (u * kMergeThreads >= all) break;
+    const uint64_t key = key_at[u];
+    const int b = (tid + u * kMergeThreads) / (a.parts * n);
+    const uint64_t c = key ? total(key, b) : 0;
+    if (c >= bound) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kMostRanked)
+        found[at] = make_ulonglong2(c, (uint64_t)(63 - b) << 52 | (key >> 32) << 20 | (key & 0xfffffu));
+    }
+  }
+  __syncthreads();
+  const int many = count;
+  const size_t o = (size_t)blockIdx.x * n;
+  if (many <= kMostRanked) {
+    if (tid < kAtOnce) found[many + tid] = make_ulonglong2(0, 0);
+    __syncthreads();
+    if (tid < many) {
+      const ulonglong2 c = found[tid];
+      int rank = 0;
+      for (int k = 0; k < many; k += kAtOnce) {
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+          const ulonglong2 x = found[k + u];
+          rank += (x.x > c.x) | ((x.x == c.x) & (x.y > c.y));
+        }
+      }
+      if (rank < n) {
+        const int b = 63 - (int)(c.y >> 52);
+        a.out_scores[o + rank] = (float)(base[b] + value_of((uint32_t)(c.y >> 20)));
+        a.out_tokens[o + rank] = 0xfffff - (int)(c.y & 0xfffffu);
+        a.out_parents[o + rank] = b;
+      }
+    }
+    for (int k = many + tid; k < n; k += kMergeThreads) {
+      a.out_scores[o + k] = -INFINITY;
+      a.out_tokens[o + k] = a.out_parents[o + k] = -1;
+    }
+    return;
+  }
+
+  // Many equal sums: the parts' lists beam by beam, each descending, a list to a lane, then the beams' lists.
+  uint64_t* best = lds + all;
+#pragma unroll
+  for (int u = 0; u < kEach; ++u)
+    if (tid + u * kMergeThreads < all) lds[tid + u * kMergeThreads] = key_at[u];
+  __syncthreads();
+  for (int b = wv; b < a.beams; b += kMergeThreads / kWave) {
+    const uint64_t* list = lds + ((size_t)b * a.parts + min(lane, a.parts - 1)) * n;
+    uint64_t head = lane < a.parts ? list[0] : 0;
     int at = 0;
     for (int k = 0; k < n; ++k) {
       const int w = wave_best(head);
       const uint64_t key = w < 0 ? 0 : (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(head >> 32), w) << 32 |
                                            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)head, w);
       if (lane == 0) best[b * n + k] = key;
-      if (lane == w) head = ++at < n ? mine[at] : 0;
+      if (lane == w) head = ++at < n ? list[at] : 0;
     }
   }
   __syncthreads();
   if (wv != 0) return;
-  // the beams' lists, a beam to a lane
-  const uint64_t* mine = best + min(lane, a.beams - 1) * n;
-  auto total = [&](uint64_t key) { return key ? order_of(base[min(lane, a.beams - 1)] + value_of((uint32_t)(key >> 32))) : 0; };
-  uint64_t key = lane < a.beams ? mine[0] : 0, head = total(key);
+  const int b = min(lane, a.beams - 1);
+  const uint64_t* list = best + b * n;
+  uint64_t key = lane < a.beams ? list[0] : 0;
+  head = total(key, b);
   int at = 0;
   for (int k = 0; k < n; ++k) {
     const int w = wave_best(head);
     if (w < 0 ? lane == 0 : lane == w) {
-      const size_t o = (size_t)blockIdx.x * n + k;
-      a.out_scores[o] = w < 0 ? -INFINITY : (float)(base[lane] + value_of((uint32_t)(key >> 32)));
-      a.out_tokens[o] = w < 0 ? -1 : (int)~(uint32_t)key;
-      a.out_parents[o] = w;
-      key = ++at < n && w >= 0 ? mine[at] : 0;
-      head = total(key);
+      a.out_scores[o + k] = w < 0 ? -INFINITY : (float)(base[b] + value_of((uint32_t)(key >> 32)));
+      a.out_tokens[o + k] = w < 0 ? -1 : (int)~(uint32_t)key;
+      a.out_parents[o + k] = w;
+      key = ++at < n && w >= 0 ? list[at] : 0;
+      head = total(key, b);
     }
   }
 }
 
 struct Plan {
-  int tiles, parts;
+  int vecs, tiles, parts;
   size_t bytes;
 };
 
@@ -264,9 +386,11 @@ bool sizes_ok(int R, int beams, int V, int n) {
 
 Plan make_plan(int R, int beams, int V, int n) {
   Plan p;
-  p.tiles = (V + kTile - 1) / kTile;
   const long long rows = (long long)R * beams;
-  const int want = (int)std::max(1ll, 2048 / rows);
+  auto tiles = [&](int vecs) { return (V + 8 * vecs * kThreads - 1) / (8 * vecs * kThreads); };
+  p.vecs = n <= kMostKept / 2 && rows * tiles(kMostVecs) >= 1024 ? kMostVecs : 2;
+  p.tiles = tiles(p.vecs);
+  const int want = (int)std::max(1ll, 4096 / rows);
   p.parts = std::min({p.tiles, want, kMostParts, std::max(1, kMostKeys / (beams * n))});
   p.bytes = (size_t)rows * p.parts * (n * sizeof(uint64_t) + sizeof(double2));
   return p;
@@ -317,12 +441,13 @@ int ns_beam_select(const void* logits, int fp32, long long row_stride, const flo
   a.parts = p.parts;
   a.tiles = p.tiles;
   const auto st = static_cast<hipStream_t>(stream);
-  const size_t list = ((size_t)n + ns::kWaves * n * ns::kPer) * sizeof(uint64_t);  // (up to 33 KB)
+  const int reach = std::min(n + ns::kSlack, ns::kWave);
+  const size_t list = ((size_t)n + ns::kWaves * reach * 8 * p.vecs + ns::kAtOnce) * sizeof(uint64_t);  // (up to 41 KB)
   const dim3 grid(p.parts, (unsigned)rows);
-  if (fp32)
-    hipLaunchKernelGGL((ns::beam_rows_kernel<float>), grid, dim3(ns::kThreads), list, st, a);
-  else
-    hipLaunchKernelGGL((ns::beam_rows_kernel<uint16_t>), grid, dim3(ns::kThreads), list, st, a);
+  const auto rows_kernel = fp32 ? (p.vecs == 2 ? ns::beam_rows_kernel<float, 2> : ns::beam_rows_kernel<float, ns::kMostVecs>)
+                                : (p.vecs == 2 ? ns::beam_rows_kernel<uint16_t, 2>
+                                               : ns::beam_rows_kernel<uint16_t, ns::kMostVecs>);
+  hipLaunchKernelGGL(rows_kernel, grid, dim3(ns::kThreads), list, st, a);
   // (its most, up to 128 KB, is asked for where 64 are not enough)
   const size_t merge = ((size_t)beams * p.parts * n + (size_t)beams * n) * sizeof(uint64_t);
   if (merge > 60 * 1024) {

@@ -58,7 +58,9 @@ struct Row {
     }
     return r;
   }
-  __device__ void read(const Raw& r, int i, float (&x)[8]) const {
+  __device__ void read(const Raw& r, int i, float (&x)[8]) const { read(r, i, x, clean); }
+  template <class Clean>
+  __device__ void read(const Raw& r, int i, float (&x)[8], Clean clean) const {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t w = sizeof(E) == 2 ? r.w[e >> 1] : r.w[e];
