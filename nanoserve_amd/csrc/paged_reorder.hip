@@ -5,7 +5,10 @@
 // of a parent's children one keeps it, and the others take over the last pages of beams that ended, of which there are as
 // many. Sources are thus pages that stay and destinations pages that nobody reads: all copies and tables go in one launch, and
 // a second run of the call gives the same. Bound by HBM for many layers (each copied row read once and written once),
-// by the latency of parents -> page ids -> rows for few.
+// by the latency of parents -> page ids -> rows for few. A wave copies the rows of one layer and head, eight loads in
+// flight to a lane and no divisions: with a workgroup per layer and an index per 16 bytes 16 x 8 beams in 28 layers (88 MB)
+// took 30.8 us, 16 beams on pages of 16 17.6. Stores pass the caches, which the copies would leave before they are read.
+// Measured: 16 x 8 beams 18.3 us, 4.8 TB/s (20.6 with ordinary stores); 4 x 4 beams on pages of 16 4.4 us.
 #include <stdint.h>
 
 #include <algorithm>
@@ -25,7 +28,7 @@ struct ReorderArgs {
   int* out;  // [rows][width]
   uint8_t *pool[2], *scale[2];  // K and V; scales null: a cache without
   long long layer, page, head, s_layer, s_page, s_head;  // strides in bytes
-  int beams, width, page_size, row_bytes, n_pages, Hk, layers, table_grid;
+  int beams, width, page_size, row_bytes, n_pages, Hk, layers, groups, table_grid;
 };
 
 // Beam i's parent and the beam whose last page it gets, of the request whose lanes hold the parents (lane = beam).
@@ -75,45 +78,38 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(ReorderArgs a) {
     }
     return;
   }
-  // a workgroup per beam, layer and one of K and V: the rows of all heads
+  // a wave per beam, layer, head and one of K and V, whose rows are contiguous
   long long id = blockIdx.x - a.table_grid;
   const int kv = (int)(id & 1);
   id >>= 1;
-  const int layer = (int)(id % a.layers);
-  const long long row = id / a.layers, request = row / a.beams;
+  const int pair = (int)(id % a.groups) * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(tid >> 6);
+  const long long row = id / a.groups, request = row / a.beams;
   const Way w = way_of(a, request, (int)(row % a.beams));
-  if (w.place == w.parent) return;
+  if (w.place == w.parent || pair >= a.layers * a.Hk) return;
   const long long from = request * a.beams + w.parent;
   const int len = min(max(a.lens[from], 0), a.width * a.page_size), part = len % a.page_size;
   if (part == 0) return;
   const int at = len / a.page_size;
   const int src = a.table[from * a.table_stride + at], dst = a.table[(request * a.beams + w.place) * a.table_stride + at];
   if ((unsigned)src >= (unsigned)a.n_pages || (unsigned)dst >= (unsigned)a.n_pages) return;
-  const uint8_t* s = a.pool[kv] + layer * a.layer + src * a.page;
-  uint8_t* d = a.pool[kv] + layer * a.layer + dst * a.page;
-  const int chunks = part * a.row_bytes / 16, total = chunks * a.Hk;  // of 16 bytes
-  constexpr int kAtOnce = 4;
-  for (int i0 = tid; i0 < total; i0 += kAtOnce * kThreads) {
-    uint4 v[kAtOnce];
-    long long off[kAtOnce];
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int i = min(i0 + u * kThreads, total - 1);
-      off[u] = i / chunks * a.head + i % chunks * 16ll;
-      v[u] = *reinterpret_cast<const uint4*>(s + off[u]);
-    }
+  const int layer = pair / a.Hk, head = pair % a.Hk, lane = tid & 63;
+  uint8_t* rows = a.pool[kv] + layer * a.layer + head * a.head;
+  const u32x4_t* s = reinterpret_cast<const u32x4_t*>(rows + src * a.page);
+  u32x4_t* d = reinterpret_cast<u32x4_t*>(rows + dst * a.page);
+  const int chunks = part * a.row_bytes / 16;  // of 16 bytes
+  constexpr int kAtOnce = 8;
+  for (int c0 = lane; c0 < chunks; c0 += kAtOnce * kWave) {
+    u32x4_t v[kAtOnce];
 #pragma unroll
     for (int u = 0; u < kAtOnce; ++u)
-      if (i0 + u * kThreads < total) *reinterpret_cast<uint4*>(d + off[u]) = v[u];
+      if (c0 + u * kWave < chunks) v[u] = s[c0 + u * kWave];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+      if (c0 + u * kWave < chunks) __builtin_nontemporal_store(v[u], &d[c0 + u * kWave]);
   }
   if (!a.scale[kv]) return;
-  const int blocks = (part + kScaleRows - 1) / kScaleRows;
-  const uint8_t* ss = a.scale[kv] + layer * a.s_layer + src * a.s_page;
-  uint8_t* sd = a.scale[kv] + layer * a.s_layer + dst * a.s_page;
-  for (int i = tid; i < blocks * a.Hk; i += kThreads) {
-    const long long off = i / blocks * a.s_head + i % blocks;
-    sd[off] = ss[off];
-  }
+  uint8_t* scales = a.scale[kv] + layer * a.s_layer + head * a.s_head;
+  for (int i = lane; i < (part + kScaleRows - 1) / kScaleRows; i += kWave) scales[dst * a.s_page + i] = scales[src * a.s_page + i];
 }
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -159,7 +155,7 @@ extern "C" int ns_paged_reorder(const int* parents, long long parent_stride, con
   if (!ns::nested(piece, layers, layer_stride, n_pages, page_stride, Hk, head_stride)) return -2;
   if (k_scales && !ns::nested(marks, layers, scale_layer_stride, n_pages, scale_page_stride, Hk, scale_head_stride))
     return -2;
-  if (rows * (2ll * layers + 1) >= (1ll << 31)) return -2;
+  if ((long long)layers * Hk >= (1ll << 30) || rows * (((long long)layers * Hk + 3) / 4 * 2 + 1) >= (1ll << 31)) return -2;
   const ns::Bytes y = ns::bytes_of(out, 4 * (size_t)rows * width), z[] = {ns::rows_of(parents, R, parent_stride, beams, 4),
                                                                         ns::rows_of(table, rows, table_stride, width, 4),
                                                                         ns::bytes_of(lens, 4 * (size_t)rows)};
@@ -218,7 +214,8 @@ extern "C" int ns_paged_reorder(const int* parents, long long parent_stride, con
   a.Hk = Hk;
   a.layers = layers;
   a.table_grid = (int)rows;
+  a.groups = (int)(((long long)layers * Hk + 3) / 4);
   const auto st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(ns::reorder_kernel, dim3((unsigned)(rows * (2ll * layers + 1))), dim3(ns::kThreads), 0, st, a);
+  hipLaunchKernelGGL(ns::reorder_kernel, dim3((unsigned)(rows * (2ll * a.groups + 1))), dim3(ns::kThreads), 0, st, a);
   return static_cast<int>(hipGetLastError());
 }
