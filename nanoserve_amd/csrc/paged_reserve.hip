@@ -76,15 +76,17 @@ __device__ __forceinline__ long long slot_of(const ReserveArgs& a, int b, int le
 __global__ void __launch_bounds__(kThreads) reserve_kernel(ReserveArgs a, int with_slots) {
   constexpr int kWaves = kThreads / kWave;
   __shared__ long long part[3][kWaves];
-  __shared__ long long ends[3][kThreads];  // per sequence of a chunk: pages taken, pages given, token rows, up to its own
+  // per sequence of a chunk: pages taken, pages given, token rows, up to its own (of a call that goes through: below 2^31)
+  __shared__ int ends[3][kThreads];
   __shared__ int firsts[2][kThreads];      // first table entry taken, given
   __shared__ int lens[kThreads];           // positions after
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   long long all[3];  // of a chunk
 
-  // inclusive sums over the workgroup; total in part[k][kWaves]. A wave's sums fit 32 bits: of entries (each below
-  // 2^26), and of token rows (below 2^30) in two halves.
-  auto scan = [&](const Ask& x, long long (&v)[3]) {
+  // Inclusive sums over a chunk of n sequences, its totals in `all`. A wave's sums fit 32 bits: of entries (each below
+  // 2^26), and of token rows (below 2^30) in two halves. (Over the waves that have sequences alone: all 16 for
+  // each of three sums took half of a small call's time.)
+  auto scan = [&](const Ask& x, int n, long long (&v)[3]) {
     v[0] = wave_scan((uint32_t)x.taken());
     v[1] = wave_scan((uint32_t)x.given());
     v[2] = (long long)wave_scan((uint32_t)x.grown >> 16) * 65536 + wave_scan((uint32_t)x.grown & 0xffff);
@@ -93,15 +95,13 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(ReserveArgs a, int wi
       if (lane == 63) part[k][wv] = v[k];
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      long long sum = 0;
+    for (int k = 0; k < 3; ++k) all[k] = 0;
+    for (int u = 0; u < (n + kWave - 1) / kWave; ++u) {
 #pragma unroll
-      for (int u = 0; u < kWaves; ++u) {
-        const long long s = part[k][u];
-        if (u < wv) v[k] += s;
-        sum += s;
+      for (int k = 0; k < 3; ++k) {
+        if (u == wv) v[k] += all[k];
+        all[k] += part[k][u];
       }
-      all[k] = sum;
     }
   };
 
@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(ReserveArgs a, int wi
   for (int base = 0; base < a.B; base += kThreads) {
     x = ask_of(a, base + tid);
     fits &= __syncthreads_and(x.fits) != 0;
-    scan(x, v);
+    scan(x, min(a.B - base, kThreads), v);
 #pragma unroll
     for (int k = 0; k < 3; ++k) total[k] += all[k];
   }
@@ -129,62 +129,65 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(ReserveArgs a, int wi
 
   // ---- pages given back go to the stack first (from all chunks, as pages taken may be among them), the last sequence's last
   // page lowest: what was taken together comes back as it lay
-  long long seen[3] = {0, 0, 0};
+  int seen[3];
   for (int pass = total[1] > 0 ? 0 : 1; pass < 2; ++pass) {
     seen[0] = seen[1] = seen[2] = 0;
     for (int base = 0; base < a.B; base += kThreads) {
       if (a.B > kThreads) {  // (otherwise the totals' values still stand)
         x = ask_of(a, base + tid);
         __syncthreads();
-        scan(x, v);
+        scan(x, min(a.B - base, kThreads), v);
       }
-      ends[0][tid] = v[0];
-      ends[1][tid] = v[1];
-      ends[2][tid] = v[2];
-      firsts[0][tid] = x.had;
-      firsts[1][tid] = x.has;
-      lens[tid] = x.len;
-      __syncthreads();
+      if (a.B > kThreads || pass == 0 || total[1] == 0) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) ends[k][tid] = (int)v[k];
+        firsts[0][tid] = x.had;
+        firsts[1][tid] = x.has;
+        lens[tid] = x.len;
+        __syncthreads();
+      }
       const int n = min(a.B - base, kThreads);
-      auto owner = [&](int k, long long i) {  // the sequence of the chunk whose share of sum k holds number i
+      auto owner = [&](const int* end, int i) {  // the sequence of the chunk whose share holds number i
         int lo = 0, hi = n - 1;
         while (lo < hi) {
           const int mid = (lo + hi) >> 1;
-          if (ends[k][mid] > i)
+          if (end[mid] > i)
             hi = mid;
           else
             lo = mid + 1;
         }
         return lo;
       };
-      const int k = 1 - pass;
-      for (long long i = tid; i < ends[k][n - 1]; i += kThreads) {
-        const int s = owner(k, i);
-        const long long in = i - (s > 0 ? ends[k][s - 1] : 0);
-        int* entry = a.table + (size_t)(base + s) * a.table_stride + firsts[k][s] + in;
-        int* page = a.free + (top - 1 - (seen[k] + i));
+      const int k = 1 - pass, moved = ends[k][n - 1];
+      int* table = a.table + (size_t)base * a.table_stride;
+      int* stack = a.free + (top - 1 - seen[k]);
+      for (int i = tid; i < moved; i += kThreads) {
+        const int s = owner(ends[k], i);
+        int* entry = table + (size_t)s * a.table_stride + (firsts[k][s] + i - (s > 0 ? ends[k][s - 1] : 0));
         if (pass == 0)
-          *page = *entry;
+          stack[-i] = *entry;
         else
-          *entry = *page;
+          *entry = stack[-i];
       }
       if (pass == 1) {
         if (tid < n) {
-          a.q_start[base + tid + 1] = (int)(seen[2] + v[2]);
+          a.q_start[base + tid + 1] = seen[2] + (int)v[2];
           a.lens[base + tid] = x.len;
         }
         if (with_slots) {
           __syncthreads();  // the entries are written
-          for (long long i = tid; i < ends[2][n - 1]; i += kThreads) {
-            const int s = owner(2, i);
-            a.slots[seen[2] + i] = slot_of(a, base + s, lens[s], (int)(ends[2][s] - i));
+          const int rows = ends[2][n - 1];
+          for (int i = tid; i < rows; i += kThreads) {
+            const int s = owner(ends[2], i);
+            a.slots[seen[2] + i] = slot_of(a, base + s, lens[s], ends[2][s] - i);
           }
         }
       }
 #pragma unroll
-      for (int q = 0; q < 3; ++q) seen[q] += all[q];
-      __syncthreads();  // (the arrays are read)
+      for (int q = 0; q < 3; ++q) seen[q] += (int)all[q];
+      if (a.B > kThreads) __syncthreads();  // (the arrays are read)
     }
+    __syncthreads();
   }
   if (tid == 0) {
     a.q_start[0] = 0;
