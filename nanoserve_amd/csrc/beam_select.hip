@@ -28,7 +28,7 @@ constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostVecs = 4;                     // vectors of 8 logits of a thread in a tile
 constexpr int kMostBeams = 64, kMostKept = 64;   // a list to a lane, and a bound from 64 lane maxima
 constexpr int kMostParts = 64;
-constexpr int kSlack = 8;                        // lanes of equal largest logits that a bound may reach beyond n
+constexpr int kSlack = 4;                        // lanes beyond n that may reach a bound
 constexpr int kAtOnce = 8;                       // comparisons whose operands are loaded together
 static_assert(kWaves == 4, "the end of beam_rows_kernel");
 constexpr int kMostKeys = 12288;                 // keys of all parts of a request in the merge's LDS
@@ -42,6 +42,7 @@ struct BeamArgs {
   float* out_scores;
   int *out_tokens, *out_parents;
   int V, beams, n, parts, tiles;  // (tiles of a row)
+  int segment;                    // keys of a wave's list of a tile
 };
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
@@ -58,9 +59,9 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// The largest `at` that n of the wave's lanes reach (0: fewer than n are not 0), and how many reach it. Searched from
-// the highest bit in which lanes differ.
-__device__ __forceinline__ uint32_t nth_value(uint32_t high, int n, int& reach) {
+// A value that n of the wave's lanes reach (0: fewer than n are not 0), and how many reach it: at most `slack` more, or
+// as many as are equal to the n-th. Searched from the highest bit in which lanes differ.
+__device__ __forceinline__ uint32_t nth_value(uint32_t high, int n, int slack, int& reach) {
   reach = __popcll(__ballot(high != 0));
   if (reach < n) return 0;
   const uint32_t most = wave_umax(high), least = ~wave_umax(~high);
@@ -74,7 +75,7 @@ __device__ __forceinline__ uint32_t nth_value(uint32_t high, int n, int& reach) 
     if (k < n) continue;
     at = next;
     reach = k;
-    if (k == n) break;
+    if (k <= n + slack) break;
   }
   return at;
 }
@@ -112,11 +113,11 @@ __device__ __forceinline__ double wave_total(double v) {
 
 template <typename E, int kVecs>
 __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
-  extern __shared__ uint64_t list[];  // n kept before + kWaves * (n + kSlack) * 8 kVecs, and kAtOnce of 0
-  __shared__ uint64_t bounds[kWaves], kept[kMostKept];
+  extern __shared__ uint64_t list[];  // a.segment for each wave: keys, and kAtOnce of 0
+  __shared__ uint64_t bounds[kWaves], kept[2][kMostKept + kAtOnce];
+  __shared__ int counts[kWaves];
   __shared__ uint32_t tops[kWaves];
   __shared__ double red_s[kWaves];
-  __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long r = blockIdx.y;
   const int part = blockIdx.x, n = a.n;
@@ -137,7 +138,9 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
   }
   float m = -INFINITY;
   double sum = 0.;  // of this lane, in units of exp(m)
-  int have = 0;     // keys in `kept`, descending
+  int have = 0;     // keys in kept[now], descending
+  int now = 0;
+  uint64_t* segment = list + wv * a.segment;
   for (int t = t0; t < t1; ++t) {
     const int v0 = t * kVecs * kThreads + tid;
     float x[kVecs][8], top = -INFINITY;
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
     };
     const uint32_t high = top > -INFINITY ? key_of(top + 0.f) : 0;
     int reach;
-    uint64_t bound = (uint64_t)nth_value(high, n, reach) << 32;
+    uint64_t bound = (uint64_t)nth_value(high, n, kSlack, reach) << 32;
     if (reach > n + kSlack) {  // many equal ones: by index too, from each lane's largest at its first place
       uint64_t best = 0;
 #pragma unroll
@@ -163,13 +166,12 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
         for (int e = 0; e < 8; ++e) best = max(best, x[j][e] == top ? key_at(j, e) : 0);
       bound = nth_key(top > -INFINITY ? best : 0, (uint32_t)(bound >> 32), n);
     }
-    if (have == n) bound = max(bound, kept[n - 1] + 1);
+    if (have == n) bound = max(bound, kept[now][n - 1] + 1);
     const uint32_t wave_top = wave_umax(high);
     if (lane == 0) {
       bounds[wv] = bound;
       tops[wv] = wave_top;
     }
-    if (tid == 0) count = 0;
     __syncthreads();
     uint32_t most = 0;
 #pragma unroll
@@ -178,16 +180,21 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
       most = max(most, tops[k]);
     }
     const float least = bound >> 32 ? value_of((uint32_t)(bound >> 32)) : -FLT_MAX;
-    if (top >= least) {
+    int mine = 0;  // keys of the wave's segment: counted by ballots, so that no wave waits for a counter
 #pragma unroll
-      for (int j = 0; j < kVecs; ++j)
+    for (int j = 0; j < kVecs; ++j)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (x[j][e] >= least) {
-            const uint64_t key = key_at(j, e);
-            if (key >= bound) list[atomicAdd(&count, 1)] = key;
-          }
-    }
+      for (int e = 0; e < 8; ++e)
+        if (__ballot(x[j][e] >= least)) {
+          const uint64_t key = key_at(j, e);
+          const bool hit = (x[j][e] >= least) & (key >= bound);
+          const uint64_t hits = __ballot(hit);
+          if (hit) segment[mine + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hits, 0))] = key;
+          mine += __popcll(hits);
+        }
+    if (lane < kAtOnce) segment[mine + lane] = 0;
+    if (lane == 0) counts[wv] = mine;
+    if (tid < kAtOnce) kept[now][have + tid] = 0;
     if (most != 0) {
       const float mt = fmaxf(m, value_of(most));
       if (mt != m) {
@@ -202,27 +209,35 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
       sum += (double)s;
     }
     __syncthreads();
-    const int fresh = count;
-    if (fresh > 0) {
-      // ranks among the new ones and those kept before (which need not reach the bound)
-      const int all = fresh + have;
-      if (tid < have) list[fresh + tid] = kept[tid];
-      if (tid < kAtOnce) list[all + tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < all; i += kThreads) {
-        const uint64_t key = list[i];
-        int rank = 0;
-        for (int k = 0; k < all; k += kAtOnce) {
+    int upto[kWaves + 1] = {have};
 #pragma unroll
-          for (int u = 0; u < kAtOnce; ++u) rank += list[k + u] > key;
-        }
-        if (rank < n) kept[rank] = key;
+    for (int k = 0; k < kWaves; ++k) upto[k + 1] = upto[k] + counts[k];
+    const int all = upto[kWaves];
+    if (all > have) {
+      // ranks among the new ones and those kept before (which need not reach the bound)
+      for (int i = tid; i < all; i += kThreads) {
+        uint64_t key = kept[now][min(i, have)];
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k)
+          if (i >= upto[k] && i < upto[k + 1]) key = list[k * a.segment + i - upto[k]];
+        int rank = 0;
+        auto above = [&](const uint64_t* from, int many) {
+          for (int k = 0; k < many; k += kAtOnce) {
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) rank += from[k + u] > key;
+          }
+        };
+        above(kept[now], have);
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) above(list + k * a.segment, upto[k + 1] - upto[k]);
+        if (rank < n) kept[now ^ 1][rank] = key;
       }
+      now ^= 1;
       have = min(all, n);
     }
     __syncthreads();
   }
-  if (tid < n) out[tid] = tid < have ? kept[tid] : 0;
+  if (tid < n) out[tid] = tid < have ? kept[now][tid] : 0;
   sum = wave_total(sum);
   if (lane == 63) red_s[wv] = sum;
   __syncthreads();
@@ -263,6 +278,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   const int n = a.n, lists = a.beams * a.parts, all = lists * n;
   const long long r0 = (long long)blockIdx.x * a.beams;
   const uint64_t* keys = a.keys + r0 * a.parts * n;
+  // the beam of list i and of key i: quotients of numbers below 2^14, exact by way of fp32 (half of one is far above its
+  // error), where an integer division takes ten times the instructions
+  const float per_list = 1.f / a.parts, per_key = 1.f / (a.parts * n);
+  auto quotient = [](int i, float per) { return (int)(((float)i + 0.5f) * per); };
   uint64_t first[2], key_at[kEach];  // of the lane's lists; of its share of all keys
 #pragma unroll
   for (int u = 0; u < 2; ++u) first[u] = tid + u * kMergeThreads < lists ? keys[(size_t)(tid + u * kMergeThreads) * n] : 0;
@@ -286,10 +305,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   uint64_t head = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
-    if (first[u]) head = max(head, total(first[u], (tid + u * kMergeThreads) / a.parts));
-  for (int i = tid + 2 * kMergeThreads; i < lists; i += kMergeThreads) head = max(head, total(keys[(size_t)i * n], i / a.parts));
+    if (first[u]) head = max(head, total(first[u], quotient(tid + u * kMergeThreads, per_list)));
+  for (int i = tid + 2 * kMergeThreads; i < lists; i += kMergeThreads) head = max(head, total(keys[(size_t)i * n], quotient(i, per_list)));
   int reach;
-  const uint64_t mine = (uint64_t)nth_value((uint32_t)(head >> 32), n, reach) << 32;
+  const uint64_t mine = (uint64_t)nth_value((uint32_t)(head >> 32), n, 0, reach) << 32;
   if (lane == 0) bounds[wv] = mine;
   __syncthreads();
   uint64_t bound = 1;
@@ -299,7 +318,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   for (int u = 0; u < kEach; ++u) {
     if (u * kMergeThreads >= all) break;
     const uint64_t key = key_at[u];
-    const int b = (tid + u * kMergeThreads) / (a.parts * n);
+    const int b = min(quotient(tid + u * kMergeThreads, per_key), a.beams - 1);
     const uint64_t c = key ? total(key, b) : 0;
     if (c >= bound) {
       const int at = atomicAdd(&count, 1);
@@ -441,8 +460,9 @@ int ns_beam_select(const void* logits, int fp32, long long row_stride, const flo
   a.parts = p.parts;
   a.tiles = p.tiles;
   const auto st = static_cast<hipStream_t>(stream);
-  const int reach = std::min(n + ns::kSlack, ns::kWave);
-  const size_t list = ((size_t)n + ns::kWaves * reach * 8 * p.vecs + ns::kAtOnce) * sizeof(uint64_t);  // (up to 41 KB)
+  // as many lanes as may reach a bound, with all of their logits
+  a.segment = std::min(n + ns::kSlack, ns::kWave) * 8 * p.vecs + ns::kAtOnce;
+  const size_t list = (size_t)ns::kWaves * a.segment * sizeof(uint64_t);  // (up to 41 KB)
   const dim3 grid(p.parts, (unsigned)rows);
   const auto rows_kernel = fp32 ? (p.vecs == 2 ? ns::beam_rows_kernel<float, 2> : ns::beam_rows_kernel<float, ns::kMostVecs>)
                                 : (p.vecs == 2 ? ns::beam_rows_kernel<uint16_t, 2>
