@@ -1,7 +1,7 @@
 /*
  * batch_ops.h -- entry points of libnanoserve_amd.so for a batch of sequences over one paged KV
- * cache, which nanoserve_amd/ops.py calls (Kernels.paged_append, paged_attention, sample) and the
- * public headers do not declare. Conventions of include/nanoserve_decode.h: caller-allocated device
+ * cache, which nanoserve_amd/ops.py calls (Kernels.paged_append, paged_attention, their forms for a cache in 8
+ * bits, paged_reserve, beam_select, paged_reorder, sample) and the public headers do not declare. Conventions of include/nanoserve_decode.h: caller-allocated device
  * memory, bf16 tensors as void*, asynchronous on `stream`, no allocation, no host synchronisation,
  * capturable; 0 on success, -2 for rejected arguments (checked before any HIP call), else the
  * hipError_t. The reference serves one sequence at a time (python/nanoserve/qwen.py:113-177) and has

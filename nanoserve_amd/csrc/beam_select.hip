@@ -8,6 +8,9 @@
 //    those from the workgroup's best such bound on can be among its n largest: about as many as are kept. Bounds come
 //    from bit-wise ballots, not from a sort.
 //  * merge: a workgroup per request joins the parts' lists beam by beam, a list to a lane, then the beams' lists.
+// Bound by HBM and by the bounds' and lists' instructions in turn: 16 x 8 beams of 151936 fp32 29.1 us, of them 22.5 the rows
+// (78 MB, 3.5 TB/s) and 5 the merge's latency; 4 beams of 152064 bf16 10.8, two launches' latency. Fewer and larger tiles of a
+// thread (8 vectors) 33.7, smaller ones (2) 47; per-entry counters in LDS instead of ballots 1 us more.
 // Keys are (logit, lowest index first), so equal logits never make a list longer than its bound. Scores are compared
 // in 64 bits: two beams' continuations are often closer than a step of fp32 at their size.
 #include <float.h>

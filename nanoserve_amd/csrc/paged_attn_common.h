@@ -354,15 +354,21 @@ __device__ __forceinline__ u32x2_t lds_read_tr8(const uint16_t* p) {
                                          (__attribute__((address_space(3))) i32x2_t*)const_cast<uint16_t*>(p)));
 }
 
-// s + A B for 32 keys and 32 queries over 64 dims of e4m3, with a power of two per row of either: bytes `ka` of
+// The bits of the four lanes of a quad together.
+__device__ __forceinline__ int quad_or(int v) {
+  v |= __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, false);
+  return v | __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, false);
+}
+
+// s + A B for 32 keys and 32 queries over 64 dims of e4m3, with a power of two per row of either: bytes 2 `ka` of
 // ks and `qa` of qs.
 __device__ __forceinline__ f32x16_t scaled_product(const i32x8_t& k, const i32x8_t& q, const f32x16_t& s, int ka, int ks,
                                                    int qa, int qs) {
   if (ka == 0)
     return qa == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 0, ks, 0, qs)
                    : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 0, ks, 1, qs);
-  return qa == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 1, ks, 0, qs)
-                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 1, ks, 1, qs);
+  return qa == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 2, ks, 0, qs)
+                 : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, q, s, 0, 0, 2, ks, 1, qs);
 }
 
 // A query head's values as two e4m3 terms, x = 2^e (hi + lo / 16). bf16 has the 8 significant bits of two
@@ -425,12 +431,17 @@ __device__ __forceinline__ void query_terms(const u32x4_t& q, int e, u32x2_t& hi
 //    sees are left out of its list, blocks that all rows see whole skip the comparisons. Windows of different
 //    sequences over the shared prefix may lie apart: the positions between them stay in the list, and their rows
 //    are not read but zero, as a value there (it may be NaN) would reach every row through 0 * NaN.
-// Measured (28 / 4 heads of 128): prompts of 5 sequences of 2000 to 8000 654 us, 677 TFLOP/s, with the second term
+// In 8 bits (kF8; paged_attn_fp8.hip): the scores on v_mfma_scale_f32_32x32x64_f8f6f4, codes as they lie in the cache with their
+// scale bytes as operands, queries in two e4m3 terms; the values' codes by ds_read_b64_tr_b8, each wave turning what it
+// reads into bf16 (64 instructions a block beside 24 products; a tile in bf16 that all waves share would save 48 of them for a
+// barrier, LDS writes and twice the reads); one probability term. A stage is half as large.
+// Measured in bf16 (28 / 4 heads of 128): prompts of 5 sequences of 2000 to 8000 654 us, 677 TFLOP/s, with the second term
 // 1015 (a large library product: 1265); matrix cores busy in half of the cycles and vector units in 58 %, at 1.8 GHz,
 // so that products and softmax still take turns for much of the time. Issuing one half block's softmax between the
 // products of its neighbours did not help (659 -> 681 to 730 us). 4095 tokens with a window of 1000 and 14 / 2 heads of
 // 64 43 us. 96 drafts of 1 to 3 tokens behind 16384 shared positions 100 to 104 us back to back, 108 to 117 among
-// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD.
+// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD. In 8 bits: 463 us (955 TFLOP/s),
+// 42 and 94; four stages instead of two level at 128 dims.
 template <int D, bool kShared, bool kF8 = false>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
   // (kRow: a row of the cache in units of 2 bytes)
@@ -562,7 +573,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   // lane i: offset in the pools of 16-row group i % 4 of block j0 + 16 (.. / 16) + i / 4 of the list
   const int* table = a.s.table + (size_t)b * a.s.table_stride;
   uint64_t offs = 0, valid = 0;
-  int scales = kNoScales;  // of the lane's group
+  int k_scales = 0, v_scales = 0;  // of the four groups of the lane's block, a byte each
   auto refill = [&](int j) {
     const int v = j + (lane >> 2);
     int id = -1, key = 0;
@@ -574,8 +585,11 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     }
     valid = __ballot((unsigned)id < (unsigned)a.p.n_pages);
     if constexpr (kF8) {
-      scales = group_scales(a, id, g, key);
-      landed(scales);
+      const int s = group_scales(a, id, g, key), at = 8 * (lane & 3);
+      k_scales = quad_or((s & 0xff) << at);
+      v_scales = quad_or((s >> 8) << at);
+      landed(k_scales);
+      landed(v_scales);
     }
   };
   // (16-byte chunks of a row lie in the order c ^ swz(row), so that the rows of one read hit distinct banks)
@@ -604,14 +618,15 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     }
     return wave_or(bits);
   };
-  auto issue = [&](uint16_t* ks, uint16_t* vs, int j, uint32_t& groups, int (&sc)[4]) {
+  auto issue = [&](uint16_t* ks, uint16_t* vs, int j, uint32_t& groups, int (&sc)[2]) {
     const int jj = j - j0;
     if ((jj & 15) == 0) refill(j);
     const int e = 4 * (jj & 15);
     groups = (uint32_t)(valid >> e) & 15u;
-    if constexpr (kF8)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) sc[u] = __builtin_amdgcn_readlane(scales, e + u);
+    if constexpr (kF8) {
+      sc[0] = __builtin_amdgcn_readlane(k_scales, e);
+      sc[1] = __builtin_amdgcn_readlane(v_scales, e);
+    }
     const int key0 = kTileKeys * kb.block(j) + 16 * wv;
     uint32_t sees = 0xffffu;
     if constexpr (kShared)
@@ -663,12 +678,12 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
       vt[d] = rr * D + 8 * ((4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swz(rr)) + 4 * (lane & 1);
   }
 
-  auto compute = [&](const uint16_t* kt, const uint16_t* vb, int j, uint32_t groups, const int (&sc)[4]) {
+  auto compute = [&](const uint16_t* kt, const uint16_t* vb, int j, uint32_t groups, const int (&sc)[2]) {
     const int key0 = kTileKeys * kb.block(j);
     if (key0 >= hi_max || (key0 + kTileKeys <= lo_min && key0 >= first)) return;  // no row sees it
     f32x16_t s[2];
-    // (scale bytes of this lane's key: of its group in the first 32 keys, then in the second 32)
-    const int kscale = kF8 ? (jq & 16 ? sc[1] & 0xff : sc[0] & 0xff) | (jq & 16 ? sc[3] & 0xff : sc[2] & 0xff) << 8 : 0;
+    // bytes 0 and 2: scales of this lane's key, of its group in the first 32 keys and in the second
+    const int kscale = kF8 ? (int)((uint32_t)sc[0] >> (jq & 16 ? 8 : 0)) : 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -757,7 +772,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
     for (int u = 0; u < 4; ++u) {
       bf16x8_t vf[kDT];
       if constexpr (kF8) {
-        const float scale = __uint_as_float((uint32_t)(sc[u] >> 8) << 23);
+        const float scale = __uint_as_float(((uint32_t)sc[1] >> 8 * u & 0xffu) << 23);
 #pragma unroll
         for (int d = 0; d < kDT; ++d) vf[d] = f8_values(lds_read_tr8(&vb[vt[d] + 16 * u * kRow]), scale, scale);
       }
@@ -780,7 +795,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   // in flight), and past the barrier nobody reads block j - 1, whose stage is loaded next: each wave waits for
   // its loads of j and its reads of j - 1.
   uint32_t gr[kStages];
-  int sg[kStages][4];
+  int sg[kStages][2];
   auto fill = [&](auto stage, int j) {
     constexpr int S = decltype(stage)::value;
     if (j < j1) issue(lds.k[S], lds.v[S], j, gr[S], sg[S]);

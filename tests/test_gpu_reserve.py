@@ -98,7 +98,7 @@ def test_grow_and_shrink(kernels, B, page, most):
             m.check(got, m.change(new, rows))
 
 
-@pytest.mark.parametrize("B,tokens", [(1, 8192), (1, 8193), (40, 1000), (1100, 30)])
+@pytest.mark.parametrize("B,tokens", [(1, 4000), (1, 4200), (1, 8192), (1, 8193), (40, 1000), (1100, 30)])
 def test_many_rows(kernels, B, tokens):
     """Slot maps on both sides of the launch of their own, and one behind which rows are left."""
     m = Model(B, tokens // 16 + 3, 16, B * (tokens // 16 + 3), B * (tokens // 16 + 3), seed=tokens)
