@@ -130,9 +130,10 @@ int ns_paged_attention_fp8(const void* q, long long q_stride, const void* k_pool
  * page * page_size + row, -1 where the table's entry is below 0 and behind the last sequence's (rows -1: no slot map, slots
  * unused); shorts [1]: 0.
  * A call that does not go through as a whole changes nothing: q_start is all 0 (rows of no sequence, on which the operators
- * here do nothing), slots are -1, and shorts is the number of pages that are missing, or -1 where a sequence would pass its
+ * that are given it do nothing; without it they take every sequence's last position for its new one), slots are -1, and shorts is the number of pages that are missing, or -1 where a sequence would pass its
  * table row, more than `rows` tokens are new, or the stack would pass its capacity.
- * Entries given back must not be in use by other rows. -2 for sizes <= 0 (B >= 2^24, rows < -1, capacity < 0 or >= 2^31),
+ * n_free below 0 counts as 0, past the capacity the call does not go through. Entries given back must not be in use by other
+ * rows. -2 for sizes <= 0 (B >= 2^24, rows < -1, capacity < 0 or >= 2^31),
  * page_size % 16, width * page_size >= 2^30, table_stride < width, NULL or misaligned pointers (slots 8, others 4
  * bytes), and any two of the arrays over each other.
  */

@@ -143,29 +143,67 @@ inline Pools scale_pools(const Scales& f, int n_pages) {
   return Pools{reinterpret_cast<uint16_t*>(f.k), reinterpret_cast<uint16_t*>(f.v), f.page_stride, f.head_stride, n_pages, 1};
 }
 
+// Pieces of `size` bytes at all sums of a stride times a number below its count (in bytes, none negative).
+struct Pieces {
+  long long stride[3], count[3];
+  long long size;
+  __int128 span() const {
+    __int128 s = size;
+    for (int i = 0; i < 3; ++i) s += (__int128)stride[i] * (count[i] - 1);
+    return s;
+  }
+};
+
+// Whether the pieces of a and those of b, `d` bytes further on, share no byte. Dimensions of the same stride in both, within
+// which the others stay, are taken out one by one (a shift of either set by a multiple of the stride meets the same
+// pieces); what is left, the heads as a rule, is compared piece by piece, and counts as not apart where that are more than
+// 2^20 comparisons.
+inline bool pieces_apart(Pieces a, Pieces b, __int128 d) {
+  const __int128 sa = a.span(), sb = b.span();
+  if (d >= sa || -d >= sb) return true;
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j) {
+      const long long s = a.stride[i];
+      if (a.count[i] == 1 || s != b.stride[j]) continue;
+      const __int128 na = a.count[i], nb = b.count[j];
+      if (sa - (na - 1) * s > s || sb - (nb - 1) * s > s) continue;
+      Pieces p = a, q = b;
+      p.count[i] = q.count[j] = 1;
+      __int128 r = d % s;
+      if (r < 0) r += s;
+      for (const __int128 at : {r, r - s}) {
+        const __int128 k = (at - d) / s;  // b's number less a's, where the two lie `at` apart
+        if (k > -na && k < nb && !pieces_apart(p, q, at)) return false;
+      }
+      return true;
+    }
+  double work = 1;
+  for (int i = 0; i < 3; ++i) work *= (double)a.count[i] * (double)b.count[i];
+  if (work > (1 << 20)) return false;
+  for (long long i0 = 0; i0 < a.count[0]; ++i0)
+    for (long long i1 = 0; i1 < a.count[1]; ++i1)
+      for (long long i2 = 0; i2 < a.count[2]; ++i2) {
+        const __int128 at = (__int128)i0 * a.stride[0] + (__int128)i1 * a.stride[1] + (__int128)i2 * a.stride[2];
+        for (long long j0 = 0; j0 < b.count[0]; ++j0)
+          for (long long j1 = 0; j1 < b.count[1]; ++j1)
+            for (long long j2 = 0; j2 < b.count[2]; ++j2) {
+              const __int128 e = d - at + (__int128)j0 * b.stride[0] + (__int128)j1 * b.stride[1] + (__int128)j2 * b.stride[2];
+              if (e < a.size && -e < b.size) return false;
+            }
+      }
+  return true;
+}
+
 // Whether a pool's pages (heads of `x` bytes) and another's (of `y`) share no byte. Exact where pages are equally far
 // apart in both; else their spans have to be apart.
 inline bool sets_apart(const void* a, const Pools& p, long long x, const void* b, const Pools& r, long long y, int Hk) {
-  const long long pages = p.n_pages - 1, heads = Hk - 1;
-  const __int128 ap = pages ? (__int128)p.size * p.page_stride : 0, ah = heads ? (__int128)p.size * p.head_stride : 0;
-  const __int128 bp = pages ? (__int128)r.size * r.page_stride : 0, bh = heads ? (__int128)r.size * r.head_stride : 0;
+  auto of = [&](const Pools& q, long long size) {
+    return Pieces{{q.size * q.page_stride, q.size * q.head_stride, 0}, {q.n_pages, Hk, 1}, size};
+  };
+  const Pieces f = of(p, x), g = of(r, y);
   const __int128 d = (__int128)reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a);
-  if (d >= pages * ap + heads * ah + x || -d >= pages * bp + heads * bh + y) return true;
-  if (ap != bp) return false;
-  for (int i = 0; i < Hk; ++i)
-    for (int j = 0; j < Hk; ++j) {
-      // pages m of b and n of a overlap where (m - n) * ap lies in (-y - at, x - at)
-      const __int128 at = d + j * bh - i * ah;
-      if (pages == 0) {
-        if (at > -(__int128)y && at < x) return false;
-        continue;
-      }
-      const __int128 lo = -(__int128)y - at, hi = x - at;
-      __int128 k = lo / ap - (lo % ap < 0) + 1;  // the first k with k * ap > lo
-      if (k < -pages) k = -pages;
-      if (k <= pages && k * ap < hi) return false;
-    }
-  return true;
+  if (d >= f.span() || -d >= g.span()) return true;
+  return (p.n_pages == 1 || f.stride[0] == g.stride[0]) && pieces_apart(f, g, d);
 }
 
 }  // namespace ns

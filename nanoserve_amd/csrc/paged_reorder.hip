@@ -171,24 +171,16 @@ extern "C" int ns_paged_reorder(const int* parents, long long parent_stride, con
                              span(v_scales, marks, scale_layer_stride, scale_page_stride, scale_head_stride)};
   for (const ns::Bytes& p : pools)
     if (!ns::apart(p, y) || !ns::apart(p, z[0]) || !ns::apart(p, z[1]) || !ns::apart(p, z[2])) return -2;
-  // but K's, V's and the scales' pages may lie between each other's
-  auto layer_of = [](const void* p, long long l, long long stride) {
-    return reinterpret_cast<uint16_t*>(reinterpret_cast<uintptr_t>(p) + l * stride);
-  };
-  const ns::Pools f{nullptr, nullptr, page_stride, head_stride, n_pages, 1},
-      g{nullptr, nullptr, scale_page_stride, scale_head_stride, n_pages, 1};
+  // but K's, V's and the scales' pages may lie between each other's, if they are equally far apart
+  const ns::Pieces codes{{layer_stride, page_stride, head_stride}, {layers, n_pages, Hk}, piece},
+      scales{{scale_layer_stride, scale_page_stride, scale_head_stride}, {layers, n_pages, Hk}, marks};
+  const bool together = n_pages == 1 || page_stride == scale_page_stride;
   for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < i; ++j) {
-      if (ns::apart(pools[i], pools[j])) continue;
-      for (int l = 0; l < layers; ++l)
-        for (int m = 0; m < layers; ++m) {
-          const void* all[] = {k_pool, v_pool, k_scales, v_scales};
-          if (!ns::sets_apart(layer_of(all[i], l, i < 2 ? layer_stride : scale_layer_stride), i < 2 ? f : g,
-                              i < 2 ? piece : marks, layer_of(all[j], m, j < 2 ? layer_stride : scale_layer_stride),
-                              j < 2 ? f : g, j < 2 ? piece : marks, Hk))
-            return -2;
-        }
-    }
+    for (int j = 0; j < i; ++j)
+      if (!ns::apart(pools[i], pools[j]) &&
+          (((i < 2) != (j < 2) && !together) || !ns::pieces_apart(i < 2 ? codes : scales, j < 2 ? codes : scales,
+                                                               (__int128)pools[j].lo - pools[i].lo)))
+        return -2;
   ns::ReorderArgs a{};
   a.parents = parents;
   a.table = table;

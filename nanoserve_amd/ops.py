@@ -901,8 +901,8 @@ class Kernels:
         its row there (an index into a pool's positions; -1 for rows behind the last sequence's). ``out``: the three of
         them (slots None without ``rows``), for a captured step.
 
-        The call goes through as a whole or changes nothing: then q_start is 0 throughout, so that the operators on
-        the batch have no rows to work on, and short[0] is the number of pages that were missing, or -1 where a sequence
+        The call goes through as a whole or changes nothing: then q_start is 0 throughout, so that the operators that
+        it is handed on to have no rows to work on (without it they take the last position for a new one), and short[0] is the number of pages that were missing, or -1 where a sequence
         would pass its table row, more tokens are new than rows, or the stack would pass its capacity; else 0. A later
         call that gives back what this one took restores the stack as it was. Pages that another sequence still
         reads (a shared prefix, beams) must not be given back. The reference keeps one sequence in one cache

@@ -342,3 +342,17 @@ def test_argument_types():
                     ("ns_beam_select", 14), ("ns_paged_reorder", 25)):
         assert len(ops.INTERNAL_SIGNATURES[name]) == n
     assert ops.RESTYPES["ns_beam_select_workspace"] is ctypes.c_size_t
+
+
+@on_cpu
+def test_checks_of_layouts_are_quick(lib):
+    """Records of a million pages, many layers and heads, and layouts whose check would be long, which are refused."""
+    import time
+    start = time.perf_counter()
+    n = 1 << 20
+    record = 2 * 80 * 16 * 2048 + 4096
+    assert _reorder(lib, n=n, layers=80, Hk=16, ls=2 * 16 * 2048, ps=record, v=K4 + 16 * 2048, ks=K4 + record - 4096,
+                    vs=K4 + record - 2048, sl=16, sp=record, sh=1, lens=1 << 61, tab=1 << 60, par=1 << 59,
+                    out=1 << 58) not in (0, -2)
+    assert _append(lib, n=n, ps=2048, hs=2048 * n, ks=APPEND["k"] + 2048 * n, sp=2048, sh=2048 * n + 16) == -2
+    assert time.perf_counter() - start < 1.0
