@@ -790,7 +790,7 @@ class Kernels:
         _require_here(v_scales, "v_scales", torch.float8_e8m0fnu, here)
         blocks = page_size // 16
         strides = k_scales.stride()
-        if tuple(k_scales.shape) != (n_pages, Hk, blocks) or (blocks > 1 and strides[2] != 1):
+        if k_scales.shape != (n_pages, Hk, blocks) or (blocks > 1 and strides[2] != 1):
             raise ValueError("k_scales must be [n_pages, Hk, page_size / 16] with contiguous heads")
         if v_scales.shape != k_scales.shape or v_scales.stride() != strides:
             raise ValueError("k_scales and v_scales must be alike")
@@ -908,37 +908,44 @@ class Kernels:
         reads (a shared prefix, beams) must not be given back. The reference keeps one sequence in one cache
         (qwen.py:103-111)."""
         here = _device_of(new, "new", torch.int32)
-        for name, t in (("lens", lens), ("pages", pages), ("free", free), ("n_free", n_free)):
-            _require_here(t, name, torch.int32, here)
-        if new.dim() != 1 or not new.is_contiguous():
+        _require_here(lens, "lens", torch.int32, here)
+        _require_here(pages, "pages", torch.int32, here)
+        _require_here(free, "free", torch.int32, here)
+        _require_here(n_free, "n_free", torch.int32, here)
+        shape = new.shape
+        if len(shape) != 1 or not new.is_contiguous():
             raise ValueError("new must be a contiguous [B] tensor")
-        B = new.shape[0]
-        if tuple(lens.shape) != (B,) or not lens.is_contiguous():
+        B = shape[0]
+        if lens.shape != shape or not lens.is_contiguous():
             raise ValueError(f"lens must be a contiguous [{B}] tensor")
-        if pages.dim() != 2 or pages.shape[0] != B or pages.stride(1) != 1:
+        shape, strides = pages.shape, pages.stride()
+        if len(shape) != 2 or shape[0] != B or strides[1] != 1:
             raise ValueError("pages must be [B, width] with contiguous rows")
+        width = shape[1]
         if free.dim() != 1 or not free.is_contiguous() or n_free.numel() != 1:
             raise ValueError("free must be a contiguous [capacity] tensor and n_free hold one value")
         if rows is not None and rows < 0:
             raise ValueError("rows must not be negative")
-        if out is None:
-            out = (new.new_empty(B + 1), None if rows is None else new.new_empty(rows, dtype=torch.int64), new.new_empty(1))
-        q_start, slots, short = out
-        _require_here(q_start, "q_start", torch.int32, here)
-        _require_here(short, "short", torch.int32, here)
-        if tuple(q_start.shape) != (B + 1,) or not q_start.is_contiguous() or short.numel() != 1:
-            raise ValueError(f"q_start must be a contiguous [{B + 1}] tensor and short hold one value")
-        if rows is not None:
-            _require_here(slots, "slots", torch.int64, here)
-            if tuple(slots.shape) != (rows,) or not slots.is_contiguous():
-                raise ValueError(f"slots must be a contiguous [{rows}] tensor")
-        elif slots is not None:
-            raise ValueError("slots without rows")
         if B == 0:
             raise ValueError("the batch has no sequence")
-        width = pages.shape[1]
+        if out is None:
+            q_start, short = new.new_empty(B + 1), new.new_empty(1)
+            slots = None if rows is None else new.new_empty(rows, dtype=torch.int64)
+            out = (q_start, slots, short)
+        else:
+            q_start, slots, short = out
+            _require_here(q_start, "q_start", torch.int32, here)
+            _require_here(short, "short", torch.int32, here)
+            if q_start.shape != (B + 1,) or not q_start.is_contiguous() or short.numel() != 1:
+                raise ValueError(f"q_start must be a contiguous [{B + 1}] tensor and short hold one value")
+            if rows is not None:
+                _require_here(slots, "slots", torch.int64, here)
+                if slots.shape != (rows,) or not slots.is_contiguous():
+                    raise ValueError(f"slots must be a contiguous [{rows}] tensor")
+            elif slots is not None:
+                raise ValueError("slots without rows")
         rc = self.lib.ns_paged_reserve(
-            new.data_ptr(), lens.data_ptr(), pages.data_ptr(), pages.stride(0) if B > 1 else width, width,
+            new.data_ptr(), lens.data_ptr(), pages.data_ptr(), strides[0] if B > 1 else width, width,
             free.data_ptr(), free.shape[0], n_free.data_ptr(), q_start.data_ptr(),
             None if slots is None else slots.data_ptr(), -1 if rows is None else rows, short.data_ptr(), B, page_size,
             _raw_stream(here))
@@ -964,15 +971,19 @@ class Kernels:
         dtype = torch.float8_e4m3fn if fp8 else torch.bfloat16
         _require_here(k_pages, "k_pages", dtype, here)
         _require_here(v_pages, "v_pages", dtype, here)
-        if parents.dim() != 2 or (parents.shape[1] > 1 and parents.stride(1) != 1):
+        shape, strides = parents.shape, parents.stride()
+        if len(shape) != 2 or (shape[1] > 1 and strides[1] != 1):
             raise ValueError("parents must be [R, beams] with contiguous rows")
-        R, beams = parents.shape
-        rows = R * beams
-        if pages.dim() != 2 or pages.shape[0] != rows or pages.stride(1) != 1:
+        R, beams = shape
+        rows, parent_stride = R * beams, strides[0] if R > 1 else beams
+        shape, strides = pages.shape, pages.stride()
+        if len(shape) != 2 or shape[0] != rows or strides[1] != 1:
             raise ValueError(f"pages must be [{rows}, width] with contiguous rows")
-        if tuple(lens.shape) != (rows,) or not lens.is_contiguous():
+        width = shape[1]
+        table_stride = strides[0] if rows > 1 else width
+        if lens.shape != (rows,) or not lens.is_contiguous():
             raise ValueError(f"lens must be a contiguous [{rows}] tensor")
-        shape, strides = tuple(k_pages.shape), k_pages.stride()
+        shape, strides = k_pages.shape, k_pages.stride()
         if len(shape) not in (4, 5) or strides[-1] != 1 or strides[-2] != shape[-1]:
             raise ValueError("k_pages must be [n_pages, Hk, page_size, D], or that for all layers, with contiguous heads")
         if v_pages.shape != k_pages.shape or v_pages.stride() != strides:
@@ -981,35 +992,34 @@ class Kernels:
             shape, strides = (1, *shape), (0, *strides)
         layers, n_pages, Hk, page_size, D = shape
         size = 1 if fp8 else 2
-        by = tuple(size * s if n > 1 else 0 for s, n in zip(strides[:3], shape[:3]))
+        by = (size * strides[0] if layers > 1 else 0, size * strides[1] if n_pages > 1 else 0,
+              size * strides[2] if Hk > 1 else 0)
         marks = (None, None, 0, 0, 0)
         if fp8:
             _require_here(k_scales, "k_scales", torch.float8_e8m0fnu, here)
             _require_here(v_scales, "v_scales", torch.float8_e8m0fnu, here)
             strides = k_scales.stride()
-            if tuple(k_scales.shape) != (*k_pages.shape[:-2], page_size // 16) or (page_size > 16 and strides[-1] != 1):
+            if k_scales.shape != (*k_pages.shape[:-2], page_size // 16) or (page_size > 16 and strides[-1] != 1):
                 raise ValueError("k_scales must be [n_pages, Hk, page_size / 16] (for all layers, as the pages) with "
                                  "contiguous heads")
             if v_scales.shape != k_scales.shape or v_scales.stride() != strides:
                 raise ValueError("k_scales and v_scales must be alike")
             if len(strides) == 3:
                 strides = (0, *strides)
-            marks = (k_scales.data_ptr(), v_scales.data_ptr(),
-                     *(s if n > 1 else 0 for s, n in zip(strides[:3], shape[:3])))
+            marks = (k_scales.data_ptr(), v_scales.data_ptr(), strides[0] if layers > 1 else 0,
+                     strides[1] if n_pages > 1 else 0, strides[2] if Hk > 1 else 0)
         elif v_scales is not None:
             raise ValueError("v_scales without k_scales")
-        width = pages.shape[1]
         if out is None:
             out = pages.new_empty((rows, width))
         else:
             _require_here(out, "out", torch.int32, here)
-            if tuple(out.shape) != (rows, width) or not out.is_contiguous():
+            if out.shape != (rows, width) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{rows}, {width}] tensor")
         if rows == 0:
             return out
         rc = self.lib.ns_paged_reorder(
-            parents.data_ptr(), parents.stride(0) if R > 1 else beams, pages.data_ptr(),
-            pages.stride(0) if rows > 1 else width, width, lens.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
+            parents.data_ptr(), parent_stride, pages.data_ptr(), table_stride, width, lens.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
             v_pages.data_ptr(), *by, *marks, layers, n_pages, page_size, size * D, R, beams, Hk, _raw_stream(here))
         self._check(rc, "ns_paged_reorder")
         return out
