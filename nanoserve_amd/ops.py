@@ -924,8 +924,10 @@ class Kernels:
         width = shape[1]
         if free.dim() != 1 or not free.is_contiguous() or n_free.numel() != 1:
             raise ValueError("free must be a contiguous [capacity] tensor and n_free hold one value")
-        if rows is not None and rows < 0:
-            raise ValueError("rows must not be negative")
+        if rows is not None and rows >> 31:  # below 0 or past the library's 32 bits
+            raise ValueError("rows must be within 0 .. 2^31 - 1")
+        if (page_size | width) >> 31:
+            raise ValueError("page_size and the width of pages must be within 32 bits")
         if B == 0:
             raise ValueError("the batch has no sequence")
         if out is None:
@@ -992,6 +994,8 @@ class Kernels:
             shape, strides = (1, *shape), (0, *strides)
         layers, n_pages, Hk, page_size, D = shape
         size = 1 if fp8 else 2
+        if (width | n_pages | page_size | size * D) >> 31:
+            raise ValueError("the width of pages and the sizes of a page must be within 32 bits")
         by = (size * strides[0] if layers > 1 else 0, size * strides[1] if n_pages > 1 else 0,
               size * strides[2] if Hk > 1 else 0)
         marks = (None, None, 0, 0, 0)
@@ -1028,7 +1032,7 @@ class Kernels:
     def beam_select_workspace(self, R, beams, vocab, n, dtype=torch.bfloat16, device=None):
         """A uint8 device tensor of the workspace beam_select uses for these sizes. Launches that may overlap in time need
         workspaces of their own."""
-        size = int(self.lib.ns_beam_select_workspace(R, beams, vocab, n))
+        size = int(self.lib.ns_beam_select_workspace(_int32(R), _int32(beams), _int32(vocab), _int32(n)))
         return torch.empty(size, dtype=torch.uint8, device=device or "cuda") if size else None
 
     def beam_select(self, logits, scores, n, work=None, out=None):
@@ -1052,6 +1056,8 @@ class Kernels:
         if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] != R * beams:
             raise ValueError(f"logits must be [{R * beams}, vocab] with contiguous rows")
         V = logits.shape[1]
+        if (n | V) >> 31:  # (the library's arguments would keep the low bits alone)
+            raise ValueError("n and the vocabulary must be within 32 bits")
         if out is None:
             out = (scores.new_empty((R, n)), scores.new_empty((R, n), dtype=torch.int32),
                    scores.new_empty((R, n), dtype=torch.int32))

@@ -292,6 +292,24 @@ def test_reserve_wrapper_refuses(stub, bad):
     assert not stub.lib.calls
 
 
+@pytest.mark.parametrize("bad", [dict(page_size=(1 << 32) + 16), dict(page_size=-16), dict(rows=1 << 31)], ids=str)
+def test_reserve_sizes_past_32_bits(stub, bad):
+    """Sizes whose low bits would pass."""
+    with pytest.raises(ValueError):
+        _room(stub, **bad)
+    assert not stub.lib.calls
+
+
+def test_select_sizes_past_32_bits(stub):
+    a = dict(logits=torch.zeros(12, 50), scores=torch.zeros(3, 4), n=8)
+    for bad in (dict(n=(1 << 32) + 8), dict(n=-1)):
+        with pytest.raises(ValueError):
+            stub.beam_select(**{**a, **bad})
+    assert not stub.lib.calls
+    stub.beam_select_workspace(3, 4, 50, (1 << 32) + 8, device="cpu")
+    assert stub.lib.calls["ns_beam_select_workspace"] == (3, 4, 50, (1 << 31) - 1)
+
+
 def test_reserve_wrapper_hands_over(stub):
     q, slots, short = _room(stub)
     assert q.shape == (4,) and slots.shape == (10,) and slots.dtype == torch.int64 and short.shape == (1,)
