@@ -655,15 +655,17 @@ class Kernels:
         _require_here(lens, "lens", torch.int32, here)
         _require_here(k_pages, "k_pages", dtype, here)
         _require_here(v_pages, "v_pages", dtype, here)
+        # (shapes and strides are read once: 0.2 us each, beside a launch of 4)
         shape, strides = k_pages.shape, k_pages.stride()
         if len(shape) != 4 or strides[3] != 1 or strides[2] != shape[3]:
             raise ValueError("k_pages must be [n_pages, Hk, page_size, D] with contiguous heads")
         if v_pages.shape != shape or v_pages.stride() != strides:
             raise ValueError("k_pages and v_pages must be alike")
+        rows, steps = pages.shape, pages.stride()
         if lens.dim() != 1 or not lens.is_contiguous():
             raise ValueError("lens must be a contiguous [B] tensor")
-        B = lens.shape[0]
-        if pages.dim() != 2 or pages.shape[0] != B or pages.stride(1) != 1:
+        B = lens.numel()
+        if len(rows) != 2 or rows[0] != B or steps[1] != 1:
             raise ValueError("pages must be [B, width] with contiguous rows")
         if q_start is None:
             if T != B:
@@ -673,11 +675,11 @@ class Kernels:
             if q_start.dim() != 1 or q_start.shape[0] != B + 1 or not q_start.is_contiguous():
                 raise ValueError("q_start must be a contiguous [B + 1] tensor")
         n_pages, Hk, page_size, D = shape
-        width = pages.shape[1]
+        width = rows[1]
         # (the stride of a dimension of size 1 says nothing)
         return (B, Hk, D, page_size, n_pages,
                 (strides[0] if n_pages > 1 else 0, strides[1] if Hk > 1 else 0),
-                (pages.data_ptr(), pages.stride(0) if B > 1 else width, width))
+                (pages.data_ptr(), steps[0] if B > 1 else width, width))
 
     def paged_append(self, qkv, bias, inv_freq, pages, lens, k_pages, v_pages, n_heads, q_start=None,
                      out=None):
@@ -810,9 +812,10 @@ class Kernels:
         Everything else as paged_append; rows of the pages that no new token writes keep their values."""
         here = _device_of(qkv, "qkv", torch.bfloat16)
         _require_here(inv_freq, "inv_freq", torch.float32, here)
-        if qkv.dim() != 2 or qkv.stride(1) != 1:
+        shape, steps = qkv.shape, qkv.stride()
+        if len(shape) != 2 or steps[1] != 1:
             raise ValueError("qkv must be [T, (Hq + 2Hk) * D] with contiguous rows")
-        T, columns = qkv.shape
+        T, columns = shape
         B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
                                                                         q_start, here, torch.float8_e4m3fn)
         scales = self._scale_args(k_scales, v_scales, n_pages, Hk, page_size, here)
@@ -828,18 +831,19 @@ class Kernels:
             out = qkv.new_empty((T, n_heads * D))
         else:
             _require_here(out, "out", torch.bfloat16, here)
-            if tuple(out.shape) != (T, n_heads * D) or not out.is_contiguous():
+            if out.shape != (T, n_heads * D) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{T}, {n_heads * D}] tensor")
-            _apart(out, qkv, "qkv")
         if T == 0 or B == 0:
             return out
         rc = self.lib.ns_paged_append_fp8(
-            qkv.data_ptr(), qkv.stride(0) if T > 1 else columns,
+            qkv.data_ptr(), steps[0] if T > 1 else columns,
             None if bias is None else bias.data_ptr(), inv_freq.data_ptr(),
             None if q_start is None else q_start.data_ptr(), lens.data_ptr(), *table, k_pages.data_ptr(),
             v_pages.data_ptr(), *strides, *scales, n_pages, page_size, out.data_ptr(), T, B, n_heads, Hk, D,
             _raw_stream(here))
-        self._check(rc, "ns_paged_append_fp8")
+        if rc:
+            _apart(out, qkv, "qkv")  # (says so; the library has refused it)
+            self._check(rc, "ns_paged_append_fp8")
         return out
 
     def paged_attention_fp8_workspace(self, T, B, n_heads, n_kv_heads, head_dim, max_len, ragged=False,
@@ -857,9 +861,10 @@ class Kernels:
         held to 2^-22 of it, and probabilities: with q_start, over a shared prefix and for more than 16 query heads per kv head
         they are rounded to bf16 before they weigh the values. ``work``: from paged_attention_fp8_workspace."""
         here = _device_of(q, "q", torch.bfloat16)
-        if q.dim() != 2 or q.stride(1) != 1:
+        shape, steps = q.shape, q.stride()
+        if len(shape) != 2 or steps[1] != 1:
             raise ValueError("q must be [T, Hq * D] with contiguous rows")
-        T, columns = q.shape
+        T, columns = shape
         B, Hk, D, page_size, n_pages, strides, table = self._batch_args(T, pages, lens, k_pages, v_pages,
                                                                         q_start, here, torch.float8_e4m3fn)
         scales = self._scale_args(k_scales, v_scales, n_pages, Hk, page_size, here)
@@ -869,9 +874,8 @@ class Kernels:
             out = q.new_empty((T, columns))
         else:
             _require_here(out, "out", torch.bfloat16, here)
-            if tuple(out.shape) != (T, columns) or not out.is_contiguous():
+            if out.shape != (T, columns) or not out.is_contiguous():
                 raise ValueError(f"out must be a contiguous [{T}, {columns}] tensor")
-            _apart(out, q, "q")
         if T == 0 or B == 0:
             return out
         if (shared | window | sinks) >> 31:  # one below 0 or past 32 bits
@@ -884,12 +888,14 @@ class Kernels:
             if not work.is_contiguous():
                 raise _strided_work()
         rc = self.lib.ns_paged_attention_fp8(
-            q.data_ptr(), q.stride(0) if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
+            q.data_ptr(), steps[0] if T > 1 else columns, k_pages.data_ptr(), v_pages.data_ptr(),
             *strides, *scales, n_pages, page_size, *table, lens.data_ptr(),
             None if q_start is None else q_start.data_ptr(), out.data_ptr(),
             None if work is None else work.data_ptr(), 0 if work is None else work.numel(), T, B, n_heads,
             Hk, D, shared, window, sinks, D ** -0.5 if scale is None else scale, _raw_stream(here))
-        self._check(rc, "ns_paged_attention_fp8")
+        if rc:
+            _apart(out, q, "q")
+            self._check(rc, "ns_paged_attention_fp8")
         return out
 
     def paged_reserve(self, new, lens, pages, free, n_free, page_size, rows=None, out=None):
@@ -1053,9 +1059,10 @@ class Kernels:
         if scores.dim() != 2 or not scores.is_contiguous():
             raise ValueError("scores must be a contiguous [R, beams] tensor")
         R, beams = scores.shape
-        if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[0] != R * beams:
+        shape, steps = logits.shape, logits.stride()
+        if len(shape) != 2 or steps[1] != 1 or shape[0] != R * beams:
             raise ValueError(f"logits must be [{R * beams}, vocab] with contiguous rows")
-        V = logits.shape[1]
+        V = shape[1]
         if (n | V) >> 31:  # (the library's arguments would keep the low bits alone)
             raise ValueError("n and the vocabulary must be within 32 bits")
         if out is None:
@@ -1064,7 +1071,7 @@ class Kernels:
         else:
             for t, name, dtype in zip(out, ("scores", "tokens", "parents"), (torch.float32, torch.int32, torch.int32)):
                 _require_here(t, "out " + name, dtype, here)
-                if tuple(t.shape) != (R, n) or not t.is_contiguous():
+                if t.shape != (R, n) or not t.is_contiguous():
                     raise ValueError(f"out {name} must be a contiguous [{R}, {n}] tensor")
         if R == 0:
             return out
@@ -1074,7 +1081,7 @@ class Kernels:
             _require_here(work, "work", torch.uint8, here)
             if not work.is_contiguous():
                 raise _strided_work()
-        rc = self.lib.ns_beam_select(logits.data_ptr(), int(fp32), logits.stride(0) if R * beams > 1 else V,
+        rc = self.lib.ns_beam_select(logits.data_ptr(), int(fp32), steps[0] if R * beams > 1 else V,
                                      scores.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
                                      None if work is None else work.data_ptr(), 0 if work is None else work.numel(), R,
                                      beams, V, n, _raw_stream(here))

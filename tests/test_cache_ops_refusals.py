@@ -1,6 +1,7 @@
 """Calls of the 8-bit cache's, the page reservation's and beam search's operators that the entry points and wrappers
 refuse before a launch, and ones that they take (no GPU)."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -259,6 +260,18 @@ def test_cache_wrappers_refuse(stub, call, bad):
     with pytest.raises((ValueError, TypeError)):
         call(stub, **bad)
     assert not any(not n.endswith("_workspace") for n in stub.lib.calls)
+
+
+@pytest.mark.parametrize("call, name, columns", [(_attend, "q", 512), (_add, "qkv", 1024)])
+def test_what_the_library_refuses(stub, call, name, columns):
+    """An output over the input is named, anything else has the library's code."""
+    stub.lib = types.SimpleNamespace(ns_paged_append_fp8=lambda *a: -2, ns_paged_attention_fp8=lambda *a: -2,
+                                     ns_paged_attention_fp8_workspace=lambda *a: 64)
+    x, work = _z(3, columns, dtype=BF16), dict(work=torch.zeros(64, dtype=torch.uint8)) if call is _attend else {}
+    with pytest.raises(ValueError, match="overlap"):
+        call(stub, **{name: x, "out": x.view(-1)[:3 * 512].view(3, 512)}, **work)
+    with pytest.raises(RuntimeError, match="-2"):
+        call(stub, **{name: x, "out": _z(3, 512, dtype=BF16)}, **work)
 
 
 def test_attention_workspace_must_be_contiguous(stub):
