@@ -4,13 +4,15 @@
 //
 // Within a beam the order is that of its logits, so the rows are read once and nothing of their length is written:
 //  * rows: a workgroup takes a part of one row, keeps the part's n largest logits and its maximum and sum of
-//    exponentials. The n-th largest of a wave's 64 lane maxima is reached by n logits of that wave, so only
-//    those from the workgroup's best such bound on can be among its n largest: about as many as are kept. Bounds come
-//    from bit-wise ballots, not from a sort.
-//  * merge: a workgroup per request joins the parts' lists beam by beam, a list to a lane, then the beams' lists.
-// Bound by HBM and by the bounds' and lists' instructions in turn: 16 x 8 beams of 151936 fp32 29.1 us, of them 22.5 the rows
-// (78 MB, 3.5 TB/s) and 5 the merge's latency; 4 beams of 152064 bf16 10.8, two launches' latency. Fewer and larger tiles of a
-// thread (8 vectors) 33.7, smaller ones (2) 47; per-entry counters in LDS instead of ballots 1 us more.
+//    exponentials. The n-th largest of a tile's 256 thread maxima is reached by n logits of that tile, so only
+//    those from it on can be among its n largest: hardly more than are kept. Bounds come from bit-wise ballots, not from a
+//    sort, and every wave finds the workgroup's by itself from LDS: each wave's own n-th of 64 lets three times as many
+//    logits through, and of n = 64 nearly all (4 beams of 152064 with n 64 302 us, 24 now; 16 x 8 beams 27.2, 25.7).
+//  * merge: a workgroup per request bounds the parts' lists the same way, by entry `depth` of each, and orders what is left
+//    by rank; lists of many equal sums are joined beam by beam, a list to a lane, then the beams' lists.
+// Bound by HBM and by the bounds' and lists' instructions in turn: 16 x 8 beams of 151936 fp32 25.7 us, of them 19.7 the rows
+// (78 MB, 4.0 TB/s) and 5 the merge's latency; 4 beams of 152064 bf16 10.7, two launches' latency. Tiles of 2 vectors
+// to a thread take 37.7 for the 16 x 8, of 8 more registers than five workgroups of a CU have.
 // Keys are (logit, lowest index first), so equal logits never make a list longer than its bound. Scores are compared
 // in 64 bits: two beams' continuations are often closer than a step of fp32 at their size.
 #include <float.h>
@@ -29,9 +31,10 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
 constexpr int kMostVecs = 4;                     // vectors of 8 logits of a thread in a tile
-constexpr int kMostBeams = 64, kMostKept = 64;   // a list to a lane, and a bound from 64 lane maxima
+constexpr int kMostBeams = 64, kMostKept = 64;   // a list to a lane
 constexpr int kMostParts = 64;
-constexpr int kSlack = 4;                        // lanes beyond n that may reach a bound
+// Threads (in the merge: lists) beyond n that may reach a bound. us with 2, 4 and 8: 8 x 8 beams of 151936 bf16 21.8, 17.1, 17.6.
+constexpr int kSlack = 4;
 constexpr int kAtOnce = 8;                       // comparisons whose operands are loaded together
 static_assert(kWaves == 4, "the end of beam_rows_kernel");
 constexpr int kMostKeys = 12288;                 // keys of all parts of a request in the merge's LDS
@@ -62,19 +65,33 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// A value that n of the wave's lanes reach (0: fewer than n are not 0), and how many reach it: at most `slack` more, or
-// as many as are equal to the n-th. Searched from the highest bit in which lanes differ.
-__device__ __forceinline__ uint32_t nth_value(uint32_t high, int n, int slack, int& reach) {
-  reach = __popcll(__ballot(high != 0));
+// How many of the lanes' values, `groups` each, reach x.
+template <int N>
+__device__ __forceinline__ int reach_of(const uint32_t (&h)[N], int groups, uint32_t x) {
+  int k = 0;
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+    if (u < groups) k += __popcll(__ballot(h[u] >= x));
+  return k;
+}
+
+// A value that n of the lanes' values reach (0: fewer than n are not 0), and how many reach it: at most `slack` more, or
+// as many as are equal to the n-th. Searched from the highest bit in which they differ. most: the largest.
+template <int N>
+__device__ __forceinline__ uint32_t nth_value(const uint32_t (&h)[N], int groups, int n, int slack, uint32_t most, int& reach) {
+  reach = reach_of(h, groups, 1);
   if (reach < n) return 0;
-  const uint32_t most = wave_umax(high), least = ~wave_umax(~high);
+  uint32_t down = 0;
+#pragma unroll
+  for (int u = 0; u < N; ++u) down = max(down, h[u] ? ~h[u] : 0);
+  const uint32_t least = ~wave_umax(down);
+  if (reach <= n + slack) return least;
   int bit = most == least ? -1 : 31 - __builtin_clz(most ^ least);
   uint32_t at = bit < 0 ? most : most & ~((2u << bit) - 1u);
-  reach = kWave;
 #pragma unroll 1
   for (; bit >= 0; --bit) {
     const uint32_t next = at | 1u << bit;
-    const int k = __popcll(__ballot(high >= next));
+    const int k = reach_of(h, groups, next);
     if (k < n) continue;
     at = next;
     reach = k;
@@ -83,15 +100,17 @@ __device__ __forceinline__ uint32_t nth_value(uint32_t high, int n, int slack, i
   return at;
 }
 
-// Of lanes whose keys differ in the low half: a key that n lanes reach, and no more than n, where more than n reach `at`.
-__device__ __forceinline__ uint64_t nth_key(uint64_t key, uint32_t at, int n) {
-  const uint32_t high = (uint32_t)(key >> 32);
-  const int more = __popcll(__ballot(high > at));
+// Of keys that differ in the low half: one that n of the lanes' keys reach, and no more than n, where more than n reach `at`.
+template <int N>
+__device__ __forceinline__ uint64_t nth_key(const uint64_t (&key)[N], uint32_t at, int n) {
   uint32_t low = 0;
 #pragma unroll 1
   for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t next = low | 1u << bit;
-    if (more + __popcll(__ballot(high == at && (uint32_t)key >= next)) >= n) low = next;
+    const uint64_t next = (uint64_t)at << 32 | low | 1u << bit;
+    int k = 0;
+#pragma unroll
+    for (int u = 0; u < N; ++u) k += __popcll(__ballot(key[u] >= next));
+    if (k >= n) low = (uint32_t)next;
   }
   return (uint64_t)at << 32 | low;
 }
@@ -115,11 +134,11 @@ __device__ __forceinline__ double wave_total(double v) {
 }
 
 template <typename E, int kVecs>
-__global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) beam_rows_kernel(BeamArgs a) {
   extern __shared__ uint64_t list[];  // a.segment for each wave: keys, and kAtOnce of 0
-  __shared__ uint64_t bounds[kWaves], kept[2][kMostKept + kAtOnce];
+  __shared__ uint64_t kept[2][kMostKept + kAtOnce], bests[kThreads];
   __shared__ int counts[kWaves];
-  __shared__ uint32_t tops[kWaves];
+  __shared__ uint32_t tops[kThreads];
   __shared__ double red_s[kWaves];
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const long long r = blockIdx.y;
@@ -158,29 +177,32 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
     auto key_at = [&](int j, int e) {
       return (uint64_t)key_of(x[j][e] + 0.f) << 32 | ~(uint32_t)(row.first(v0 + j * kThreads) + e);
     };
-    const uint32_t high = top > -INFINITY ? key_of(top + 0.f) : 0;
-    int reach;
-    uint64_t bound = (uint64_t)nth_value(high, n, kSlack, reach) << 32;
-    if (reach > n + kSlack) {  // many equal ones: by index too, from each lane's largest at its first place
-      uint64_t best = 0;
-#pragma unroll
-      for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) best = max(best, x[j][e] == top ? key_at(j, e) : 0);
-      bound = nth_key(top > -INFINITY ? best : 0, (uint32_t)(bound >> 32), n);
-    }
-    if (have == n) bound = max(bound, kept[now][n - 1] + 1);
-    const uint32_t wave_top = wave_umax(high);
-    if (lane == 0) {
-      bounds[wv] = bound;
-      tops[wv] = wave_top;
-    }
+    // The bound, which every wave finds by itself from all threads' largest
+    tops[tid] = top > -INFINITY ? key_of(top + 0.f) : 0;
     __syncthreads();
-    uint32_t most = 0;
+    uint32_t h[kWaves], most = 0;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      bound = max(bound, bounds[k]);
-      most = max(most, tops[k]);
+    for (int k = 0; k < kWaves; ++k) most = max(most, h[k] = tops[k * kWave + lane]);
+    most = wave_umax(most);
+    uint64_t bound = have == n ? kept[now][n - 1] + 1 : 0;
+    if (have < n || reach_of(h, kWaves, (uint32_t)(bound >> 32)) > n + kSlack) {
+      int reach;
+      const uint32_t nth = nth_value(h, kWaves, n, kSlack, most, reach);
+      uint64_t by_nth = (uint64_t)nth << 32;
+      if (reach > n + kSlack) {  // many equal ones: by index too, from each thread's largest at its first place
+        uint64_t best = 0;
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) best = max(best, x[j][e] == top ? key_at(j, e) : 0);
+        bests[tid] = top > -INFINITY ? best : 0;
+        __syncthreads();  // (all waves have found the same)
+        uint64_t f[kWaves];
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) f[k] = bests[k * kWave + lane];
+        by_nth = nth_key(f, nth, n);
+      }
+      bound = max(bound, by_nth);
     }
     const float least = bound >> 32 ? value_of((uint32_t)(bound >> 32)) : -FLT_MAX;
     int mine = 0;  // keys of the wave's segment: counted by ballots, so that no wave waits for a counter
@@ -201,7 +223,10 @@ __global__ void __launch_bounds__(kThreads) beam_rows_kernel(BeamArgs a) {
     if (most != 0) {
       const float mt = fmaxf(m, value_of(most));
       if (mt != m) {
-        sum = m == -INFINITY ? 0. : sum * exp((double)m - mt);
+        // exp(m - mt) in 32 bits, the product's rounding put right (exp of a double takes 20 registers more)
+        const float d = fmaxf(m - mt, -200.f), up = d * 1.44269504f, rest = fmaf(d, 1.44269504f, -up) + d * 1.92596299e-8f;
+        const float f = __builtin_amdgcn_exp2f(up);
+        sum = m == -INFINITY ? 0. : sum * (double)fmaf(f, rest * 0.69314718f, f);
         m = mt;
       }
       float s = 0.f;
@@ -267,13 +292,15 @@ __device__ __forceinline__ uint64_t order_of(double x) {
 }
 
 constexpr int kMergeThreads = 512;
+constexpr int kGroups = kMergeThreads / kWave;
+constexpr int kUnbounded = 128;  // so many keys are ordered as they are (4 x 4 beams of 4000 9.1 us, with a bound 11.6)
 constexpr int kMostRanked = kMergeThreads;  // continuations that are ordered by rank, one to a thread
 constexpr int kEach = kMostKeys / kMergeThreads;
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   extern __shared__ uint64_t lds[];  // [beams][parts][n], then [beams][n]
   __shared__ double base[kMostBeams];
-  __shared__ uint64_t bounds[kMergeThreads / kWave];
+  __shared__ uint32_t heads[kMergeThreads];
   // the sum's order, and what decides between equal sums: beam (6 bits, complement), logit key (32), index (20, complement)
   __shared__ __align__(16) ulonglong2 found[kMostRanked + kAtOnce];
   __shared__ int count;
@@ -285,9 +312,12 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   // error), where an integer division takes ten times the instructions
   const float per_list = 1.f / a.parts, per_key = 1.f / (a.parts * n);
   auto quotient = [](int i, float per) { return (int)(((float)i + 0.5f) * per); };
+  // entry `depth` of `need` lists is reached by n continuations; both so that half of the lists are enough
+  const int depth = min(n, (2 * n + lists - 1) / lists), need = (n + depth - 1) / depth;
+  const uint64_t* entry = keys + depth - 1;
   uint64_t first[2], key_at[kEach];  // of the lane's lists; of its share of all keys
 #pragma unroll
-  for (int u = 0; u < 2; ++u) first[u] = tid + u * kMergeThreads < lists ? keys[(size_t)(tid + u * kMergeThreads) * n] : 0;
+  for (int u = 0; u < 2; ++u) first[u] = tid + u * kMergeThreads < lists ? entry[(size_t)(tid + u * kMergeThreads) * n] : 0;
 #pragma unroll
   for (int u = 0; u < kEach; ++u) {
     if (u * kMergeThreads >= all) break;
@@ -304,19 +334,24 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   __syncthreads();
   auto total = [&](uint64_t key, int b) { return key ? order_of(base[b] + value_of((uint32_t)(key >> 32))) : 0; };
 
-  // A bound that n continuations reach: of the lists' first ones, a list to a lane (or several: their largest)
-  uint64_t head = 0;
-#pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (first[u]) head = max(head, total(first[u], quotient(tid + u * kMergeThreads, per_list)));
-  for (int i = tid + 2 * kMergeThreads; i < lists; i += kMergeThreads) head = max(head, total(keys[(size_t)i * n], quotient(i, per_list)));
-  int reach;
-  const uint64_t mine = (uint64_t)nth_value((uint32_t)(head >> 32), n, 0, reach) << 32;
-  if (lane == 0) bounds[wv] = mine;
-  __syncthreads();
+  // A bound that n continuations reach: of the lists' entries, a list to a thread (or several: their largest)
   uint64_t bound = 1;
+  if (all > kUnbounded) {
+    uint64_t head = 0;
 #pragma unroll
-  for (int k = 0; k < kMergeThreads / kWave; ++k) bound = max(bound, bounds[k]);
+    for (int u = 0; u < 2; ++u)
+      if (first[u]) head = max(head, total(first[u], quotient(tid + u * kMergeThreads, per_list)));
+    for (int i = tid + 2 * kMergeThreads; i < lists; i += kMergeThreads) head = max(head, total(entry[(size_t)i * n], quotient(i, per_list)));
+    heads[tid] = (uint32_t)(head >> 32);
+    __syncthreads();
+    const int groups = (min(lists, kMergeThreads) + kWave - 1) / kWave;
+    uint32_t h[kGroups], most = 0;
+#pragma unroll
+    for (int u = 0; u < kGroups; ++u) most = max(most, h[u] = u < groups ? heads[u * kWave + lane] : 0);
+    int reach;
+    // (to the last bit where lists are few: another one that reaches the bound may bring all of its entries)
+    bound = max((uint64_t)nth_value(h, groups, need, depth > 1 ? -1 : kSlack, wave_umax(most), reach) << 32, bound);
+  }
 #pragma unroll
   for (int u = 0; u < kEach; ++u) {
     if (u * kMergeThreads >= all) break;
@@ -382,7 +417,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(BeamArgs a) {
   const int b = min(lane, a.beams - 1);
   const uint64_t* list = best + b * n;
   uint64_t key = lane < a.beams ? list[0] : 0;
-  head = total(key, b);
+  uint64_t head = total(key, b);
   int at = 0;
   for (int k = 0; k < n; ++k) {
     const int w = wave_best(head);
@@ -463,9 +498,9 @@ int ns_beam_select(const void* logits, int fp32, long long row_stride, const flo
   a.parts = p.parts;
   a.tiles = p.tiles;
   const auto st = static_cast<hipStream_t>(stream);
-  // as many lanes as may reach a bound, with all of their logits
+  // as many threads as may reach a bound, with all of their logits
   a.segment = std::min(n + ns::kSlack, ns::kWave) * 8 * p.vecs + ns::kAtOnce;
-  const size_t list = (size_t)ns::kWaves * a.segment * sizeof(uint64_t);  // (up to 41 KB)
+  const size_t list = (size_t)ns::kWaves * a.segment * sizeof(uint64_t);  // (up to 37 KB)
   const dim3 grid(p.parts, (unsigned)rows);
   const auto rows_kernel = fp32 ? (p.vecs == 2 ? ns::beam_rows_kernel<float, 2> : ns::beam_rows_kernel<float, ns::kMostVecs>)
                                 : (p.vecs == 2 ? ns::beam_rows_kernel<uint16_t, 2>

@@ -139,6 +139,35 @@ def test_select_far_scores(kernels):
     _check(kernels, _logits(32, 30000, torch.float32, 5), scores, 16)
 
 
+def test_select_maxima_that_rise(kernels):
+    """Rows in parts of several tiles whose maximum rises from tile to tile, a little or by more than fp32 holds; and beams
+    that do not count beside them."""
+    beams, n, V = 16, 32, 152064
+    x = _logits(beams, V, torch.float32, 21)
+    at = torch.arange(V, device="cuda", dtype=torch.float32)
+    x[0] = at * (60 / V)
+    x[1] = -at * (60 / V)
+    x[2], x[2, 11000] = -3e38, 3e38
+    x[3], x[3, V - 1] = -80.0, 20.0
+    x[4], x[4, ::5000] = -math.inf, at[::5000] / 1000
+    scores = torch.linspace(-9, -5, beams, device="cuda").view(1, beams)
+    _check(kernels, x, scores, n)
+    for live in (1, 2, 5):
+        some = torch.full_like(scores, -math.inf)
+        some[0, 4:4 + live] = scores[0, :live]
+        _check(kernels, x, some, n)
+        _check(kernels, x[:, :20001], some, n)
+
+
+@pytest.mark.parametrize("R,beams,n,V", [(2, 2, 64, 32000), (1, 3, 50, 12289), (3, 1, 17, 4097), (1, 64, 1, 152064),
+                                         (1, 64, 2, 100001), (4, 5, 63, 8191)])
+def test_select_few_and_many_lists(kernels, R, beams, n, V):
+    """Fewer lists than continuations asked for, and more of them than threads that join them."""
+    scores = torch.linspace(-4, -3, R * beams, device="cuda").view(R, beams)
+    _check(kernels, _logits(R * beams, V, BF16, V), scores, n)
+    _check(kernels, _logits(R * beams, V, torch.float32, V), scores, n)
+
+
 def test_select_captured_and_given_buffers(kernels):
     R, beams, n, V = 3, 4, 8, 30001
     x, scores = _logits(R * beams, V, BF16, 1), torch.full((R, beams), -1.0, device="cuda")
