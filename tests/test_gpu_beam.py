@@ -159,6 +159,23 @@ def test_select_maxima_that_rise(kernels):
         _check(kernels, x[:, :20001], some, n)
 
 
+@pytest.mark.parametrize("dtype,n", [(BF16, 9), (torch.float32, 32)])
+def test_select_many_rows_with_ties(kernels, dtype, n):
+    """Enough rows for the widest tiles: rows that are equal throughout, hold a few values, or rise."""
+    R, beams, V = 8, 4, 152064
+    x = _logits(R * beams, V, dtype, 31)
+    at = torch.arange(V, device="cuda")
+    x[0:4] = 0.0
+    x[4:8] = (at % 7).to(dtype)
+    x[8] = (at >= 100000).to(dtype)
+    x[9] = at.to(torch.float32).mul(40 / V).to(dtype)
+    x[10], x[10, 5] = -3e38, 3e38
+    x[11] = math.nan
+    scores = torch.linspace(-4, -2, R * beams, device="cuda").view(R, beams)
+    scores[0] = -1.0
+    _check(kernels, x, scores, n)
+
+
 @pytest.mark.parametrize("R,beams,n,V", [(2, 2, 64, 32000), (1, 3, 50, 12289), (3, 1, 17, 4097), (1, 64, 1, 152064),
                                          (1, 64, 2, 100001), (4, 5, 63, 8191)])
 def test_select_few_and_many_lists(kernels, R, beams, n, V):
