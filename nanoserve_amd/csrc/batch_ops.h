@@ -95,9 +95,7 @@ int ns_paged_attention(const void* q, long long q_stride, const void* k_pool, co
  * Two sequences that append to one page leave one of the two values of each element and scale, which need not
  * belong together.
  *
- * ns_paged_attention_fp8: ns_paged_attention over the values, but that probabilities enter the second product as one
- * bf16 term (8 significant bits, and their sum is that of the rounded ones) in tiles: with q_start, over a shared prefix,
- * and for more than 16 query heads per kv head; single tokens keep two. The query enters the first product as two e4m3
+ * ns_paged_attention_fp8: ns_paged_attention over the values. The query enters the first product as two e4m3
  * terms under a power of two per head: exact down to 2^-14 of the head's largest magnitude, within 2^-22 of it below,
  * held to 448 * 2^119; infinities in it become NaN. A scale byte of 255 counts as 254.
  */

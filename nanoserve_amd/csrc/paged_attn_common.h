@@ -314,7 +314,6 @@ __device__ __forceinline__ void one_finish(const PagedArgs& a, const Ring& lds, 
 // ------------------------------------------------------------------ caches in 8 bits
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef int i32x2_t __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ i32x8_t join(const u32x4_t& a, const u32x4_t& b) {
   return (i32x8_t){(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
@@ -433,20 +432,20 @@ __device__ __forceinline__ void query_terms(const u32x4_t& q, int e, u32x2_t& hi
 //    are not read but zero, as a value there (it may be NaN) would reach every row through 0 * NaN.
 // In 8 bits (kF8; paged_attn_fp8.hip): the scores on v_mfma_scale_f32_32x32x64_f8f6f4, codes as they lie in the cache with their
 // scale bytes as operands, queries in two e4m3 terms; the values' codes by ds_read_b64_tr_b8, each wave turning what it
-// reads into bf16 (64 instructions a block beside 24 products; a tile in bf16 that all waves share would save 48 of them for a
-// barrier, LDS writes and twice the reads); one probability term. A stage is half as large.
+// reads into bf16 (64 instructions a block beside 40 products; a tile in bf16 that all waves share would save 48 of them for a
+// barrier, LDS writes and twice the reads). A stage is half as large.
 // Measured in bf16 (28 / 4 heads of 128): prompts of 5 sequences of 2000 to 8000 654 us, 677 TFLOP/s, with the second term
 // 1015 (a large library product: 1265); matrix cores busy in half of the cycles and vector units in 58 %, at 1.8 GHz,
 // so that products and softmax still take turns for much of the time. Issuing one half block's softmax between the
 // products of its neighbours did not help (659 -> 681 to 730 us). 4095 tokens with a window of 1000 and 14 / 2 heads of
 // 64 43 us. 96 drafts of 1 to 3 tokens behind 16384 shared positions 100 to 104 us back to back, 108 to 117 among
-// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD. In 8 bits: 463 us (955 TFLOP/s),
-// 42 and 94; four stages instead of two level at 128 dims.
+// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD. In 8 bits: 612 us (722 TFLOP/s),
+// 47.5 and 104, with one probability term 467, 41 and 94.
 template <int D, bool kShared, bool kF8 = false>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
   // (kRow: a row of the cache in units of 2 bytes)
   constexpr int kRow = kF8 ? D / 2 : D, kChunks = kRow / 8, kRowsPerLoad = 64 / kChunks, kLoads = 16 / kRowsPerLoad,
-                kDT = D / 32, kStages = ring_stages<D>(), kTerms = kF8 ? 1 : 2;
+                kDT = D / 32, kStages = ring_stages<D>();
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int R = a.R;
@@ -750,7 +749,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
     const float mc = m == -INFINITY ? 0.f : m * c;
-    u32x4_t pt[kTerms][4];  // B operands of the four 16-key steps
+    u32x4_t pt[2][4];  // B operands of the four 16-key steps
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -759,14 +758,9 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][r + 1], c, -mc));
         const uint32_t term = pack_bf16x2_rne(p0, p1);
         pt[0][2 * u + (r >> 3)][(r & 7) >> 1] = term;
-        if constexpr (kTerms == 1) {  // the sum of what enters the product
-          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, term), __builtin_bit_cast(bf16x2_t, 0x3f803f80u),
-                                              l, false);
-        } else {
-          l += p0 + p1;
-          pt[1][2 * u + (r >> 3)][(r & 7) >> 1] = pack_bf16x2_rne(p0 - __uint_as_float(term << 16),
-                                                                  p1 - __uint_as_float(term & 0xffff0000u));
-        }
+        l += p0 + p1;
+        pt[1][2 * u + (r >> 3)][(r & 7) >> 1] = pack_bf16x2_rne(p0 - __uint_as_float(term << 16),
+                                                                p1 - __uint_as_float(term & 0xffff0000u));
       }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -784,7 +778,7 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
         vf[d] = __builtin_bit_cast(bf16x8_t, (u32x4_t){v0[0], v0[1], v1[0], v1[1]});
       }
 #pragma unroll
-      for (int i = 0; i < kTerms; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int d = 0; d < kDT; ++d)
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[d], __builtin_bit_cast(bf16x8_t, pt[i][u]), o[d], 0, 0, 0);

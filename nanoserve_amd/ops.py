@@ -857,9 +857,8 @@ class Kernels:
                             shared=0, window=0, sinks=0, scale=None, work=None, out=None):
         """paged_attention over a cache in 8 bits (pools and scales as paged_append_fp8 writes them): the result of
         paged_attention over a bf16 cache that holds code times scale, but for infinities in a query, which count as NaN,
-        query magnitudes above 448 * 2^119, which are held to it, those below 2^-14 of their head's largest, which are
-        held to 2^-22 of it, and probabilities: with q_start, over a shared prefix and for more than 16 query heads per kv head
-        they are rounded to bf16 before they weigh the values. ``work``: from paged_attention_fp8_workspace."""
+        query magnitudes above 448 * 2^119, which are held to it, and those below 2^-14 of their head's largest, which are
+        held to 2^-22 of it. ``work``: from paged_attention_fp8_workspace."""
         here = _device_of(q, "q", torch.bfloat16)
         shape, steps = q.shape, q.stride()
         if len(shape) != 2 or steps[1] != 1:

@@ -1,0 +1,61 @@
+"""Attention over a paged cache in 8 bits where its formats end: probabilities beside values that cancel, scales and queries
+near the ends of their ranges, scores that fp32 holds and a factor of them does not, batches of more tiles than workgroups."""
+import pytest
+import torch
+
+import paged_fp8_ref as F
+import paged_ref as R
+
+BF16, U8 = torch.bfloat16, torch.uint8
+NAN = float("nan")
+pytestmark = pytest.mark.gpu
+
+
+def _queries(T, Hq, D, seed, scale=2.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(T, Hq * D, generator=g) * scale).to(BF16).cuda()
+
+
+def _attend(kernels, batch, q, Hq, **kw):
+    got = kernels.paged_attention_fp8(q, *batch.cache(), batch.table, batch.lens, Hq, q_start=batch.q_start, **kw)
+    torch.cuda.synchronize()
+    return got
+
+
+def _fill(batch, name, codes, byte):
+    """Codes (broadcast over positions) and one scale byte for every position of the batch, and the values they stand for."""
+    values, pool, marks = getattr(batch, name), getattr(batch, name + "8"), getattr(batch, name + "s")
+    live = ~torch.isnan(values.float())
+    codes = codes.to("cuda").float().expand(values.shape).to(F.FP8)
+    bits = pool.view(U8)
+    bits.copy_(torch.where(live, codes.view(U8), bits))
+    there = live.any(3).unflatten(2, (-1, 16)).any(3)
+    marks.view(U8).copy_(torch.where(there, byte, 255).to(U8))
+    exact = codes.double() * 2.0 ** (byte - 127)
+    assert torch.equal(exact.to(BF16).double(), exact)
+    setattr(batch, name, torch.where(live, exact, NAN).to(BF16))
+
+
+def _check(got, want, v):
+    """Half a bf16 step of the result (2^-8 of it), and of the largest value v that a token can see: 2^-16 for probabilities of
+    16 bits, 2^-13 for fp32 scores up to a few hundred in the exponent (128 products of 2^-24 each) and fp32 sums, 2^-15 for the
+    query's terms below 2^-14 of its largest (off by 2^-22 of 8, times keys of 5, a scale of 0.09 and a quarter of 128 dims)."""
+    err = (got.cpu().double().view_as(want) - want).abs()
+    bound = want.abs() * 2.0 ** -8 + (2.0 ** -16 + 2.0 ** -13 + 2.0 ** -15) * v
+    assert bool((err <= bound).all()), float((err - bound).max())
+
+
+# (positions, new tokens, shared): tiles whole and split, single tokens and tiles behind a shared prefix
+BATCHES = [([70, 0, 300, 65, 1], [70, 0, 44, 1, 1], 0), ([2000, 1111], [130, 1], 0), ([33, 700], None, 0),
+           ([300, 257, 256, 280], None, 256), ([700, 65, 64, 70], [3, 1, 2, 6], 64)]
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(28, 4, 128), (14, 2, 64), (40, 2, 128)])
+@pytest.mark.parametrize("lens,new,shared", BATCHES)
+def test_values_that_cancel(kernels, lens, new, shared, Hq, Hk, D):
+    """Values of 1 and -1: what is left of them shows the probabilities themselves, which have 16 bits on every path."""
+    batch = F.Fp8Batch(lens, new, Hk, D, 16, shared=shared, seed=11)
+    g = torch.Generator().manual_seed(12)
+    _fill(batch, "v", torch.randint(0, 2, tuple(batch.v.shape), generator=g) * 2 - 1, 127)
+    q = _queries(batch.T, Hq, D, 13)
+    _check(_attend(kernels, batch, q, Hq, shared=shared), R.attention(batch, q, Hq), 1.0)
