@@ -87,7 +87,6 @@ __device__ __forceinline__ void one8_body(const PagedArgs& a, int item, int g, c
   if (cnt > 0) refill(0);  // (its loads beside the query's)
   i64_t qh[D / 32], ql[D / 32];
   const int qe = query_exponent<D / 32, true>(qf);
-  const float cq = a.c * __uint_as_float((uint32_t)(qe + 127) << 23);  // of this lane's head
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
     u32x2_t hi, low;
@@ -174,9 +173,10 @@ __device__ __forceinline__ void one8_body(const PagedArgs& a, int item, int g, c
           low = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(x, ql[2 * s + h], low, 0, 0, 0);
         }
       }
-      const float f = cq * __uint_as_float((uint32_t)(at.sc[u] & 0xff) << 23);
+      // (as an exponent: the powers of two of query and keys together may pass fp32 where the score is small or 0)
+      const int e = qe + (at.sc[u] & 0xff) - 127;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sr[u][r] = fmaf(low[r], 0.0625f, hi[r]) * f;
+      for (int r = 0; r < 4; ++r) sr[u][r] = __builtin_amdgcn_ldexpf(fmaf(low[r], 0.0625f, hi[r]), e) * a.c;
     }
     if (!at.whole) {
 #pragma unroll

@@ -59,3 +59,36 @@ def test_values_that_cancel(kernels, lens, new, shared, Hq, Hk, D):
     _fill(batch, "v", torch.randint(0, 2, tuple(batch.v.shape), generator=g) * 2 - 1, 127)
     q = _queries(batch.T, Hq, D, 13)
     _check(_attend(kernels, batch, q, Hq, shared=shared), R.attention(batch, q, Hq), 1.0)
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(8, 2, 128), (8, 2, 64), (40, 2, 128)])
+@pytest.mark.parametrize("lens,new,shared", BATCHES)
+def test_large_queries_beside_large_scales(kernels, lens, new, shared, Hq, Hk, D):
+    """Queries of 2^21 in a dim where the keys are 0, keys of 448 * 2^119 in one where the queries are: scores are 0, not 0 times a
+    factor that passes fp32."""
+    batch = F.Fp8Batch(lens, new, Hk, D, 16, shared=shared, seed=14, spread=0)
+    codes = torch.zeros(D)
+    codes[2] = 448.0
+    _fill(batch, "k", codes, 119 + 127)
+    q = torch.zeros(batch.T, Hq, D)
+    q[:, :, 0] = 2.0 ** 21
+    q = q.view(batch.T, -1).to(BF16).cuda()
+    want = R.attention(batch, q, Hq)
+    _check(_attend(kernels, batch, q, Hq, shared=shared), want, 8.0)
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(8, 2, 128), (8, 2, 64), (40, 2, 128)])
+@pytest.mark.parametrize("lens,new,shared", BATCHES)
+def test_scales_of_byte_zero(kernels, lens, new, shared, Hq, Hk, D):
+    """2^-127, which no append writes and fp32's normal numbers do not reach: for keys, and for values (all with the same
+    probability, so that no product is smaller than they are)."""
+    batch = F.Fp8Batch(lens, new, Hk, D, 16, shared=shared, seed=16, spread=0)
+    g = torch.Generator().manual_seed(17)
+    size = tuple(batch.k.shape)
+    _fill(batch, "k", torch.randint(2, 8, size, generator=g) * (torch.randint(0, 2, size, generator=g) * 2 - 1), 0)
+    q = (torch.randn(batch.T, Hq * D, generator=g) * 2.0 ** 124).to(BF16).cuda()
+    _check(_attend(kernels, batch, q, Hq, shared=shared), R.attention(batch, q, Hq), 8.0)
+    _fill(batch, "v", torch.randint(2, 8, size, generator=g) * 64, 0)
+    q.zero_()
+    got, up = _attend(kernels, batch, q, Hq, shared=shared).double(), 2.0 ** 127
+    _check(got * up, R.attention(batch, q, Hq) * up, 448.0)
