@@ -24,6 +24,10 @@ namespace {
 constexpr int kTileRows = 128;  // query rows of a tile
 constexpr int kTileKeys = 64;   // keys per block of the tile kernel
 constexpr int kOneWaves = 4;
+// Where a row's largest logit (base 2) is larger, the maximum is taken off its scores before they are multiplied: s c - m c as
+// one fma is off by m c's rounding, 2^-24 of it, by which all of the row's exponentials are moved together (2^-4 in the
+// exponent up to here), and past 2^31 out of fp32.
+constexpr float kFarLogit = 1048576.f;
 constexpr uint32_t kOut = 0x7fffffffu;  // a buffer offset out of every range: reads as zero
 
 struct PagedArgs {
@@ -659,7 +663,8 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
   for (int d = 0; d < kDT; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, mc = 0.f, l = 0.f;
+  bool far = false;  // some row's maximum is past kFarLogit
   const float c = a.c;
 
   // transpose-read offsets (in units of 2 bytes) of the 32-dim tiles at key row 4 kh + (lane % 16) / 4; 8 bits: at
@@ -737,18 +742,26 @@ __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, c
 #pragma unroll
       for (int r = 0; r < 16; ++r) bm = fmaxf(bm, s[u][r]);
     bm = fmaxf(bm, lane_xor32(bm));
-    if (__any(bm > m)) {
+    if (far | __any(bm > m)) {
       const float mn = fmaxf(m, bm);
       const float ms = mn == -INFINITY ? 0.f : mn;
       const float alpha = __builtin_amdgcn_exp2f((m - ms) * c);
       m = mn;
+      mc = ms * c;
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < kDT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      far = __any(fabsf(mc) > kFarLogit);
+      if (far) {
+        mc = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[u][r] -= ms;
+      }
     }
-    const float mc = m == -INFINITY ? 0.f : m * c;
     u32x4_t pt[2][4];  // B operands of the four 16-key steps
 #pragma unroll
     for (int u = 0; u < 2; ++u)

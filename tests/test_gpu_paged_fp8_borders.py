@@ -79,6 +79,24 @@ def test_large_queries_beside_large_scales(kernels, lens, new, shared, Hq, Hk, D
 
 @pytest.mark.parametrize("Hq,Hk,D", [(8, 2, 128), (8, 2, 64), (40, 2, 128)])
 @pytest.mark.parametrize("lens,new,shared", BATCHES)
+@pytest.mark.parametrize("large,less,e,q0,q1", [(1.0, 0.875, 14, 2.0 ** 8, 1.75 * 2.0 ** -4), (1.0, 0.875, 44, 2.0 ** 8, 1.75 * 2.0 ** -4),
+                                                (2.0 ** -8, 2.0 ** -9, 119, 2.0 ** 21, 1.75 * 2.0 ** 8)])
+def test_large_scores(kernels, lens, new, shared, large, less, e, q0, q1, Hq, Hk, D):
+    """Scores of 0 and finite ones far from it, in the last case where queries and scales together pass fp32: the tokens of the
+    largest share the weight (the next ones are 0.22 * 2^10 / 11.3 or more below, e^-19)."""
+    batch = F.Fp8Batch(lens, new, Hk, D, 16, shared=shared, seed=15, spread=0)
+    codes = torch.zeros(16, D)
+    codes[1::3, 1], codes[2::5, 1] = large, less
+    codes[:, 2] = 448.0
+    _fill(batch, "k", codes.repeat(batch.k.shape[2] // 16, 1), e + 127)
+    q = torch.zeros(batch.T, Hq, D)
+    q[:, :, 0], q[:, :, 1] = q0, q1
+    q = q.view(batch.T, -1).to(BF16).cuda()
+    _check(_attend(kernels, batch, q, Hq, shared=shared), R.attention(batch, q, Hq), 8.0)
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(8, 2, 128), (8, 2, 64), (40, 2, 128)])
+@pytest.mark.parametrize("lens,new,shared", BATCHES)
 def test_scales_of_byte_zero(kernels, lens, new, shared, Hq, Hk, D):
     """2^-127, which no append writes and fp32's normal numbers do not reach: for keys, and for values (all with the same
     probability, so that no product is smaller than they are)."""
