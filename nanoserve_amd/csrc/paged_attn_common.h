@@ -157,12 +157,20 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int item, int& b, 
     tiles += (float)x.tiles;
   }
   total = wave_sum(total);
-  // Tiles of a cache in 8 bits: half as many workgroups aimed at (one per CU) once there are four tiles to five CUs, as a
-  // range then costs more in partials than it gains. us with all and half of them, on 256 CUs: 2000 tokens of 8
-  // sequences of 1000 to 4000 (476 tiles) 163, 111; 1000 tokens (220) 46.2, 41.3; 800 after 3000 (176) 88.7, 99.1; 2 x
-  // 300 after 8000 (160) 125, 210; 512 after 3000 (112) 54.5, 61.6.
+  // Tiles of a cache in 8 bits: half as many workgroups aimed at (one per CU) where the tiles times kv heads are nearly as
+  // many as the two per CU, so that splitting them makes a second round, and from four fifths of one per CU on where the tiles'
+  // lists are so short (in the mean) that a range costs more in partials than it gains. us with all and half of them, 28 / 4
+  // heads of 128 on 256 CUs, by tiles times kv heads: 448 (8 x 200 to 300 tokens up to 1000 to 4000 positions) 209, 157; 392
+  // (7 of the same, 39 blocks) 168, 136; 220 (1000 tokens, 16) 48.4, 44.4; 224 (4 x 250 tokens after 1000, 20) 60.8, 52.4; 256
+  // (64 x 2 to 5 after 300 to 500, 6) 30.7, 28.0. Not halved: 256 (64 x 2 to 5 after 4000 to 8000, 94) 157, 237; 224 (4 x
+  // 250 after 8000, 127) 207, 237; 220 (1000 after 30000, 477) 669, 826; 400 (100 x 2 to 5 after 4000 to 8000, 94) 269, 301.
+  // Against the rule, by a few per cent: 256 (64 x 2 to 5 after 600 to 1000, 13) 39.6, 41.8; 224 (4 x 250 after 1500, 28)
+  // 71.7, 66.0. Past 512 it makes little difference.
   float per_target = a.per_target;
-  if (kSorted && wave_sum(tiles) * per_target > 0.4f) per_target *= 2.f;
+  if constexpr (kSorted) {
+    const float all = wave_sum(tiles), fill = all * per_target;
+    if (fill > 0.8f || (fill > 0.4f && total <= (fill > 0.7f ? 60.f : 20.f) * all)) per_target *= 2.f;
+  }
   const int share = __builtin_amdgcn_readfirstlane((int)ceilf(total * per_target));
   int per = max(a.unit, (share + a.unit - 1) / a.unit * a.unit);
   // Sequences end inside a share: where that makes more items than workgroups aimed at, the last ones would

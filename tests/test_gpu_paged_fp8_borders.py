@@ -110,3 +110,19 @@ def test_scales_of_byte_zero(kernels, lens, new, shared, Hq, Hk, D):
     q.zero_()
     got, up = _attend(kernels, batch, q, Hq, shared=shared).double(), 2.0 ** 127
     _check(got * up, R.attention(batch, q, Hq) * up, 448.0)
+
+
+@pytest.mark.parametrize("Hq,Hk,D,lens,new", [
+    (32, 16, 64, [300, 310, 200], [300, 250, 200]), (28, 4, 128, [500 + 3 * i for i in range(60)], [1 + i % 30 for i in range(60)]),
+    (8, 4, 64, [40 + 7 * i for i in range(70)], [1 + i % 5 for i in range(70)]),
+    (16, 8, 128, [40 + 7 * i for i in range(70)], [1 + i % 5 for i in range(70)]),
+    (64, 64, 64, [700, 31, 1], [130, 31, 1]), (32, 32, 64, [2500, 1400], [500, 300])])
+def test_many_tiles(kernels, Hq, Hk, D, lens, new):
+    """Tiles times kv heads from two fifths of the workgroups aimed at to more than they are, of few blocks and of many, of up to
+    64 sequences and of more."""
+    batch = F.Fp8Batch(lens, new, Hk, D, 16, seed=18, spread=0)
+    q = _queries(batch.T, Hq, D, 19)
+    v = batch.v.float().nan_to_num(0, 0, 0).abs().amax().item()
+    _check(_attend(kernels, batch, q, Hq), R.attention(batch, q, Hq), v)
+    kw = dict(window=100, sinks=5)
+    _check(_attend(kernels, batch, q, Hq, **kw), R.attention(batch, q, Hq, **kw), v)
