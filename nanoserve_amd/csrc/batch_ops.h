@@ -170,6 +170,8 @@ int ns_beam_select(const void* logits, int fp32, long long row_stride, const flo
  * n % page_size rows of every layer and head are copied in both pools, and the scales of their blocks (k_scales and
  * v_scales NULL: a cache without). The last, partly filled pages of a request must be the beams' own. table is not changed,
  * so a repeated call gives the same; entries outside [0, n_pages) are moved and not copied from or to.
+ * Whole pages that only beams had which no one goes on from are in no row of out: ns_paged_reorder_back gives them back, or else
+ * the caller has to keep count of a request's pages.
  * Pools: + layer * layer_stride + page * page_stride + head * head_stride + row * row_bytes (bytes, multiples of 16); scales
  * alike, one byte per 16 rows. -2 for sizes <= 0, beams > 64, R * beams >= 2^24, page_size % 16, width * page_size
  * >= 2^30, page_size * row_bytes * Hk >= 2^31, strides by which layers, pages and heads overlap, NULL or misaligned pointers
@@ -180,6 +182,22 @@ int ns_paged_reorder(const int* parents, long long parent_stride, const int* tab
                      long long page_stride, long long head_stride, void* k_scales, void* v_scales,
                      long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride, int layers,
                      int n_pages, int page_size, int row_bytes, int R, int beams, int Hk, void* stream);
+
+/*
+ * ns_paged_reorder, and the whole pages (of columns below w) that are in rows of beams which no one goes on from and in no row of
+ * one from which someone does are pushed on the stack of ns_paged_reserve, each once: free[n_free[0]] on, the last one the
+ * top, in the order of the requests, their columns and in a column the beams. Entries outside [0, n_pages) are no pages. A
+ * repeated call pushes them again. n_free below 0 counts as 0; past the capacity nothing is pushed, and what would lie past it
+ * is left out: the stack needs room for every page. Pages that rows of another request hold too must be in all of a request's
+ * rows (a common prefix is). -2 also for n_free NULL, free NULL with a capacity, capacity < 0 or >= 2^31, either misaligned (4
+ * bytes), and the two over each other or anything else.
+ */
+int ns_paged_reorder_back(const int* parents, long long parent_stride, const int* table, long long table_stride, int width,
+                          const int* lens, int* out, void* k_pool, void* v_pool, long long layer_stride,
+                          long long page_stride, long long head_stride, void* k_scales, void* v_scales,
+                          long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride, int layers,
+                          int n_pages, int page_size, int row_bytes, int R, int beams, int Hk, int* free,
+                          long long capacity, int* n_free, void* stream);
 
 /*
  * Bytes of workspace ns_sample uses for these sizes, 0 for none or for sizes it rejects. Launches that

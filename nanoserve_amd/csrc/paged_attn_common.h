@@ -130,17 +130,6 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, int b) {
   return x;
 }
 
-// Inclusive prefix sums over the wave by DPP (row shifts, then row broadcasts).
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return v;
-}
-
 // Item `item` of the batch: its sequence, the number within it, and the sequence's first partial (a
 // token slot). False past the last item. Uniform over the workgroup's waves. kSorted: up to 64 sequences go by falling
 // length, so that what starts last is short.

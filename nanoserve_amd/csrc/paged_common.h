@@ -4,11 +4,26 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "spans.h"
 #include "w4_common.h"
 
 namespace ns {
+
+// Inclusive sums over the wave by DPP (row shifts, then row broadcasts).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  auto from = [](uint32_t x, auto ctrl, auto rows) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using M = std::integral_constant<int, 0xf>;
+  v += from(v, std::integral_constant<int, 0x111>{}, M{});
+  v += from(v, std::integral_constant<int, 0x112>{}, M{});
+  v += from(v, std::integral_constant<int, 0x114>{}, M{});
+  v += from(v, std::integral_constant<int, 0x118>{}, M{});
+  v += from(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+  return v + from(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+}
 
 struct Batch {
   const int *q_start, *lens, *table;  // q_start null: one token per sequence

@@ -9,6 +9,12 @@
 // flight to a lane and no divisions: with a workgroup per layer and an index per 16 bytes 16 x 8 beams in 28 layers (88 MB)
 // took 30.8 us, 16 beams on pages of 16 17.6. Stores pass the caches, which the copies would leave before they are read.
 // Measured: 16 x 8 beams 18.3 us, 4.8 TB/s (20.6 with ordinary stores); 4 x 4 beams on pages of 16 4.4 us.
+//
+// Whole pages that only ended beams had are in no table afterwards. They go to the stack of free pages, where the caller gives
+// it: one workgroup looks at every column of the requests' tables, 64 of one request to a wave, and prefix sums say which place
+// is whose, so the order is always the same. Bound by the latency of parents -> entries -> others' entries, wave by wave: with
+// it 4 beams of 333 positions take 6.5 us instead of 3.3, 16 x 8 beams of 100 to 900 on pages of 64 in 28 layers 23.5 instead of
+// 17.6, of 8000 on pages of 16 in one layer 36 instead of 3.2 (52 where half of the columns are each beam's own).
 #include <stdint.h>
 
 #include <algorithm>
@@ -112,6 +118,81 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(ReorderArgs a) {
   for (int i = lane; i < (part + kScaleRows - 1) / kScaleRows; i += kWave) scales[dst * a.s_page + i] = scales[src * a.s_page + i];
 }
 
+constexpr int kBackThreads = 1024, kBackWaves = kBackThreads / kWave;
+
+struct BackArgs {
+  const int *parents, *table, *lens;
+  long long parent_stride, table_stride, capacity;
+  int *free, *n_free;
+  int R, beams, width, page_size, n_pages;
+};
+
+// The beams, as bits, whose page in column `col` (one to a lane) no beam has that goes on, nor an earlier one of them.
+__device__ __forceinline__ unsigned long long dropped_of(const BackArgs& a, long long request, int col) {
+  const int lane = __lane_id();
+  int p = -1, whole = 0;
+  if (lane < a.beams) {
+    p = a.parents[request * a.parent_stride + lane];
+    if ((unsigned)p >= (unsigned)a.beams) p = lane;
+    whole = min(max(a.lens[request * a.beams + lane], 0), a.width * a.page_size) / a.page_size;
+  }
+  unsigned long long goes_on = 0;
+  for (int q = 0; q < a.beams; ++q)
+    if (__ballot(p == q)) goes_on |= 1ull << q;
+  const unsigned long long all = a.beams == 64 ? ~0ull : (1ull << a.beams) - 1;
+  const int* column = a.table + request * a.beams * a.table_stride + min(col, a.width - 1);
+  unsigned long long dropped = 0;
+  for (unsigned long long ended = all & ~goes_on; ended; ended &= ended - 1) {
+    const int e = __builtin_ctzll(ended);
+    if (!__any(col < __builtin_amdgcn_readlane(whole, e))) continue;
+    const int id = column[e * a.table_stride];
+    bool held = col >= __builtin_amdgcn_readlane(whole, e) || (unsigned)id >= (unsigned)a.n_pages;
+    // four at a time, the first ones beside the page itself; most columns are shared with one of them
+    unsigned long long others = goes_on | (all & ~goes_on & ((1ull << e) - 1));
+    do {
+      int other[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        other[u] = others ? column[__builtin_ctzll(others) * a.table_stride] : -1;
+        others &= others - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) held |= other[u] == id;
+    } while (others && !__all(held));
+    if (!held) dropped |= 1ull << e;
+  }
+  return dropped;
+}
+
+__global__ void __launch_bounds__(kBackThreads) back_kernel(BackArgs a) {
+  __shared__ int part[2][kBackWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const long long chunks = (a.width + kWave - 1) / kWave, tasks = a.R * chunks;
+  long long top = max(a.n_free[0], 0);
+  if (top > a.capacity) return;
+  int now = 0;
+  for (long long base = 0; base < tasks; base += kBackWaves, now ^= 1) {
+    const long long task = base + wv, request = task / chunks;
+    const int col = (int)(task % chunks) * kWave + lane;
+    unsigned long long dropped = task < tasks ? dropped_of(a, request, col) : 0;
+    const int n = __popcll(dropped), upto = wave_scan(n);
+    if (lane == 63) part[now][wv] = upto;
+    __syncthreads();  // (the other half is read until here)
+    long long at = top + upto - n;
+#pragma unroll
+    for (int u = 0; u < kBackWaves; ++u) {
+      if (u < wv) at += part[now][u];
+      top += part[now][u];
+    }
+    for (; dropped; dropped &= dropped - 1, ++at) {
+      const int e = __builtin_ctzll(dropped);
+      if (at < a.capacity) a.free[at] = a.table[(request * a.beams + e) * a.table_stride + col];
+    }
+  }
+  __syncthreads();  // (every wave has read the height)
+  if (tid == 0) a.n_free[0] = (int)min(top, a.capacity);
+}
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // Pages, heads and layers of pieces of `piece` bytes: whether no two share a byte, whichever of the dimensions is the
@@ -129,59 +210,67 @@ bool nested(long long piece, long long layers, long long layer, long long pages,
   return true;
 }
 
-}  // namespace
-}  // namespace ns
-
-extern "C" int ns_paged_reorder(const int* parents, long long parent_stride, const int* table, long long table_stride,
-                                int width, const int* lens, int* out, void* k_pool, void* v_pool, long long layer_stride,
-                                long long page_stride, long long head_stride, void* k_scales, void* v_scales,
-                                long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride,
-                                int layers, int n_pages, int page_size, int row_bytes, int R, int beams, int Hk,
-                                void* stream) {
-  if (R <= 0 || beams <= 0 || beams > ns::kMostBeams || (long long)R * beams >= (1 << 24)) return -2;
+// Both entry points; n_free null: no stack.
+int reorder(const int* parents, long long parent_stride, const int* table, long long table_stride, int width, const int* lens,
+            int* out, void* k_pool, void* v_pool, long long layer_stride, long long page_stride, long long head_stride,
+            void* k_scales, void* v_scales, long long scale_layer_stride, long long scale_page_stride,
+            long long scale_head_stride, int layers, int n_pages, int page_size, int row_bytes, int R, int beams, int Hk,
+            int* free_pages, long long capacity, int* n_free, void* stream) {
+  if (R <= 0 || beams <= 0 || beams > kMostBeams || (long long)R * beams >= (1 << 24)) return -2;
   if (width <= 0 || page_size <= 0 || page_size % 16 || (long long)width * page_size >= (1ll << 30)) return -2;
   if (layers <= 0 || n_pages <= 0 || Hk <= 0 || row_bytes <= 0 || row_bytes % 16) return -2;
   if ((long long)page_size * row_bytes * Hk >= (1ll << 31)) return -2;
   if (parent_stride < beams || parent_stride >> 46 || table_stride < width || table_stride >> 46) return -2;
   if (!parents || !table || !lens || !out || !k_pool || !v_pool || !k_scales != !v_scales) return -2;
   for (const void* p : {(const void*)parents, (const void*)table, (const void*)lens, (const void*)out})
-    if (!ns::aligned(p, 4)) return -2;
-  if (!ns::aligned(k_pool, 16) || !ns::aligned(v_pool, 16)) return -2;
+    if (!aligned(p, 4)) return -2;
+  if (!aligned(k_pool, 16) || !aligned(v_pool, 16)) return -2;
   for (const long long s : {layer_stride, page_stride, head_stride})
     if (s < 0 || s % 16 || s >> 46) return -2;
   for (const long long s : {scale_layer_stride, scale_page_stride, scale_head_stride})
     if (s < 0 || s >> 46) return -2;
-  const long long piece = (long long)page_size * row_bytes, marks = page_size / ns::kScaleRows, rows = (long long)R * beams;
-  if (!ns::nested(piece, layers, layer_stride, n_pages, page_stride, Hk, head_stride)) return -2;
-  if (k_scales && !ns::nested(marks, layers, scale_layer_stride, n_pages, scale_page_stride, Hk, scale_head_stride))
+  const long long piece = (long long)page_size * row_bytes, marks = page_size / kScaleRows, rows = (long long)R * beams;
+  if (!nested(piece, layers, layer_stride, n_pages, page_stride, Hk, head_stride)) return -2;
+  if (k_scales && !nested(marks, layers, scale_layer_stride, n_pages, scale_page_stride, Hk, scale_head_stride))
     return -2;
   if ((long long)layers * Hk >= (1ll << 30) || rows * (((long long)layers * Hk + 3) / 4 * 2 + 1) >= (1ll << 31)) return -2;
-  const ns::Bytes y = ns::bytes_of(out, 4 * (size_t)rows * width), z[] = {ns::rows_of(parents, R, parent_stride, beams, 4),
-                                                                        ns::rows_of(table, rows, table_stride, width, 4),
-                                                                        ns::bytes_of(lens, 4 * (size_t)rows)};
-  for (const ns::Bytes& r : z)
-    if (!ns::apart(y, r)) return -2;
+  const Bytes y = bytes_of(out, 4 * (size_t)rows * width), z[] = {rows_of(parents, R, parent_stride, beams, 4),
+                                                                        rows_of(table, rows, table_stride, width, 4),
+                                                                        bytes_of(lens, 4 * (size_t)rows)};
+  for (const Bytes& r : z)
+    if (!apart(y, r)) return -2;
   // what lies between the pools' pages counts as theirs here
   auto span = [&](const void* p, long long x, long long layer, long long page, long long head) {
-    return ns::bytes_of(p, (layers - 1) * layer + (n_pages - 1) * page + (Hk - 1) * head + x);
+    return bytes_of(p, (layers - 1) * layer + (n_pages - 1) * page + (Hk - 1) * head + x);
   };
-  const ns::Bytes pools[] = {span(k_pool, piece, layer_stride, page_stride, head_stride),
+  const Bytes pools[] = {span(k_pool, piece, layer_stride, page_stride, head_stride),
                              span(v_pool, piece, layer_stride, page_stride, head_stride),
                              span(k_scales, marks, scale_layer_stride, scale_page_stride, scale_head_stride),
                              span(v_scales, marks, scale_layer_stride, scale_page_stride, scale_head_stride)};
-  for (const ns::Bytes& p : pools)
-    if (!ns::apart(p, y) || !ns::apart(p, z[0]) || !ns::apart(p, z[1]) || !ns::apart(p, z[2])) return -2;
+  for (const Bytes& p : pools)
+    if (!apart(p, y) || !apart(p, z[0]) || !apart(p, z[1]) || !apart(p, z[2])) return -2;
+  if (n_free) {
+    if (capacity < 0 || capacity >= (1ll << 31) || (!free_pages && capacity > 0)) return -2;
+    if (!aligned(free_pages, 4) || !aligned(n_free, 4)) return -2;
+    const Bytes stack[] = {bytes_of(free_pages, 4 * (size_t)capacity), bytes_of(n_free, 4)};
+    if (!apart(stack[0], stack[1])) return -2;
+    for (const Bytes& r : stack) {
+      if (!apart(r, y) || !apart(r, z[0]) || !apart(r, z[1]) || !apart(r, z[2])) return -2;
+      for (const Bytes& p : pools)
+        if (!apart(r, p)) return -2;
+    }
+  }
   // but K's, V's and the scales' pages may lie between each other's, if they are equally far apart
-  const ns::Pieces codes{{layer_stride, page_stride, head_stride}, {layers, n_pages, Hk}, piece},
+  const Pieces codes{{layer_stride, page_stride, head_stride}, {layers, n_pages, Hk}, piece},
       scales{{scale_layer_stride, scale_page_stride, scale_head_stride}, {layers, n_pages, Hk}, marks};
   const bool together = n_pages == 1 || page_stride == scale_page_stride;
   for (int i = 0; i < 4; ++i)
     for (int j = 0; j < i; ++j)
-      if (!ns::apart(pools[i], pools[j]) &&
-          (((i < 2) != (j < 2) && !together) || !ns::pieces_apart(i < 2 ? codes : scales, j < 2 ? codes : scales,
+      if (!apart(pools[i], pools[j]) &&
+          (((i < 2) != (j < 2) && !together) || !pieces_apart(i < 2 ? codes : scales, j < 2 ? codes : scales,
                                                                (__int128)pools[j].lo - pools[i].lo)))
         return -2;
-  ns::ReorderArgs a{};
+  ReorderArgs a{};
   a.parents = parents;
   a.table = table;
   a.lens = lens;
@@ -208,6 +297,40 @@ extern "C" int ns_paged_reorder(const int* parents, long long parent_stride, con
   a.table_grid = (int)rows;
   a.groups = (int)(((long long)layers * Hk + 3) / 4);
   const auto st = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(ns::reorder_kernel, dim3((unsigned)(rows * (2ll * a.groups + 1))), dim3(ns::kThreads), 0, st, a);
+  hipLaunchKernelGGL(reorder_kernel, dim3((unsigned)(rows * (2ll * a.groups + 1))), dim3(kThreads), 0, st, a);
+  if (n_free) {
+    const BackArgs b{parents, table, lens, parent_stride, table_stride, capacity, free_pages, n_free, R, beams, width, page_size,
+                     n_pages};
+    hipLaunchKernelGGL(back_kernel, dim3(1), dim3(kBackThreads), 0, st, b);
+  }
   return static_cast<int>(hipGetLastError());
 }
+
+}  // namespace
+}  // namespace ns
+
+extern "C" {
+
+int ns_paged_reorder(const int* parents, long long parent_stride, const int* table, long long table_stride, int width,
+                     const int* lens, int* out, void* k_pool, void* v_pool, long long layer_stride,
+                     long long page_stride, long long head_stride, void* k_scales, void* v_scales,
+                     long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride, int layers,
+                     int n_pages, int page_size, int row_bytes, int R, int beams, int Hk, void* stream) {
+  return ns::reorder(parents, parent_stride, table, table_stride, width, lens, out, k_pool, v_pool, layer_stride, page_stride,
+                     head_stride, k_scales, v_scales, scale_layer_stride, scale_page_stride, scale_head_stride, layers, n_pages,
+                     page_size, row_bytes, R, beams, Hk, nullptr, 0, nullptr, stream);
+}
+
+int ns_paged_reorder_back(const int* parents, long long parent_stride, const int* table, long long table_stride, int width,
+                          const int* lens, int* out, void* k_pool, void* v_pool, long long layer_stride,
+                          long long page_stride, long long head_stride, void* k_scales, void* v_scales,
+                          long long scale_layer_stride, long long scale_page_stride, long long scale_head_stride, int layers,
+                          int n_pages, int page_size, int row_bytes, int R, int beams, int Hk, int* free_pages,
+                          long long capacity, int* n_free, void* stream) {
+  if (!n_free) return -2;
+  return ns::reorder(parents, parent_stride, table, table_stride, width, lens, out, k_pool, v_pool, layer_stride, page_stride,
+                     head_stride, k_scales, v_scales, scale_layer_stride, scale_page_stride, scale_head_stride, layers, n_pages,
+                     page_size, row_bytes, R, beams, Hk, free_pages, capacity, n_free, stream);
+}
+
+}  // extern "C"

@@ -33,18 +33,6 @@ struct ReserveArgs {
 // and from 8192: 2400 rows 13.7, 12.2, 12.2; 6800 13.8, 13.7, 14.6.
 constexpr int kOwnRows = 4096;
 
-// Inclusive sums over the wave by DPP (row shifts, then row broadcasts).
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  int v = (int)x;
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-  return (uint32_t)v;
-}
-
 // What one sequence asks for.
 struct Ask {
   int had, has;         // table entries before and after

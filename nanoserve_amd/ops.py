@@ -79,6 +79,8 @@ INTERNAL_SIGNATURES = {
     "ns_beam_select_workspace": [_I32] * 4,
     "ns_beam_select": [_VP, _I32, _I64] + [_VP] * 5 + [_SZ] + [_I32] * 4 + [_VP],
     "ns_paged_reorder": [_VP, _I64, _VP, _I64, _I32] + [_VP] * 4 + [_I64] * 3 + [_VP] * 2 + [_I64] * 3 + [_I32] * 7 + [_VP],
+    "ns_paged_reorder_back": [_VP, _I64, _VP, _I64, _I32] + [_VP] * 4 + [_I64] * 3 + [_VP] * 2 + [_I64] * 3 + [_I32] * 7 +
+                             [_VP, _I64, _VP, _VP],
     "ns_sample_workspace": [_I32] * 3,
     "ns_sample": [_VP, _I32, _I64, _VP, _VP, _F32, _VP, _I32, _VP, _F32, _VP, _F32, _VP, _VP, _SZ, _I32,
                   _I32, _VP],
@@ -959,7 +961,8 @@ class Kernels:
         self._check(rc, "ns_paged_reserve")
         return out
 
-    def paged_reorder(self, parents, pages, lens, k_pages, v_pages, k_scales=None, v_scales=None, out=None):
+    def paged_reorder(self, parents, pages, lens, k_pages, v_pages, k_scales=None, v_scales=None, out=None, free=None,
+                      n_free=None):
         """The pages of beam search's sequences after a selection: beam i of request r goes on from beam parents[r, i]
         (int32 [R, beams], rows may be strided, e.g. beam_select's first columns; -1: stays). pages [R * beams, width] and
         lens [R * beams] are the batch's, request by request; the beams of a request have one length. Returns the new
@@ -969,8 +972,13 @@ class Kernels:
         keeps its parent's; for the others its rows are copied, in every layer, to the pages of beams that ended. So
         neither pages nor copies are needed beyond the beams' own, and entries behind the last position stay each
         beam's. k_pages, v_pages: bf16 [n_pages, Hk, page_size, D] or all layers' [layers, n_pages, Hk, page_size,
-        D] (strides as in paged_append), or float8_e4m3fn with k_scales, v_scales as in paged_append_fp8. A repeated call
-        with the same arguments gives the same. The reference serves one sequence (qwen.py:166-177)."""
+        D] (strides as in paged_append), or float8_e4m3fn with k_scales, v_scales as in paged_append_fp8.
+
+        Whole pages that only ended beams had are in no row of the result. With ``free`` and ``n_free``, paged_reserve's stack, they
+        are pushed on it (request by request, column by column, then by beam; it needs room for every page). Without, a
+        repeated call with the same arguments gives the same, and the caller has to know which pages a request took. Pages that
+        rows of another request hold too must be in all of a request's rows. The reference serves one sequence
+        (qwen.py:166-177)."""
         here = _device_of(parents, "parents", torch.int32)
         _require_here(pages, "pages", torch.int32, here)
         _require_here(lens, "lens", torch.int32, here)
@@ -1019,6 +1027,13 @@ class Kernels:
                      strides[1] if n_pages > 1 else 0, strides[2] if Hk > 1 else 0)
         elif v_scales is not None:
             raise ValueError("v_scales without k_scales")
+        if free is not None or n_free is not None:
+            if free is None or n_free is None:
+                raise ValueError("free and n_free go together")
+            _require_here(free, "free", torch.int32, here)
+            _require_here(n_free, "n_free", torch.int32, here)
+            if free.dim() != 1 or not free.is_contiguous() or n_free.numel() != 1:
+                raise ValueError("free must be a contiguous [capacity] tensor and n_free hold one value")
         if out is None:
             out = pages.new_empty((rows, width))
         else:
@@ -1027,10 +1042,14 @@ class Kernels:
                 raise ValueError(f"out must be a contiguous [{rows}, {width}] tensor")
         if rows == 0:
             return out
-        rc = self.lib.ns_paged_reorder(
-            parents.data_ptr(), parent_stride, pages.data_ptr(), table_stride, width, lens.data_ptr(), out.data_ptr(), k_pages.data_ptr(),
-            v_pages.data_ptr(), *by, *marks, layers, n_pages, page_size, size * D, R, beams, Hk, _raw_stream(here))
-        self._check(rc, "ns_paged_reorder")
+        args = (parents.data_ptr(), parent_stride, pages.data_ptr(), table_stride, width, lens.data_ptr(), out.data_ptr(),
+                k_pages.data_ptr(), v_pages.data_ptr(), *by, *marks, layers, n_pages, page_size, size * D, R, beams, Hk)
+        if free is None:
+            rc = self.lib.ns_paged_reorder(*args, _raw_stream(here))
+            self._check(rc, "ns_paged_reorder")
+        else:
+            rc = self.lib.ns_paged_reorder_back(*args, free.data_ptr(), free.shape[0], n_free.data_ptr(), _raw_stream(here))
+            self._check(rc, "ns_paged_reorder_back")
         return out
 
     # ------------------------------------------------------------------ beam search
