@@ -1063,10 +1063,10 @@ class Kernels:
         """The n best continuations (at most 64) of R requests with up to 64 beams each: logits [R * beams, vocab] (bf16 or
         float32, request by request, rows may be strided, vocab at most 2^20), scores [R, beams] float32, the beams' sums of log
         probabilities so far. Returns (scores float32, tokens int32, parents int32), each [R, n]: the largest scores[r, i] +
-        log softmax(logits[r, i])[v], falling, with their v and i; equal ones by beam, then by token. A beam whose score is -inf
-        does not count (after the prompt: all but one). NaN counts as -inf and is never taken, +inf as the largest float32;
-        where fewer than n are left, -inf, -1 and -1. Scores are compared in float64; the sum below a logarithm is good to
-        some 2^-22, and beams whose scores lie closer than that may come in either order.
+        log softmax(logits[r, i])[v], falling, with their v and i; equal ones by beam, within a beam by falling logit, then by
+        token. A beam whose score is -inf does not count (after the prompt: all but one). NaN counts as -inf and is never taken,
+        +inf as the largest float32; where fewer than n are left, -inf, -1 and -1. Scores are compared in float64; the sum below
+        a logarithm is good to some 2^-22, and beams whose scores lie closer than that may come in either order.
         ``work``: from beam_select_workspace, allocated here when it is not given; ``out``: the three results. The
         reference decodes one sequence greedily (qwen.py:166-177)."""
         if not isinstance(logits, torch.Tensor):
