@@ -440,8 +440,8 @@ __device__ __forceinline__ void query_terms(const u32x4_t& q, int e, u32x2_t& hi
 // so that products and softmax still take turns for much of the time. Issuing one half block's softmax between the
 // products of its neighbours did not help (659 -> 681 to 730 us). 4095 tokens with a window of 1000 and 14 / 2 heads of
 // 64 43 us. 96 drafts of 1 to 3 tokens behind 16384 shared positions 100 to 104 us back to back, 108 to 117 among
-// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD. In 8 bits: 612 us (722 TFLOP/s),
-// 47.5 and 104, with one probability term 467, 41 and 94.
+// other launches: 220 workgroups of the shared keys, one to a CU, with one wave per SIMD. In 8 bits: 604 us (732 TFLOP/s),
+// 47.4 and 107, with one probability term 463, 41 and 94.
 template <int D, bool kShared, bool kF8 = false>
 __device__ __forceinline__ void tile_body(const PagedArgs& a, int item, int g, const Ring& lds, SharedRows& sh) {
   // (kRow: a row of the cache in units of 2 bytes)

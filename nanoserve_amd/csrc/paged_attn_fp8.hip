@@ -28,9 +28,9 @@ typedef long i64_t;
 //    8-bit LDS reads.
 //  * The first blocks' loads go out beside those of their scales, which depend on the page ids too (16 sequences 23.2 ->
 //    22.9 us), and probabilities come from v_exp_f32 as it is (22.7 -> 22.1).
-// Measured (28 / 4 heads of 128): 4 sequences of 98 000 71 us, 5.6 TB/s, the streaming launch 64.4 and 6.2; 16 of 33 to 8191
-// 21.9 us, 18 before the merge; 32 with a window of 4096 32.6; 64 of 1000 to 8000 69 (4.3 TB/s: the longest range is a third
-// above the mean one); one of 700 with 12 / 2 heads 10.9, the latency of length -> page -> scale and rows -> merge. Shares of
+// Measured (28 / 4 heads of 128): 4 sequences of 98 000 72 us, 5.5 TB/s, the streaming launch 65.2 and 6.1; 16 of 33 to 8191
+// 22.3 us, 18 before the merge; 32 with a window of 4096 32.7; 64 of 1000 to 8000 70 (4.3 TB/s: the longest range is a third
+// above the mean one); one of 700 with 12 / 2 heads 11.0, the latency of length -> page -> scale and rows -> merge. Shares of
 // equal size cut from all sequences end to end take 64 us there but 29 for 16 sequences and 23 for 64 of up to 100 (8.9), as a
 // workgroup then starts on two sequences or more; three or four workgroups per CU aimed at 26.8 and 26.8 for the 16.
 template <int D>
